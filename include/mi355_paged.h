@@ -433,6 +433,108 @@ int mi355_paged_prefill(void* out, const void* q, int64_t q_stride_tok,
 int32_t mi355_paged_prefill_max_context(int32_t dtype, int32_t D, int32_t block_size, int32_t max_q_len);
 
 /*
+ * ---------------------------------------------------------------------------------------------
+ * The 4-bit KV cache.  The reference keeps keys and values in the activations' type
+ * (01_paged_attention/paged_attention.py:30-51, 05_mini_vllm/mini_vllm.py:517-545); the entry
+ * points below are the same steps -- rotation and cache write :415-427, decode attention :460-481,
+ * prompt attention :437-458 -- over a cache of 17/64 of a 16-bit cache's bytes.
+ *
+ * Values are E2M1 codes (0 .5 1 1.5 2 3 4 6 and negatives) times one power of two per 32 dims of a
+ * token's head row, kept as an E8M0 byte (2^(byte - 127)): the smallest power with
+ * max|x| <= 6 * 2^e, e in [-120, 125] (larger values saturate); codes round to nearest, ties to the
+ * even code.  A block of 32 that holds a NaN or an infinity gets byte 255 and reads as NaN.
+ *   A cache is two byte tensors (K and V) of [num_blocks, Hkv, block_size / 16, 17 * D / 2]: per
+ *   block, head and tile of 16 tokens a record of 8 D bytes of codes followed by D / 2 scale bytes.
+ *     K record  codes [16 tokens][D / 2] (even dim in the low nibble), scales [16][D / 32]
+ *     V record  codes [4 g][16 c][D / 32][4 j]: byte = dims 32 b + 2 c (low nibble) and 32 b + 2 c + 1
+ *               of token 4 g + j; scales [4 g][D / 32][4 j]
+ *   stride_block, stride_head: BYTES between blocks / heads, multiples of 16, the same for K and V; a
+ *   head's tiles are contiguous.  D in {32, 64, 128, 256}; block_size a multiple of 16.
+ *   A slot (block * block_size + row) nobody wrote may hold anything: no result depends on it.
+ * ---------------------------------------------------------------------------------------------
+ */
+
+/*
+ * cos_out[t][i] = factor * cos(positions[t] * inv_freq[i]), sin_out likewise; both [T, half_dim]
+ * floats.  The product and its reduction are done in double (positions up to 2^53), so that far
+ * positions keep their angle; the reference's tables end at position 8191
+ * (RotaryEmbedding, 05_mini_vllm/mini_vllm.py:360-374).  One call serves every layer of a step.
+ *   positions [T] int64, inv_freq [half_dim] double (device memory)
+ */
+int mi355_rope_angles(float* cos_out, float* sin_out, const int64_t* positions, const double* inv_freq,
+                      double factor, int32_t T, int32_t half_dim, void* stream);
+
+/*
+ * Rotary embedding of the first rotary_dim dims of every head row, out of place; the other dims are
+ * copied.  Pairs are (i, i + rotary_dim / 2), or (2 i, 2 i + 1) when `interleaved`:
+ *   a' = a cos[t][i] - b sin[t][i],  b' = b cos[t][i] + a sin[t][i]      (one rounding per value)
+ *   out [T, H, D] contiguous; x [T, H, D], x_stride_tok elements between tokens, heads D apart;
+ *   cos_rows / sin_rows [T, rotary_dim / 2] floats, one row per token (mi355_rope_angles);
+ *   rotary_dim a multiple of 16 in [0, D] (0: cos_rows / sin_rows may be NULL); out must not
+ *   overlap x.  D in {32, 64, 128, 256}.
+ */
+int mi355_rope_rotate(void* out, const void* x, int64_t x_stride_tok, const float* cos_rows,
+                      const float* sin_rows, int32_t rotary_dim, int32_t interleaved, int32_t T, int32_t H,
+                      int32_t D, int32_t dtype, void* stream);
+
+/*
+ * mi355_rope_rotate of the query rows (to q_out [T, Hq, D]), and the rotated key rows and the value
+ * rows rounded into the 4-bit cache at slots[t]: one launch, q / k / v are read only and may be views
+ * of one projection output.  Keys are rotated in double and rounded once, to 4 bits, so that the
+ * codes are those of the real product.  Tokens whose slot is negative or >= num_blocks * block_size
+ * have no cache write (their query row is rotated all the same); two tokens must not share a slot.
+ */
+int mi355_rope_kv4_write(void* q_out, const void* q, const void* k, const void* v, int64_t q_stride_tok,
+                         int64_t k_stride_tok, int64_t v_stride_tok, const float* cos_rows,
+                         const float* sin_rows, int32_t rotary_dim, int32_t interleaved, const int64_t* slots,
+                         void* k_cache, void* v_cache, int32_t T, int32_t Hq, int32_t Hkv, int32_t D,
+                         int32_t block_size, int32_t num_blocks, int64_t stride_block, int64_t stride_head,
+                         int32_t dtype, void* stream);
+
+/*
+ * The cached rows of T slots as values: k_out, v_out [T, Hkv, D] contiguous.  A slot outside the
+ * cache gives zeros; bf16 and fp32 hold every cached value exactly.
+ */
+int mi355_kv4_read_slots(void* k_out, void* v_out, const void* k_cache, const void* v_cache,
+                         const int64_t* slots, int32_t T, int32_t Hkv, int32_t D, int32_t block_size,
+                         int32_t num_blocks, int64_t stride_block, int64_t stride_head, int32_t dtype,
+                         void* stream);
+
+/*
+ * mi355_paged_decode over the 4-bit cache: same arguments and meaning (out, q [B, Hq, D], tables,
+ * context_lens clamped to min(max_context, max_blocks * block_size), 0 gives zeros, ids clamped into
+ * the pool) but for the cache's strides.  Scores, softmax and sums are fp32; the cached values and
+ * the queries enter the products exactly, the softmax weights with 8 / 16 / 24 bits for bf16 / fp16 /
+ * fp32 queries.
+ */
+int mi355_paged_decode_kv4(void* out, const void* q, int64_t q_stride_seq, const void* k_cache,
+                           const void* v_cache, const int32_t* block_tables, const int32_t* context_lens,
+                           int32_t B, int32_t Hq, int32_t Hkv, int32_t D, int32_t block_size,
+                           int32_t max_blocks, int32_t num_blocks, int32_t max_context, int64_t stride_block,
+                           int64_t stride_head, float scale, int32_t dtype, void* workspace,
+                           size_t workspace_bytes, void* stream);
+
+/* Scratch bytes mi355_paged_decode_kv4 needs for this shape (max_context after its clamp); nothing is
+ * kept in it between calls, and calls that may overlap on the GPU must not share it. */
+size_t mi355_paged_decode_kv4_workspace_bytes(int32_t B, int32_t Hq, int32_t Hkv, int32_t D,
+                                              int32_t max_context, int32_t dtype);
+
+/*
+ * mi355_paged_prefill over the 4-bit cache: query token j of segment s attends to positions
+ * 0 .. seg_pos0[s] + j, whose rows (the segment's own among them) are in the cache.  Rows of out
+ * outside every segment are left as they are; a segment may be empty.  A value row that a query must
+ * not see never reaches it, NaN or not.  Precision as in mi355_paged_decode_kv4.
+ */
+int mi355_paged_prefill_kv4(void* out, const void* q, int64_t q_stride_tok, const void* k_cache,
+                            const void* v_cache, const int32_t* block_tables, const int32_t* seg_q_start,
+                            const int32_t* seg_len, const int32_t* seg_pos0, int32_t nseg, int32_t max_q_len,
+                            int32_t Hq, int32_t Hkv, int32_t D, int32_t block_size, int32_t max_blocks,
+                            int32_t num_blocks, int32_t max_context, int64_t stride_block, int64_t stride_head,
+                            float scale, int32_t dtype, void* workspace, size_t workspace_bytes, void* stream);
+size_t mi355_paged_prefill_kv4_workspace_bytes(int32_t nseg, int32_t total_rows, int32_t max_q_len, int32_t Hq,
+                                               int32_t Hkv, int32_t D, int32_t max_context, int32_t dtype);
+
+/*
  * Data-parallel exchange of the sampled token ids, one process per GPU, over RCCL (xGMI inside a
  * node).  No counterpart in the reference, which is single-process and single-device (its only
  * collective is a commented-out all-reduce, 03_moe/mini_moe.py:356-357): sequences are sharded

@@ -1,0 +1,531 @@
+"""The 4-bit KV cache's kernels against the float64 checker (needs an MI355X).
+
+Bounds, derived from how the kernels compute (u = 2^-24; a rounding to t is off by at most
+finfo(t).eps / 2 relative):
+  cached codes and scales   equal: keys are rotated in double and rounded once
+  rotated queries           two products and a sum: 2 u (|x cos| + |y sin|), and the rounding to the dtype
+  angles                    the float's rounding, and 2^-52 |angle| for the double product
+  attention                 scores: a dot product of D exact products in up to three pieces, accumulated in
+                            float: (3 D + 8) u S with S the largest sum |q| |k| |scale|; a score error d moves
+                            a softmax weight by 2 d; the weights enter the second product with 2^-8 (bf16),
+                            2^-16 (fp16) or 2^-24 (fp32); exp2 and the n-term sums add 2^-22 + 2 (n + 8) u.
+                            All of that times the weighted mean of |v|, plus the rounding of the result.
+"""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import kv4_oracle as orc
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+HALF = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+WEIGHT = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -16, torch.bfloat16: 2.0 ** -8}
+TINY = {torch.float32: 2.0 ** -149, torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -134}      # half a subnormal step
+ALL = [torch.float32, torch.bfloat16, torch.float16]
+
+
+@pytest.fixture(scope='module')
+def ops(device):
+    from mi355_paged import ops
+    return ops
+
+
+def _cast(x, dtype):
+    """float64 numpy -> (device tensor of dtype, its values in float64)."""
+    t = torch.from_numpy(np.asarray(x)).to(dtype)
+    return t.cuda(), t.double().numpy()
+
+
+def _near(got, want, bound):
+    got = got.double().cpu().numpy()
+    bad = ~(np.abs(got - want) <= bound)
+    assert not bad.any(), (f"{bad.sum()} of {bad.size} off, first at {np.argwhere(bad)[0]}: {got[bad][:4]} for {want[bad][:4]}, "
+                           f"allowed {np.broadcast_to(bound, want.shape)[bad][:4]}")
+
+
+# ------------------------------------------------------------------ angles
+@pytest.mark.parametrize('T,half', [(1, 8), (3, 1), (77, 24), (1025, 64)])
+def test_angles(ops, device, T, half):
+    rng = np.random.default_rng(T + half)
+    pos = rng.integers(0, 1 << 22, T)
+    pos[0] = 0
+    if T > 5:
+        pos[1:6] = [1, 8191, (1 << 31) + 5, (1 << 40) + 1, -7]
+    freq, factor = ops.rope_frequencies(2 * half, scaling={'kind': 'yarn', 'factor': 8, 'original': 4096})
+    cos, sin = ops.rope_angles(torch.from_numpy(pos).cuda(), freq.cuda(), factor)
+    assert cos.dtype == sin.dtype == torch.float32 and cos.shape == sin.shape == (T, half)
+    a = pos[:, None].astype(np.float64) * freq.numpy()
+    for got, want in ((cos, np.cos(a) * factor), (sin, np.sin(a) * factor)):
+        _near(got, want, U * np.abs(want) + factor * (2.0 ** -52 * np.abs(a) + 2e-11))
+
+
+def test_angles_refusals(ops, device):
+    pos, freq = torch.zeros(3, dtype=torch.int64, device=device), torch.ones(4, dtype=torch.float64, device=device)
+    with pytest.raises(TypeError):
+        ops.rope_angles(pos.int(), freq)
+    with pytest.raises(TypeError):
+        ops.rope_angles(pos, freq.float())
+    cos, sin = ops.rope_angles(pos[:0], freq)
+    assert cos.shape == (0, 4)
+
+
+# ------------------------------------------------------------------ rotation and append
+def _rows(rng, T, Hq, Hkv, D, dtype):
+    """q, k, v as views of one projection output, and their values."""
+    x = rng.standard_normal((T, (Hq + 2 * Hkv) * D)) * np.exp2(rng.integers(-3, 4, (Hq + 2 * Hkv) * D))
+    t, val = _cast(x, dtype)
+    cut = [Hq * D, Hkv * D, Hkv * D]
+    views = [c.view(T, -1, D) for c in t.split(cut, -1)]
+    vals = [c.reshape(T, -1, D) for c in np.split(val, np.cumsum(cut)[:-1], -1)]
+    return views, vals
+
+
+def _angle_rows(ops, rng, T, R):
+    if R == 0:
+        return None, None, np.zeros((T, 0)), np.zeros((T, 0))
+    freq, _ = ops.rope_frequencies(R)
+    cos, sin = ops.rope_angles(torch.from_numpy(rng.integers(0, 100000, T)).cuda(), freq.cuda())
+    return cos, sin, cos.double().cpu().numpy(), sin.double().cpu().numpy()
+
+
+def _rotation_bound(x, cos, sin, inter, dtype, want):
+    size = orc.rotate(np.abs(x), np.abs(cos), -np.abs(sin), inter)      # |a c| + |b s| for the first of a pair
+    other = orc.rotate(np.abs(x), np.abs(cos), np.abs(sin), inter)      # ... and for the second
+    return 2 * U * np.maximum(np.abs(size), np.abs(other)) * (1 + HALF[dtype]) + HALF[dtype] * np.abs(want) + TINY[dtype]
+
+
+@pytest.mark.parametrize('dtype', ALL)
+@pytest.mark.parametrize('T,Hq,Hkv,D,BS,R,inter', [
+    (1, 8, 8, 64, 16, 64, False), (37, 8, 2, 128, 16, 128, True), (50, 4, 4, 32, 32, 16, False), (19, 6, 3, 256, 48, 64, True),
+    (64, 7, 1, 64, 64, 32, False), (300, 2, 2, 32, 16, 32, True), (33, 3, 3, 128, 16, 0, False)])
+def test_append_rounds_rotates_and_scatters(ops, device, dtype, T, Hq, Hkv, D, BS, R, inter):
+    rng = np.random.default_rng(T * 1000 + D + Hq)
+    (q, k, v), (qv, kv, vv) = _rows(rng, T, Hq, Hkv, D, dtype)
+    cos, sin, cv, sv = _angle_rows(ops, rng, T, R)
+    NB = -(-T // BS) + 3
+    slots = rng.permutation(NB * BS)[:T]
+    if T > 4:
+        slots[2], slots[4] = -1, NB * BS                       # skipped
+    old = [rng.integers(0, 256, ops.kv4_cache_shape(NB, Hkv, BS, D)).astype(np.uint8) for _ in range(2)]
+    kc, vc = (torch.from_numpy(o).cuda() for o in old)
+    before = [t.clone() for t in (q, k, v)]
+    out = ops.rope_kv4_write(q, k, v, cos, sin, torch.from_numpy(slots).cuda(), kc, vc, interleaved=inter)
+    assert all(torch.equal(a, b) for a, b in zip(before, (q, k, v)))
+    want = orc.rotate(qv, cv, sv, inter)
+    _near(out, want, _rotation_bound(qv, cv, sv, inter, dtype, want))
+    want = [old[0].copy(), old[1].copy()]
+    for form, x in enumerate((orc.rotate(kv, cv, sv, inter), vv)):
+        code, byte = orc.quantise(x)
+        for t in range(T):
+            if 0 <= slots[t] < NB * BS:
+                blk, at = divmod(int(slots[t]), BS)
+                for h in range(Hkv):
+                    orc.write_row(want[form][blk, h, at // 16], at % 16, code[t, h], byte[t, h], bool(form))
+    for got, w in ((kc, want[0]), (vc, want[1])):
+        np.testing.assert_array_equal(got.cpu().numpy(), w)    # written rows and every byte beside them
+    # the same rows read back, at an invalid slot zeros
+    rk, rv = ops.kv4_read_slots(kc, vc, torch.from_numpy(slots).cuda(), torch.float32)
+    for form, got in enumerate((rk, rv)):
+        for t in range(T):
+            if 0 <= slots[t] < NB * BS:
+                blk, at = divmod(int(slots[t]), BS)
+                values = orc.unpack(want[form][blk, :, at // 16], bool(form))[:, at % 16]
+                np.testing.assert_array_equal(got[t].double().cpu().numpy(), values)
+            else:
+                assert not got[t].any()
+
+
+def test_append_values_at_borders_extremes_and_nan(ops, device):
+    D, T = 64, 9
+    x = np.zeros((T, 1, D))
+    x[0, 0, :16] = [6, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5, -0.25, -0.75, -5, 0.2500001, 0.7499999, 4.9999995, 5.0000005, -0.0]
+    x[1, 0, :4] = [3.4e38, 1.0, -3.4e38, 1e30]                 # saturates at 6 * 2^125
+    x[2, 0, :4] = [1e-38, 1e-40, -1e-36, 2e-36]                # below the smallest scale
+    x[3, 0, 5] = np.nan
+    x[4, 0, 40] = np.inf                                       # only its own block of 32 reads as NaN
+    x[5, 0, :3] = [6.0000005, 1, 2]
+    x[6] = 0.0
+    x[7, 0, :32] = 2.0 ** -126
+    x[8, 0, 33] = -np.inf
+    t, val = _cast(x, torch.float32)
+    kc, vc = (torch.zeros(ops.kv4_cache_shape(1, 1, 16, D), dtype=torch.uint8, device=device) for _ in range(2))
+    out = ops.rope_kv4_write(t, t, t, None, None, torch.arange(T, device=device), kc, vc)
+    assert torch.equal(out.view(torch.int32), t.view(torch.int32))
+    code, byte = orc.quantise(val)
+    want = orc.dequantise(code, byte)
+    rk, rv = ops.kv4_read_slots(kc, vc, torch.arange(T, device=device), torch.float32)
+    np.testing.assert_array_equal(rk.double().cpu().numpy(), want)
+    np.testing.assert_array_equal(rv.double().cpu().numpy(), want)
+    half, _ = ops.kv4_read_slots(kc, vc, torch.arange(1, device=device), torch.float16)
+    np.testing.assert_array_equal(half.double().cpu().numpy(), want[:1])
+
+
+@pytest.mark.parametrize('dtype', ALL)
+@pytest.mark.parametrize('T,H,D,R,inter', [(1, 1, 32, 32, False), (41, 5, 64, 48, True), (7, 3, 256, 128, False), (9, 2, 128, 0, False)])
+def test_rotate(ops, device, dtype, T, H, D, R, inter):
+    rng = np.random.default_rng(T + R)
+    wide, val = _cast(rng.standard_normal((T, (H + 1) * D)), dtype)
+    x, xv = wide[:, D:].view(T, H, D), val[:, D:].reshape(T, H, D)
+    cos, sin, cv, sv = _angle_rows(ops, rng, T, R)
+    want = orc.rotate(xv, cv, sv, inter)
+    out = torch.full((T, H, D), math.nan, dtype=dtype, device=device)
+    assert ops.rope_rotate(x, cos, sin, inter, out=out) is out
+    _near(out, want, _rotation_bound(xv, cv, sv, inter, dtype, want))
+    assert torch.equal(out[..., R:], x[..., R:])
+
+
+def test_append_refusals(ops, device):
+    kc, vc = (torch.zeros(ops.kv4_cache_shape(4, 2, 16, 64), dtype=torch.uint8, device=device) for _ in range(2))
+    x = torch.zeros(3, 2, 64, device=device, dtype=torch.bfloat16)
+    cs = torch.zeros(3, 32, device=device)
+    slots = torch.arange(3, device=device)
+    for bad in (dict(k=x[:2]), dict(v=x[:, :1]), dict(k_cache=kc[:2]), dict(slots=slots[:2].int()), dict(slots=slots[:2]),
+                dict(cos=None), dict(cos=cs[:2], sin=cs[:2]), dict(cos=cs.double(), sin=cs.double()), dict(q=x.float()),
+                dict(q=torch.zeros(3, 2, 128, device=device, dtype=torch.bfloat16)), dict(k_cache=kc.int(), v_cache=vc.int()),
+                dict(out=torch.empty(3, 2, 64, device=device)), dict(q=x.transpose(0, 1)),
+                dict(k_cache=kc[..., :500], v_cache=vc[..., :500])):
+        args = dict(q=x, k=x, v=x, cos=cs, sin=cs, slots=slots, k_cache=kc, v_cache=vc)
+        with pytest.raises((TypeError, ValueError)):
+            ops.rope_kv4_write(**dict(args, **bad))
+    from mi355_paged._lib import Mi355Error
+    odd = torch.zeros(3 * 128 + 1, device=device, dtype=torch.bfloat16)[1:].view(3, 2, 64)
+    with pytest.raises(Mi355Error, match='aligned'):
+        ops.rope_kv4_write(odd, x, x, cs, cs, slots, kc, vc)
+    with pytest.raises(Mi355Error, match='rotary_dim'):
+        ops.rope_rotate(x, cs[:, :12].contiguous(), cs[:, :12].contiguous())
+    assert ops.rope_kv4_write(x[:0], x[:0], x[:0], cs[:0], cs[:0], slots[:0], kc, vc).shape == (0, 2, 64)
+
+
+# ------------------------------------------------------------------ caches for the attention tests
+def _cache(rng, lens, Hkv, D, BS, spare=2, fill=255):
+    """(K records, V records, block tables) of sequences with `lens` cached tokens; rows nobody wrote hold `fill`."""
+    need = [-(-n // BS) for n in lens]
+    NB = sum(need) + spare
+    order = rng.permutation(NB)
+    width = max(max(need), 1)
+    tables = np.full((len(lens), width), NB + 7, dtype=np.int32)     # entries nobody may follow
+    caches = []
+    at = 0
+    for i, n in enumerate(need):
+        tables[i, :n] = order[at:at + n]
+        at += n
+    for form in (False, True):
+        x = rng.standard_normal((NB, Hkv, BS // 16, 16, D)) * np.exp2(0.5 * rng.standard_normal(D))
+        rec = orc.pack(*orc.quantise(x), form)
+        empty = np.full(orc.record_bytes(D), fill, dtype=np.uint8)
+        used = np.zeros((NB, BS), dtype=bool)
+        for i, n in enumerate(lens):
+            for t in range(n):
+                used[tables[i, t // BS], t % BS] = True
+        for blk in range(NB):
+            for t in range(BS):
+                if not used[blk, t]:
+                    for h in range(Hkv):
+                        r = rec[blk, h, t // 16]
+                        for d in range(D):
+                            a, s = orc.code_place(D, t % 16, d, form)
+                            r[a] = (int(r[a]) & (0xF0 >> s)) | (int(empty[a]) & (15 << s))
+                        for b in range(D // 32):
+                            r[orc.scale_place(D, t % 16, b, form)] = fill
+        caches.append(rec)
+    return caches[0], caches[1], tables
+
+
+def _attend_all(q, kc, vc, tables, lens, scale, limits):
+    """q [rows of one sequence each: list of [n, Hq, D]]; limits [list of [n]] -> out, size, big as lists."""
+    res = []
+    for i, (qi, lim) in enumerate(zip(q, limits)):
+        Hkv, Hq = kc.shape[1], qi.shape[1]
+        G = Hq // Hkv
+        o, s, b = np.zeros(qi.shape), np.zeros(qi.shape), np.zeros(qi.shape[:2] + (1,))
+        for h in range(Hkv):
+            if lens[i] == 0:
+                continue
+            k, v = orc.gather(kc, tables[i], lens[i], h, False), orc.gather(vc, tables[i], lens[i], h, True)
+            for g in range(G):
+                o[:, h * G + g], s[:, h * G + g], b[:, h * G + g] = orc.attend(qi[:, h * G + g], k, v, scale, lim)
+        res.append((o, s, b))
+    return [np.concatenate([r[j] for r in res]) for j in range(3)]
+
+
+def _attention_bound(size, big, want, D, n, dtype):
+    return (2 * (3 * D + 8) * U * big + 2.0 ** -22 + 2 * (n + 8) * U + WEIGHT[dtype]) * size + \
+        (HALF[dtype] + 2 * (n + 8) * U) * np.abs(want) + 1e-30
+
+
+DECODE = [
+    # Hq, Hkv, D, BS, context lengths
+    (8, 8, 64, 16, [1, 2, 15, 16, 17, 0, 31, 32, 33, 37]),
+    (8, 8, 32, 32, [127, 128, 129, 1, 0, 200]),
+    (32, 8, 128, 16, [50, 257]),
+    (14, 2, 64, 48, [300, 7, 48]),
+    (6, 6, 256, 16, [65, 16]),
+    (3, 3, 64, 16, [140]),
+    (16, 1, 128, 64, [33, 500]),
+    (20, 1, 64, 16, [70]),
+    (40, 2, 32, 16, [90, 3]),
+    (8, 4, 256, 16, [20]),
+    (5, 5, 128, 16, [0, 0]),
+    (8, 8, 64, 16, [1900, 40]),
+]
+
+
+@pytest.mark.parametrize('dtype', ALL)
+@pytest.mark.parametrize('Hq,Hkv,D,BS,lens', DECODE, ids=lambda v: str(v))
+def test_decode(ops, device, dtype, Hq, Hkv, D, BS, lens):
+    rng = np.random.default_rng(Hq * 131 + D + sum(lens))
+    kc, vc, tables = _cache(rng, lens, Hkv, D, BS)
+    B = len(lens)
+    wide, val = _cast(rng.standard_normal((B, (Hq + 1) * D)) * 1.5, dtype)
+    q, qv = wide[:, D:].view(B, Hq, D), val[:, D:].reshape(B, Hq, D)
+    scale = D ** -0.5
+    want, size, big = _attend_all([qv[i:i + 1] for i in range(B)], kc, vc, tables, lens, scale, [[n - 1] for n in lens])
+    out = ops.paged_decode_kv4(q, torch.from_numpy(kc).cuda(), torch.from_numpy(vc).cuda(), torch.from_numpy(tables).cuda(),
+                               torch.tensor(lens, dtype=torch.int32, device=device), max(lens))
+    _near(out, want, _attention_bound(size, big, want, D, max(lens), dtype))
+    for i, n in enumerate(lens):
+        if n == 0:
+            assert not out[i].any()
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+def test_decode_long_context_split_and_bounds(ops, device, dtype):
+    """Many splits (some of them empty), a max_context far above and one below the contexts."""
+    rng = np.random.default_rng(3)
+    lens, Hq, Hkv, D, BS = [9001, 130, 0, 4097], 4, 2, 64, 16
+    kc, vc, tables = _cache(rng, lens, Hkv, D, BS)
+    q, qv = _cast(rng.standard_normal((4, Hq, D)), dtype)
+    args = [torch.from_numpy(a).cuda() for a in (kc, vc, tables)]
+    ctx = torch.tensor(lens, dtype=torch.int32, device=device)
+    for bound in (9001, 100000, 4100):
+        seen = [min(n, bound) for n in lens]
+        want, size, big = _attend_all([qv[i:i + 1] for i in range(4)], kc, vc, tables, seen, D ** -0.5, [[n - 1] for n in seen])
+        out = ops.paged_decode_kv4(q, *args, ctx, bound)
+        _near(out, want, _attention_bound(size, big, want, D, max(lens), dtype))
+    again = ops.paged_decode_kv4(q, *args, ctx, 4100)
+    assert torch.equal(again, out)
+
+
+def test_decode_scale_out_and_strided_caches(ops, device):
+    """A layer's caches as a slice of one pool with heads of another order, a scale of either sign, out=."""
+    rng = np.random.default_rng(8)
+    lens, Hq, Hkv, D, BS = [100, 23], 8, 4, 64, 32
+    kc, vc, tables = _cache(rng, lens, Hkv, D, BS)
+    pool = torch.zeros((Hkv, 3, 2) + kc.shape[:1] + kc.shape[2:], dtype=torch.uint8, device=device)   # [H, layer, K/V, NB, tiles, bytes]
+    pool[:, 1, 0] = torch.from_numpy(kc).cuda().transpose(0, 1)
+    pool[:, 1, 1] = torch.from_numpy(vc).cuda().transpose(0, 1)
+    k, v = pool[:, 1, 0].transpose(0, 1), pool[:, 1, 1].transpose(0, 1)
+    q, qv = _cast(rng.standard_normal((2, Hq, D)), torch.bfloat16)
+    for scale in (0.3, -0.2, 0.0):
+        want, size, big = _attend_all([qv[i:i + 1] for i in range(2)], kc, vc, tables, lens, scale, [[n - 1] for n in lens])
+        out = torch.full((2, Hq, D), math.nan, dtype=torch.bfloat16, device=device)
+        got = ops.paged_decode_kv4(q, k, v, torch.from_numpy(tables).cuda(),
+                                   torch.tensor(lens, dtype=torch.int32, device=device), 100, scale=scale, out=out)
+        assert got is out
+        _near(out, want, _attention_bound(size, big, want, D, 100, torch.bfloat16))
+
+
+def test_decode_nan_stays_in_its_head_and_large_scores(ops, device):
+    rng = np.random.default_rng(4)
+    lens, Hq, Hkv, D, BS = [77], 8, 8, 64, 16
+    kc, vc, tables = _cache(rng, lens, Hkv, D, BS)
+    kc[tables[0, 2], 3, 0, orc.scale_place(D, 5, 0, False)] = 255          # a key of head 3, a value block of head 6
+    vc[tables[0, 0], 6, 0, orc.scale_place(D, 1, 1, True)] = 255
+    q, qv = _cast(rng.standard_normal((1, Hq, D)) * 300, torch.float32)
+    args = [torch.from_numpy(a).cuda() for a in (kc, vc, tables)]
+    out = ops.paged_decode_kv4(q, *args, torch.tensor(lens, dtype=torch.int32, device=device), 77)
+    want, size, big = _attend_all([qv], kc, vc, tables, lens, D ** -0.5, [[76]])
+    nan = np.isnan(out.cpu().numpy())
+    assert nan[0, 3].all() and nan[0, 6, 32:].all() and nan.sum() == D + 32
+    keep = [h for h in range(Hq) if h not in (3, 6)]
+    _near(out[:, keep], want[:, keep], _attention_bound(size, big, want, D, 77, torch.float32)[:, keep])
+
+
+def test_attention_refusals(ops, device):
+    kc, vc = (torch.zeros(ops.kv4_cache_shape(4, 2, 16, 64), dtype=torch.uint8, device=device) for _ in range(2))
+    q = torch.zeros(3, 4, 64, device=device, dtype=torch.bfloat16)
+    bt, ctx = torch.zeros(3, 2, dtype=torch.int32, device=device), torch.ones(3, dtype=torch.int32, device=device)
+    for bad in (dict(block_tables=bt[:2]), dict(block_tables=bt.long()), dict(context_lens=ctx[:1]), dict(context_lens=ctx.long()),
+                dict(q=q[..., :32].contiguous()), dict(q=q.double()), dict(out=q[:2]), dict(v_cache=vc[:3]),
+                dict(k_cache=kc.transpose(0, 1))):
+        with pytest.raises((TypeError, ValueError)):
+            ops.paged_decode_kv4(**dict(dict(q=q, k_cache=kc, v_cache=vc, block_tables=bt, context_lens=ctx, max_context=5), **bad))
+    seg = dict(seg_q_start=ctx, seg_len=ctx, seg_pos0=ctx)
+    for bad in (dict(block_tables=bt[:2]), dict(seg_len=ctx.long()), dict(seg_pos0=ctx[:2]), dict(q=q.transpose(0, 1)),
+                dict(out=q.float()), dict(q=q[..., :32].contiguous())):
+        with pytest.raises((TypeError, ValueError)):
+            ops.paged_prefill_kv4(**dict(dict(q=q, k_cache=kc, v_cache=vc, block_tables=bt, max_q_len=1, max_context=5, **seg), **bad))
+    from mi355_paged._lib import Mi355Error
+    with pytest.raises(Mi355Error, match='bad shape'):
+        ops.paged_decode_kv4(q[:, :3].contiguous(), kc, vc, bt, ctx, 5)
+
+
+# ------------------------------------------------------------------ prompt chunks
+CHUNKS = [
+    # Hq, Hkv, D, BS, chunk lengths, first positions
+    (8, 8, 64, 16, [1, 5, 0, 40], [0, 30, 12, 0]),
+    (8, 2, 128, 16, [33, 64], [100, 0]),
+    (4, 4, 32, 32, [130, 3], [0, 260]),
+    (7, 1, 64, 48, [50], [77]),
+    (2, 2, 256, 16, [20, 17], [5, 0]),
+    (32, 1, 64, 16, [9, 1], [0, 40]),
+    (3, 3, 128, 64, [300], [0]),
+    (8, 8, 64, 16, [2, 1], [1500, 900]),
+]
+
+
+@pytest.mark.parametrize('dtype', ALL)
+@pytest.mark.parametrize('Hq,Hkv,D,BS,lens,pos0', CHUNKS, ids=lambda v: str(v))
+def test_chunks(ops, device, dtype, Hq, Hkv, D, BS, lens, pos0):
+    rng = np.random.default_rng(Hq + D + sum(lens))
+    total = [n + p for n, p in zip(lens, pos0)]
+    kc, vc, tables = _cache(rng, total, Hkv, D, BS)
+    start, rows = [], 2                                        # rows before, between and behind the segments
+    for n in lens:
+        start.append(rows)
+        rows += n + 1
+    wide, val = _cast(rng.standard_normal((rows, (Hq + 1) * D)) * 1.5, dtype)
+    q, qv = wide[:, D:].view(rows, Hq, D), val[:, D:].reshape(rows, Hq, D)
+    want, size, big = _attend_all([qv[s:s + n] for s, n in zip(start, lens)], kc, vc, tables, total, D ** -0.5,
+                                  [[p + j for j in range(n)] for n, p in zip(lens, pos0)])
+    out = torch.full((rows, Hq, D), 7.0, dtype=dtype, device=device)
+    meta = torch.tensor([start, lens, pos0], dtype=torch.int32, device=device)
+    got = ops.paged_prefill_kv4(q, torch.from_numpy(kc).cuda(), torch.from_numpy(vc).cuda(), torch.from_numpy(tables).cuda(),
+                                meta[0], meta[1], meta[2], max(lens), max(total), out=out)
+    assert got is out
+    inside = np.concatenate([np.arange(s, s + n) for s, n in zip(start, lens)])
+    outside = np.setdiff1d(np.arange(rows), inside)
+    assert bool((out[torch.from_numpy(outside).cuda()] == 7.0).all())
+    _near(out[torch.from_numpy(inside).cuda()], want, _attention_bound(size, big, want, D, max(total), dtype))
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16])
+def test_chunk_long_context_few_rows(ops, device, dtype):
+    rng = np.random.default_rng(12)
+    lens, pos0, Hq, Hkv, D, BS = [5, 1, 40], [7000, 0, 2500], 4, 2, 64, 16
+    total = [n + p for n, p in zip(lens, pos0)]
+    kc, vc, tables = _cache(rng, total, Hkv, D, BS)
+    q, qv = _cast(rng.standard_normal((sum(lens), Hq, D)), dtype)
+    start = [0, 5, 6]
+    want, size, big = _attend_all([qv[s:s + n] for s, n in zip(start, lens)], kc, vc, tables, total, D ** -0.5,
+                                  [[p + j for j in range(n)] for n, p in zip(lens, pos0)])
+    args = [torch.from_numpy(a).cuda() for a in (kc, vc, tables)]
+    meta = torch.tensor([start, lens, pos0], dtype=torch.int32, device=device)
+    for bound in (7005, 50000):
+        out = ops.paged_prefill_kv4(q, *args, meta[0], meta[1], meta[2], 40, bound)
+        _near(out, want, _attention_bound(size, big, want, D, 7005, dtype))
+
+
+def test_chunk_nan_reaches_only_the_queries_that_see_it(ops, device):
+    """A NaN key or value at a position of the chunk itself: the queries before it stay finite, whatever
+    else shares their tiles."""
+    rng = np.random.default_rng(5)
+    n, p0, Hq, Hkv, D, BS = 45, 10, 4, 2, 64, 16
+    kc, vc, tables = _cache(rng, [n + p0], Hkv, D, BS)
+    q, qv = _cast(rng.standard_normal((n, Hq, D)), torch.float32)
+    at = 36
+    vc[tables[0, at // BS], 1, 0, orc.scale_place(D, at % 16, 0, True)] = 255       # dims 0..31 of head 1
+    kc[tables[0, 50 // BS], 0, 0, orc.scale_place(D, 50 % 16, 1, False)] = 255       # a key of head 0, position 50
+    args = [torch.from_numpy(a).cuda() for a in (kc, vc, tables)]
+    meta = torch.tensor([[0], [n], [p0]], dtype=torch.int32, device=device)
+    out = ops.paged_prefill_kv4(q, *args, meta[0], meta[1], meta[2], n, n + p0)
+    want, size, big = _attend_all([qv], kc, vc, tables, [n + p0], D ** -0.5, [[p0 + j for j in range(n)]])
+    nan = np.isnan(out.cpu().numpy())
+    expect = np.zeros(nan.shape, dtype=bool)
+    expect[at - p0:, 2:, :32] = True
+    expect[50 - p0:, :2] = True
+    np.testing.assert_array_equal(nan, expect)
+    bound = _attention_bound(size, big, want, D, n + p0, torch.float32)
+    _near(torch.where(torch.isnan(out), torch.zeros_like(out), out), np.where(expect, 0.0, want), np.where(expect, 1.0, bound))
+
+
+# ------------------------------------------------------------------ streams, graphs, all of them together
+def _step(ops, s):
+    """One layer's work on new rows: angles, rotation + append, attention."""
+    cos, sin = ops.rope_angles(s['pos'], s['freq'])
+    q = ops.rope_kv4_write(s['q'], s['k'], s['v'], cos, sin, s['slots'], s['kc'], s['vc'])
+    if s['meta'] is None:
+        return ops.paged_decode_kv4(q, s['kc'], s['vc'], s['tables'], s['ctx'], s['bound'])
+    return ops.paged_prefill_kv4(q, s['kc'], s['vc'], s['tables'], s['meta'][0], s['meta'][1], s['meta'][2], s['longest'], s['bound'])
+
+
+def _sequence_state(ops, rng, dtype, lens, new, Hq, Hkv, D, BS, decode):
+    """Sequences that hold lens[i] tokens of which the last new[i] are about to be appended."""
+    kc, vc, tables = _cache(rng, lens, Hkv, D, BS)
+    pos = np.concatenate([np.arange(n - m, n) for n, m in zip(lens, new)])
+    slots = np.concatenate([tables[i, np.arange(n - m, n) // BS].astype(np.int64) * BS + np.arange(n - m, n) % BS
+                            for i, (n, m) in enumerate(zip(lens, new))])
+    (q, k, v), vals = _rows(rng, len(pos), Hq, Hkv, D, dtype)
+    freq, _ = ops.rope_frequencies(D)
+    start = np.cumsum([0] + list(new))[:-1]
+    meta = None if decode else torch.tensor(np.array([start, new, [n - m for n, m in zip(lens, new)]]), dtype=torch.int32).cuda()
+    s = dict(q=q, k=k, v=v, pos=torch.from_numpy(pos).cuda(), slots=torch.from_numpy(slots).cuda(), freq=freq.cuda(),
+             kc=torch.from_numpy(kc).cuda(), vc=torch.from_numpy(vc).cuda(), tables=torch.from_numpy(tables).cuda(),
+             ctx=torch.tensor(lens, dtype=torch.int32).cuda(), bound=max(lens), meta=meta, longest=max(new))
+    return s, vals, kc, vc, tables, pos, slots
+
+
+def _expected(vals, kc, vc, tables, pos, slots, freq, lens, new, D, BS, dtype):
+    """The step in float64: rotation with float32 angle rows, 4-bit rows written, attention of rounded queries."""
+    a = pos[:, None] * freq
+    cos, sin = np.cos(a).astype(np.float32).astype(np.float64), np.sin(a).astype(np.float32).astype(np.float64)
+    qv, kv, vv = vals
+    kc, vc = kc.copy(), vc.copy()
+    for form, (cache, x) in enumerate(((kc, orc.rotate(kv, cos, sin, False)), (vc, vv))):
+        code, byte = orc.quantise(x)
+        for t, slot in enumerate(slots):
+            for h in range(cache.shape[1]):
+                orc.write_row(cache[slot // BS, h, slot % BS // 16], slot % 16, code[t, h], byte[t, h], bool(form))
+    q = torch.from_numpy(orc.rotate(qv, cos, sin, False)).to(dtype).double().numpy()
+    cut = np.split(q, np.cumsum(new)[:-1])
+    return _attend_all(cut, kc, vc, tables, lens, D ** -0.5, [list(range(n - m, n)) for n, m in zip(lens, new)])
+
+
+@pytest.mark.parametrize('decode', [True, False])
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+def test_a_layers_step_together(ops, device, dtype, decode):
+    rng = np.random.default_rng(21)
+    lens, new = [70, 1, 33, 200], [1, 1, 1, 1] if decode else [9, 1, 33, 50]
+    Hq, Hkv, D, BS = 8, 4, 64, 16
+    s, vals, kc, vc, tables, pos, slots = _sequence_state(ops, rng, dtype, lens, new, Hq, Hkv, D, BS, decode)
+    want, size, big = _expected(vals, kc, vc, tables, pos, slots, s['freq'].cpu().numpy(), lens, new, D, BS, dtype)
+    # a query off by one rounding of its dtype moves a score by HALF * big (an angle's last bit flips 4-bit codes too
+    # rarely to meet one here: 2^-24 of the values lie that near a border)
+    slack = 4 * HALF[dtype] * big * size
+    _near(_step(ops, s), want, _attention_bound(size, big, want, D, max(lens), dtype) + slack)
+
+
+@pytest.mark.parametrize('decode', [True, False])
+def test_captured_and_replayed(ops, device, decode):
+    """The step as a graph, replayed on new inputs between eager work of other shapes that grows the shared
+    workspace, and on a stream of its own."""
+    rng = np.random.default_rng(30)
+    lens, new = [3000, 64, 900], [1, 1, 1] if decode else [2, 64, 20]
+    mk = lambda: _sequence_state(ops, rng, torch.bfloat16, lens, new, 8, 4, 64, 16, decode)[0]
+    s, fresh = mk(), [mk() for _ in range(3)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        _step(ops, s)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = _step(ops, s)
+    big = _sequence_state(ops, rng, torch.bfloat16, [6000, 5000], [1, 1], 8, 4, 64, 16, True)[0]
+    for f in fresh:
+        for name in ('q', 'k', 'v', 'pos', 'slots', 'kc', 'vc', 'tables', 'ctx'):
+            s[name].copy_(f[name])
+        graph.replay()
+        _step(ops, big)                       # eager, larger: a workspace shared with the graph would be overwritten
+        got = out.clone()
+        torch.cuda.synchronize()
+        assert torch.equal(got, _step(ops, f))
+        assert torch.equal(s['kc'], f['kc']) and torch.equal(s['vc'], f['vc'])
+    with torch.cuda.stream(side):
+        other = _step(ops, fresh[0])
+    side.synchronize()
+    assert torch.equal(other, _step(ops, fresh[0]))

@@ -7,7 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_uint64, c_void_p
+from ctypes import c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_size_t, c_uint64, c_void_p
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # MI355_PAGED_LIB selects another build of the same library (kernel tuning experiments)
@@ -74,6 +74,27 @@ SIGNATURES = {
     'mi355_rmsnorm': (c_int, [
         c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_float, c_int32, c_int32,
         c_int32, c_void_p]),
+    'mi355_rope_angles': (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_double, c_int32, c_int32, c_void_p]),
+    'mi355_rope_rotate': (c_int, [
+        c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32,
+        c_void_p]),
+    'mi355_rope_kv4_write': (c_int, [
+        c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int32, c_int32,
+        c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int64, c_int64,
+        c_int32, c_void_p]),
+    'mi355_kv4_read_slots': (c_int, [
+        c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32, c_int32,
+        c_int64, c_int64, c_int32, c_void_p]),
+    'mi355_paged_decode_kv4': (c_int, [
+        c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32,
+        c_int32, c_int32, c_int32, c_int32, c_int64, c_int64, c_float, c_int32, c_void_p, c_size_t, c_void_p]),
+    'mi355_paged_decode_kv4_workspace_bytes': (c_size_t, [c_int32, c_int32, c_int32, c_int32, c_int32, c_int32]),
+    'mi355_paged_prefill_kv4': (c_int, [
+        c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32,
+        c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int64, c_int64, c_float, c_int32,
+        c_void_p, c_size_t, c_void_p]),
+    'mi355_paged_prefill_kv4_workspace_bytes': (c_size_t, [
+        c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32]),
     'mi355_dp_unique_id': (c_int, [c_void_p]),
     'mi355_dp_init': (c_int, [c_void_p, c_int32, c_int32, c_void_p]),
     'mi355_dp_allgather_i32': (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),

@@ -760,3 +760,262 @@ def paged_prefill(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
             float(scale), dtype_code(q), _stream(dev))
     _lib.check(rc, 'mi355_paged_prefill')
     return out
+
+
+# ---------------------------------------------------------------------------
+# the 4-bit KV cache (E2M1 codes, one E8M0 scale per 32 dims; record layout: include/mi355_paged.h)
+# ---------------------------------------------------------------------------
+
+KV4_HEAD_DIMS = (32, 64, 128, 256)
+KV4_TILE = 16          # tokens per record; a block holds a whole number of them
+
+
+def kv4_cache_shape(num_blocks: int, kv_heads: int, block_size: int, head_dim: int) -> Tuple[int, int, int, int]:
+    """Shape of one uint8 cache tensor (K and V have one each): 17 * head_dim / 2 bytes per head and 16
+    tokens.  Slots nobody wrote may hold anything, so torch.empty will do."""
+    if head_dim not in KV4_HEAD_DIMS:
+        raise ValueError(f"the 4-bit cache holds head_dim {KV4_HEAD_DIMS}, not {head_dim}")
+    if block_size <= 0 or block_size % KV4_TILE:
+        raise ValueError(f"the 4-bit cache keeps tiles of {KV4_TILE} tokens: block_size {block_size} is no multiple")
+    return num_blocks, kv_heads, block_size // KV4_TILE, 17 * head_dim // 2
+
+
+def _kv4_geometry(k_cache: torch.Tensor, v_cache: torch.Tensor):
+    """(num_blocks, kv_heads, block_size, head_dim, block stride, head stride) of a pair of cache tensors."""
+    shape = k_cache.shape
+    if k_cache.dtype != torch.uint8 or v_cache.dtype != torch.uint8:
+        raise TypeError("4-bit caches are uint8 tensors")
+    if len(shape) != 4 or shape != v_cache.shape or (shape[3] * 2) % 17 or shape[3] * 2 // 17 not in KV4_HEAD_DIMS:
+        raise ValueError(f"4-bit caches must share the shape kv4_cache_shape gives, got {tuple(shape)} and "
+                         f"{tuple(v_cache.shape)}")
+    sb, sh = _stride(k_cache, 0), _stride(k_cache, 1)
+    if k_cache.stride(3) != 1 or _stride(k_cache, 2) != shape[3] or v_cache.stride(3) != 1 or \
+            _stride(v_cache, 2) != shape[3] or _stride(v_cache, 0) != sb or _stride(v_cache, 1) != sh:
+        raise ValueError("4-bit caches must share strides, with the tiles of a head contiguous")
+    return shape[0], shape[1], shape[2] * KV4_TILE, shape[3] * 2 // 17, sb, sh
+
+
+def rope_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional[dict] = None):
+    """(inv_freq float64 [rotary_dim / 2] on the CPU, factor) for rope_angles.
+
+    inv_freq[i] = base^(-2 i / rotary_dim), changed by `scaling` for contexts `factor` times as long as
+    the `original` ones a model was trained on:
+      {'kind': 'linear', 'factor': s}   positions divided by s
+      {'kind': 'ntk', 'factor': s}      the base raised to base * s^(rotary_dim / (rotary_dim - 2)): the
+                                        slowest pair turns s times slower, the fastest as before
+      {'kind': 'yarn', 'factor': s, 'original': n}   pairs that turn more than beta_fast (32) times over n
+                                        positions keep their frequency, those below beta_slow (1) turns
+                                        are divided by s, a linear ramp in between; cos and sin are
+                                        multiplied by 0.1 ln s + 1 (Peng et al. 2023)"""
+    if rotary_dim <= 0 or rotary_dim % 2:
+        raise ValueError(f"rotary_dim {rotary_dim} must be a positive even number")
+    i = torch.arange(rotary_dim // 2, dtype=torch.float64)
+    if scaling is None:
+        return base ** (-2.0 * i / rotary_dim), 1.0
+    kind, s = scaling.get('kind'), float(scaling.get('factor', 1.0))
+    if not s > 0:
+        raise ValueError(f"rope scaling factor {s} must be positive")
+    if kind == 'linear':
+        return base ** (-2.0 * i / rotary_dim) / s, 1.0
+    if kind == 'ntk':
+        if rotary_dim <= 2:
+            raise ValueError("'ntk' scaling needs more than one rotated pair")
+        return (base * s ** (rotary_dim / (rotary_dim - 2))) ** (-2.0 * i / rotary_dim), 1.0
+    if kind == 'yarn':
+        if not scaling.get('original'):
+            raise ValueError("'yarn' scaling needs the 'original' context length")
+        fast, slow = float(scaling.get('beta_fast', 32.0)), float(scaling.get('beta_slow', 1.0))
+        if not fast > slow:
+            raise ValueError("'yarn' scaling needs beta_fast > beta_slow")
+        freq = base ** (-2.0 * i / rotary_dim)
+        turns = freq * (scaling['original'] / (2.0 * math.pi))
+        keep = ((turns - slow) / (fast - slow)).clamp(0.0, 1.0)
+        return freq * (keep + (1.0 - keep) / s), 0.1 * math.log(s) + 1.0
+    raise ValueError(f"unknown rope scaling kind {kind!r}; use 'linear', 'ntk' or 'yarn'")
+
+
+def rope_angles(positions: torch.Tensor, inv_freq: torch.Tensor, factor: float = 1.0):
+    """(cos, sin), each float32 [T, half]: factor * cos / sin of positions[t] * inv_freq[i], with the
+    angle formed in double.  positions int64 [T], inv_freq float64 [half].  The rows rope_rotate and
+    rope_kv4_write take; one call serves every layer of a step."""
+    dev = require_device(positions, inv_freq)
+    lib = _lib.load()
+    if positions.dtype != torch.int64 or positions.dim() != 1 or inv_freq.dtype != torch.float64 or inv_freq.dim() != 1:
+        raise TypeError("positions must be int64 [T] and inv_freq float64 [half]")
+    positions, inv_freq = positions.contiguous(), inv_freq.contiguous()
+    T, half = positions.shape[0], inv_freq.shape[0]
+    cos = torch.empty((T, half), dtype=torch.float32, device=dev)
+    sin = torch.empty((T, half), dtype=torch.float32, device=dev)
+    with _on(dev):
+        rc = lib.mi355_rope_angles(cos.data_ptr(), sin.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(),
+                                   float(factor), T, half, _stream(dev))
+    if rc:
+        _lib.check(rc, 'mi355_rope_angles')
+    return cos, sin
+
+
+def _angle_rows(cos: Optional[torch.Tensor], sin: Optional[torch.Tensor], T: int) -> int:
+    """rotary_dim of a pair of angle row tensors (0 when there are none)."""
+    if cos is None and sin is None:
+        return 0
+    if cos is None or sin is None or cos.dtype != torch.float32 or sin.dtype != torch.float32:
+        raise TypeError("cos and sin must both be float32 (or both None: no rotation)")
+    if cos.dim() != 2 or cos.shape[0] != T or cos.shape != sin.shape or not cos.is_contiguous() or not sin.is_contiguous():
+        raise ValueError("cos and sin must be contiguous [T, rotary_dim / 2], one row per token")
+    return 2 * cos.shape[1]
+
+
+def rope_rotate(x: torch.Tensor, cos: Optional[torch.Tensor], sin: Optional[torch.Tensor], interleaved: bool = False,
+                out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """x [T, H, D] with the first 2 * cos.shape[1] dims of every head row rotated (a new tensor, or `out`,
+    which must not overlap x).  cos / sin float32 [T, rotary_dim / 2], one row per token (rope_angles).
+    Pairs are (i, i + rotary_dim / 2), or neighbours (2 i, 2 i + 1) when `interleaved`."""
+    dev = require_device(x, cos, sin, out)
+    lib = _lib.load()
+    x = _head_rows(x)
+    T, H, D = x.shape
+    R = _angle_rows(cos, sin, T)
+    out = _checked_out(out, (T, H, D), x.dtype, dev)
+    with _on(dev):
+        rc = lib.mi355_rope_rotate(out.data_ptr(), x.data_ptr(), _stride(x, 0), cos.data_ptr() if R else None,
+                                   sin.data_ptr() if R else None, R, int(interleaved), T, H, D, dtype_code(x),
+                                   _stream(dev))
+    if rc:
+        _lib.check(rc, 'mi355_rope_rotate')
+    return out
+
+
+def rope_kv4_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: Optional[torch.Tensor],
+                   sin: Optional[torch.Tensor], slots: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                   interleaved: bool = False, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """rope_rotate(q), returned, and the rotated k and v [T, Hkv, D] rounded into the 4-bit caches at
+    `slots` (int64 [T]; a slot outside the cache writes nothing, no two tokens may share one).  q / k / v
+    are read only and may be views of one projection output; cos = sin = None: nothing is rotated."""
+    dev = require_device(q, k, v, cos, sin, slots, k_cache, v_cache, out)
+    lib = _lib.load()
+    q, k, v = _head_rows(q), _head_rows(k), _head_rows(v)
+    T, Hq, D = q.shape
+    NB, Hkv, BS, cache_dim, sb, sh = _kv4_geometry(k_cache, v_cache)
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError("q, k and v must share one dtype")
+    if k.shape != (T, Hkv, D) or v.shape != k.shape or cache_dim != D:
+        raise ValueError("k and v must be [T, kv_heads, head_dim] matching q and the caches")
+    if slots.dtype != torch.int64 or slots.numel() != T:
+        raise TypeError("slots must be int64 [T]")
+    slots = slots.contiguous()
+    R = _angle_rows(cos, sin, T)
+    out = _checked_out(out, (T, Hq, D), q.dtype, dev)
+    with _on(dev):
+        rc = lib.mi355_rope_kv4_write(
+            out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), _stride(q, 0), _stride(k, 0), _stride(v, 0),
+            cos.data_ptr() if R else None, sin.data_ptr() if R else None, R, int(interleaved), slots.data_ptr(),
+            k_cache.data_ptr(), v_cache.data_ptr(), T, Hq, Hkv, D, BS, NB, sb, sh, dtype_code(q), _stream(dev))
+    if rc:
+        _lib.check(rc, 'mi355_rope_kv4_write')
+    return out
+
+
+def kv4_read_slots(k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor,
+                   dtype: torch.dtype = torch.bfloat16):
+    """(k, v), each [T, kv_heads, head_dim]: the values cached at `slots` (int64 [T]); zeros for a slot
+    outside the cache.  bfloat16 and float32 hold every cached value exactly."""
+    dev = require_device(k_cache, v_cache, slots)
+    lib = _lib.load()
+    NB, Hkv, BS, D, sb, sh = _kv4_geometry(k_cache, v_cache)
+    if slots.dtype != torch.int64 or slots.dim() != 1:
+        raise TypeError("slots must be int64 [T]")
+    slots = slots.contiguous()
+    T = slots.shape[0]
+    k = torch.empty((T, Hkv, D), dtype=dtype, device=dev)
+    v = torch.empty((T, Hkv, D), dtype=dtype, device=dev)
+    code = dtype_code(k)
+    with _on(dev):
+        rc = lib.mi355_kv4_read_slots(k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+                                      slots.data_ptr(), T, Hkv, D, BS, NB, sb, sh, code, _stream(dev))
+    if rc:
+        _lib.check(rc, 'mi355_kv4_read_slots')
+    return k, v
+
+
+def paged_decode_kv4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
+                     context_lens: torch.Tensor, max_context: int, scale: Optional[float] = None,
+                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """paged_decode over a 4-bit cache (kv4_cache_shape): q [B, Hq, D], block_tables [B, max_blocks] and
+    context_lens [B] int32, max_context = host-side upper bound of context_lens.  Returns [B, Hq, D] in
+    q's dtype; a context of 0 gives zeros."""
+    dev = require_device(q, k_cache, v_cache, block_tables, context_lens, out)
+    lib = _lib.load()
+    if q.dim() != 3 or q.stride(2) != 1 or _stride(q, 1) != q.shape[2]:
+        q = q.contiguous()
+    B, Hq, D = q.shape
+    NB, Hkv, BS, cache_dim, sb, sh = _kv4_geometry(k_cache, v_cache)
+    if cache_dim != D:
+        raise ValueError(f"head_dim mismatch: q {D}, cache {cache_dim}")
+    if block_tables.dtype != torch.int32 or context_lens.dtype != torch.int32:
+        raise TypeError("block_tables and context_lens must be int32")
+    if block_tables.dim() != 2 or block_tables.shape[0] != B or context_lens.numel() != B:
+        raise ValueError("block_tables must be [B, max_blocks] and context_lens [B]")
+    block_tables, context_lens = block_tables.contiguous(), context_lens.contiguous()
+    out = _checked_out(out, (B, Hq, D), q.dtype, dev)
+    code = dtype_code(q)
+    if scale is None:
+        scale = 1.0 / math.sqrt(D)
+    width = block_tables.shape[1]
+    max_context = min(int(max_context), width * BS)
+    with _on(dev):
+        stream = _stream(dev)
+        need = lib.mi355_paged_decode_kv4_workspace_bytes(B, Hq, Hkv, D, max_context, code)
+        ws, ws_bytes = _workspace(dev, need, stream)
+        rc = lib.mi355_paged_decode_kv4(
+            out.data_ptr(), q.data_ptr(), _stride(q, 0), k_cache.data_ptr(), v_cache.data_ptr(),
+            block_tables.data_ptr(), context_lens.data_ptr(), B, Hq, Hkv, D, BS, width, NB, max_context, sb, sh,
+            float(scale), code, ws.data_ptr() if ws is not None else None, ws_bytes, stream)
+    if rc:
+        _lib.check(rc, 'mi355_paged_decode_kv4')
+    return out
+
+
+def paged_prefill_kv4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
+                      seg_q_start: torch.Tensor, seg_len: torch.Tensor, seg_pos0: torch.Tensor, max_q_len: int,
+                      max_context: int, scale: Optional[float] = None,
+                      out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """paged_prefill over a 4-bit cache: causal attention of new query tokens whose K / V rows are already
+    in it.  q [T, Hq, D]; segment s owns rows seg_q_start[s] .. +seg_len[s]-1, its first token sits at
+    position seg_pos0[s] and reads through block_tables[s]; all three int32 [nseg], max_q_len and
+    max_context their host-side bounds.  Rows of `out` outside every segment are left untouched."""
+    dev = require_device(q, k_cache, v_cache, block_tables, seg_q_start, seg_len, seg_pos0, out)
+    lib = _lib.load()
+    q = _head_rows(q)
+    T, Hq, D = q.shape
+    NB, Hkv, BS, cache_dim, sb, sh = _kv4_geometry(k_cache, v_cache)
+    if cache_dim != D:
+        raise ValueError(f"head_dim mismatch: q {D}, cache {cache_dim}")
+    for t in (block_tables, seg_q_start, seg_len, seg_pos0):
+        if t.dtype != torch.int32:
+            raise TypeError("block_tables and the segment vectors must be int32")
+    nseg = seg_len.numel()
+    if block_tables.dim() != 2 or block_tables.shape[0] != nseg or seg_q_start.numel() != nseg \
+            or seg_pos0.numel() != nseg:
+        raise ValueError("block_tables must be [nseg, max_blocks]; the segment vectors [nseg]")
+    block_tables = block_tables.contiguous()
+    seg_q_start, seg_len, seg_pos0 = seg_q_start.contiguous(), seg_len.contiguous(), seg_pos0.contiguous()
+    out = _checked_out(out, (T, Hq, D), q.dtype, dev)
+    if T == 0:
+        return out
+    code = dtype_code(q)
+    if scale is None:
+        scale = 1.0 / math.sqrt(D)
+    width = block_tables.shape[1]
+    max_context = min(int(max_context), width * BS)
+    with _on(dev):
+        stream = _stream(dev)
+        need = lib.mi355_paged_prefill_kv4_workspace_bytes(nseg, T, int(max_q_len), Hq, Hkv, D, max_context, code)
+        ws, ws_bytes = _workspace(dev, need, stream)
+        rc = lib.mi355_paged_prefill_kv4(
+            out.data_ptr(), q.data_ptr(), _stride(q, 0), k_cache.data_ptr(), v_cache.data_ptr(),
+            block_tables.data_ptr(), seg_q_start.data_ptr(), seg_len.data_ptr(), seg_pos0.data_ptr(), nseg,
+            int(max_q_len), Hq, Hkv, D, BS, width, NB, max_context, sb, sh, float(scale), code,
+            ws.data_ptr() if ws is not None else None, ws_bytes, stream)
+    if rc:
+        _lib.check(rc, 'mi355_paged_prefill_kv4')
+    return out
