@@ -27,6 +27,7 @@ namespace mi355 {
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 
 constexpr int kKv4Tile = 16;          // tokens per record
+constexpr int kKv4MaxContext = 1 << 29;   // positions are ints, and a step looks past its end
 constexpr int kKv4Step = 32;          // tokens per contraction step: two records
 constexpr int kKv4MinExp = -120, kKv4MaxExp = 125;
 constexpr float kKv4Floor = -3e38f;   // a running maximum no score has raised yet
@@ -40,18 +41,45 @@ struct Kv4Cache {
   char* k;
   char* v;
   int64_t s_blk, s_head;
-  int num_blocks, tpb;   // blocks in the pool, tiles per block
+  int num_blocks, tpb;       // blocks in the pool, tiles per block
+  uint32_t tpb_mul;          // tile / tpb = tile * tpb_mul >> tpb_shift for tile < 2^31
+  int tpb_shift;
 };
-
+static inline Kv4Cache kv4_cache(const void* k, const void* v, int64_t s_blk, int64_t s_head, int num_blocks, int tpb) {
+  int up = 0;
+  while ((1ll << up) < tpb) ++up;
+  const uint32_t mul = (uint32_t)(((1ull << (31 + up)) + tpb - 1) / tpb);   // ceil(2^(31+up) / tpb) <= 2^31 + ...: fits
+  return Kv4Cache{static_cast<char*>(const_cast<void*>(k)), static_cast<char*>(const_cast<void*>(v)), s_blk, s_head,
+                  num_blocks, tpb, mul, 31 + up};
+}
 // Checks what every entry point over the cache asks of it; 0 or the recorded error.
 int kv4_check_cache(const char* what, const void* k_cache, const void* v_cache, int Hkv, int D, int block_size,
                     int num_blocks, int64_t s_blk, int64_t s_head);
 
 __device__ __forceinline__ constexpr int kv4_tile_bytes(int D) { return 17 * D / 2; }
 
-// E8M0 byte j of a dword -> the float 2^(byte - 127) that the conversion instructions take
-// (255 becomes the pattern they answer with NaN).
-__device__ __forceinline__ float kv4_scale(uint32_t w, int j) { return u2f(((w >> (8 * j)) & 0xffu) << 23); }
+// Where tile `tile` of a sequence lies: the table entry that names its block, and its place in the block.
+struct Kv4Place {
+  int id, sub;
+};
+__device__ __forceinline__ Kv4Place kv4_place(const Kv4Cache& c, const int32_t* table, int tile) {
+  const int blk = (int)(((uint64_t)(uint32_t)tile * c.tpb_mul) >> c.tpb_shift);
+  // (constant memory for this launch, and the index is uniform: a scalar load, which vector loads in flight need not wait for)
+  typedef const __attribute__((address_space(4))) int32_t* ctable;
+  return Kv4Place{((ctable)table)[blk], tile - blk * c.tpb};
+}
+// Byte offset of its record within a head's part of the pool.
+__device__ __forceinline__ int64_t kv4_record(const Kv4Cache& c, Kv4Place at, int tile_bytes) {
+  const int id = at.id < 0 ? 0 : (at.id >= c.num_blocks ? c.num_blocks - 1 : at.id);
+  return (int64_t)((uint64_t)(uint32_t)id * (uint64_t)c.s_blk) + (int64_t)(at.sub * tile_bytes);
+}
+
+// E8M0 byte j of a dword -> the scale operand of the conversion instructions, which read the exponent
+// field of a float and nothing else (255 is answered with NaN): one shift, whatever lands in the sign
+// and the fraction.
+__device__ __forceinline__ float kv4_scale(uint32_t w, int j) {
+  return u2f(j == 3 ? w >> 1 : w << (23 - 8 * j));
+}
 
 // Byte J of `w` -> (low nibble, high nibble) as two bf16, times the scale: exact.
 template <int J>
@@ -157,39 +185,79 @@ __device__ __forceinline__ void store8(char* p, const float (&x)[8]) {
 template <int D>
 struct Kv4TileRegs {
   uint32_t k[D / 32], v[D / 32], vs[D / 32];
-  uint32_t ks;   // scale bytes of the lane's dims [g D/4, +D/4)
+  uint32_t ks;   // the dword that holds the scale byte(s) of the lane's dims [g D/4, +D/4)
 };
 
-template <int W>
-__device__ __forceinline__ void load_words(const char* p, uint32_t (&w)[W]) {
+typedef const __attribute__((address_space(1))) char* gptr;   // (an address that passes through asm has to say that it is global)
+
+// NT: rows that one workgroup reads once bypass the caches' retention.
+template <bool NT, int W>
+__device__ __forceinline__ void load_words(gptr p, uint32_t (&w)[W]) {
+  auto get = [](auto* q) { return NT ? __builtin_nontemporal_load(q) : *q; };
+  typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+  typedef const __attribute__((address_space(1))) uint32_t* p1;
+  typedef const __attribute__((address_space(1))) u32x2* p2;
+  typedef const __attribute__((address_space(1))) u32x4* p4;
   if constexpr (W == 1) {
-    w[0] = *reinterpret_cast<const uint32_t*>(p);
+    w[0] = get((p1)p);
   } else if constexpr (W == 2) {
-    const uint2 a = *reinterpret_cast<const uint2*>(p);
-    w[0] = a.x, w[1] = a.y;
+    const u32x2 a = get((p2)p);
+    w[0] = a[0], w[1] = a[1];
   } else {
 #pragma unroll
     for (int i = 0; i < W; i += 4) {
-      const u32x4 a = *reinterpret_cast<const u32x4*>(p + 4 * i);
+      const u32x4 a = get((p4)(p + 4 * i));
       w[i] = a[0], w[i + 1] = a[1], w[i + 2] = a[2], w[i + 3] = a[3];
     }
   }
 }
 
+// Where a lane finds its parts of a record (unsigned, so that a load is a uniform base and a 32-bit
+// lane offset), and by how much its K scale byte has to turn within its dword to land in the
+// exponent field.
 template <int D>
-__device__ __forceinline__ void kv4_load_k(const char* rec, int lane, Kv4TileRegs<D>& t) {
-  const int g = lane >> 4, c = lane & 15;
-  load_words(rec + c * (D / 2) + g * (D / 8), t.k);
-  const char* s = rec + 8 * D + c * (D / 32);
-  if constexpr (D == 32) t.ks = *reinterpret_cast<const uint8_t*>(s);
-  else if constexpr (D == 64) t.ks = *reinterpret_cast<const uint8_t*>(s + (g >> 1));
-  else if constexpr (D == 128) t.ks = *reinterpret_cast<const uint8_t*>(s + g);
-  else t.ks = *reinterpret_cast<const uint16_t*>(s + 2 * g);
+struct Kv4Lane {
+  uint32_t k, ks, v, vs, turn;
+  __device__ __forceinline__ explicit Kv4Lane(int lane) {
+    const uint32_t g = (uint32_t)lane >> 4, c = (uint32_t)lane & 15;
+    k = c * (D / 2) + g * (D / 8);
+    v = (uint32_t)lane * (D / 8);
+    vs = 8 * D + g * (D / 8);
+    const uint32_t at = c * (D / 32) + (g * (D / 4)) / 32;   // the lane's (first) scale byte
+    ks = 8 * D + (at & ~3u);
+    turn = (9 + 8 * (at & 3)) & 31;
+  }
+};
+// A uniform address kept in scalar registers: left alone, the compiler adds the loop's invariant part
+// of an address to the lane offsets and pays a 64-bit vector addition per load.
+__device__ __forceinline__ gptr scalar_base(const char* p) {
+  gptr g = (gptr)p;
+  asm("" : "+s"(g));
+  return g;
 }
+// The lane's 32-bit offset, as a value the compiler cannot widen outside the loop (the widening has to
+// stand next to the load for the load to take a scalar base and a 32-bit offset).
+__device__ __forceinline__ uint32_t lane_offset(uint32_t& o) {
+  asm volatile("" : "+v"(o));
+  return o;
+}
+template <int D, bool NT>
+__device__ __forceinline__ void kv4_load_k(gptr rec, Kv4Lane<D>& at, Kv4TileRegs<D>& t) {
+  load_words<NT>(rec + lane_offset(at.k), t.k);
+  uint32_t s[1];
+  load_words<NT>(rec + lane_offset(at.ks), s);
+  t.ks = s[0];
+}
+template <int D, bool NT>
+__device__ __forceinline__ void kv4_load_v(gptr rec, Kv4Lane<D>& at, Kv4TileRegs<D>& t) {
+  load_words<NT>(rec + lane_offset(at.v), t.v);
+  load_words<NT>(rec + lane_offset(at.vs), t.vs);
+}
+// The scale of contraction step s (of D / 32): a lane's dims span one scale block, two at D = 256.
 template <int D>
-__device__ __forceinline__ void kv4_load_v(const char* rec, int lane, Kv4TileRegs<D>& t) {
-  load_words(rec + lane * (D / 8), t.v);
-  load_words(rec + 8 * D + (lane >> 4) * (D / 8), t.vs);
+__device__ __forceinline__ float kv4_k_scale(const Kv4TileRegs<D>& t, const Kv4Lane<D>& at, int s) {
+  const uint32_t turn = D == 256 && s >= 4 ? (at.turn + 8) & 31 : at.turn;
+  return u2f(__builtin_amdgcn_alignbit(t.ks, t.ks, turn));
 }
 
 }  // namespace mi355

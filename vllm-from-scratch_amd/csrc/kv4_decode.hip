@@ -8,16 +8,16 @@
 // were born in (see kv4.h) against the same step's V tiles; every kv head accumulates into registers
 // of its own, so a NaN in one head never meets another.  The running maximum is only raised when a
 // score passes it by more than kKv4Raise powers of two: until then the sums stay on the old one.
-// The four waves of a workgroup take steps in turn and combine their sums in LDS; a long context is
+// The waves of a workgroup take steps in turn and combine their sums in LDS; a long context is
 // split over workgroups, whose partial sums kv4_merge_kernel joins.
 #include <algorithm>
+#include <cmath>
 
 #include "kv4.h"
 
 namespace mi355 {
 namespace {
 
-constexpr int kWaves = 4;
 
 struct Kv4DecodeParams {
   char* out;
@@ -30,125 +30,145 @@ struct Kv4DecodeParams {
   int64_t q_stride;   // elements
   int B, Hq, Hkv, G /* query heads per kv head */, gc /* of them per workgroup */, qchunks, hgroups;
   int max_blocks, max_ctx, nsplit, tps /* tokens per split */;
-  float scale2;   // scale * log2(e)
+  float scale2, raise;   // |scale| * log2(e); kKv4Raise in units of a raw score
+  int flip;              // a negative scale: the queries are negated
 };
 
-template <class Tag, int D, int NH>
-__global__ void __launch_bounds__(256) kv4_decode_kernel(const Kv4DecodeParams p) {
+template <class Tag, int D, int NH, int W>
+__global__ void __launch_bounds__(W * 64) kv4_decode_kernel(const Kv4DecodeParams p) {
   constexpr int NP = Kv4Pieces<Tag>::n, KS = D / 32, EB = Tag::kBytes;
-  __shared__ float s_o[kWaves][16][D + 4];
-  __shared__ float s_m[kWaves][16], s_l[kWaves][16];
+  __shared__ float s_o[W][16][D + 4];
+  __shared__ float s_m[W][16], s_l[W][16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, col = lane & 15;
+  Kv4Lane<D> at(lane);
   int idx = blockIdx.x;
   const int sp = idx % p.nsplit;
   idx /= p.nsplit;
   const int qc = idx % p.qchunks;
   idx /= p.qchunks;
   const int hg = idx % p.hgroups, b = idx / p.hgroups;
-  const int h0 = hg * NH, nh = min(NH, p.Hkv - h0);
+  const int h0 = hg * NH;
   // column -> (kv head h0 + my_j, query head of its group)
   const int my_j = col / p.gc, my_q = qc * p.gc + col % p.gc;
-  const bool used = my_j < nh && my_q < p.G;
+  const bool used = my_j < NH && my_q < p.G;
   const int hq = (h0 + my_j) * p.G + my_q;
 
-  int ctx = min(p.ctx[b], p.max_ctx);
+  const int ctx = min(p.ctx[b], p.max_ctx);
   const int lo = sp * p.tps, hi = min(ctx, lo + p.tps);   // this workgroup's tokens
-  if (lo >= hi && !(sp == 0 && p.nsplit == 1)) return;    // (the merge knows which splits are empty)
+  if (lo >= hi && p.nsplit > 1) return;                   // (the merge knows which splits are empty)
 
   bf16x8_t qf[KS][NP];
 #pragma unroll
   for (int s = 0; s < KS; ++s) {
     float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (used) load8<Tag>(p.q + ((int64_t)b * p.q_stride + (int64_t)hq * D + g * (D / 4) + s * 8) * EB, x);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = p.flip ? -x[e] : x[e];
     bf16_pieces<NP>(x, qf[s]);
   }
-  f32x4 acc[NH][KS][2];
+  f32x4 acc[NH][KS][2], sum = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int j = 0; j < NH; ++j)
 #pragma unroll
     for (int s = 0; s < KS; ++s) acc[j][s][0] = acc[j][s][1] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float m = kKv4Floor, l = 0.f;
+  float m = kKv4Floor, m2 = kKv4Floor;   // running maximum of the raw scores, and times the scale
+  bf16x8_t ones;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) ones[e] = (__bf16)1.f;
 
   const int32_t* table = p.bt + (int64_t)b * p.max_blocks;
-  const int last_tile = hi > 0 ? (hi - 1) / kKv4Tile : 0;
-  auto record = [&](int tile) -> int64_t {   // byte offset of a tile's record of kv head h0
-    tile = min(tile, last_tile);             // (a step's second tile may lie beyond the context: read the last one)
-    int id = table[tile / p.cache.tpb];
-    id = id < 0 ? 0 : (id >= p.cache.num_blocks ? p.cache.num_blocks - 1 : id);
-    return (int64_t)id * p.cache.s_blk + (int64_t)h0 * p.cache.s_head + (tile % p.cache.tpb) * kv4_tile_bytes(D);
+  const char* const kbase = p.cache.k + (int64_t)h0 * p.cache.s_head;
+  const char* const vbase = p.cache.v + (int64_t)h0 * p.cache.s_head;
+  const int last_tile = (hi - 1) / kKv4Tile;
+  // (a step's second tile may lie beyond the context: the last one is read twice)
+  auto place = [&](int t, int i) { return kv4_place(p.cache, table, min((int)((uint32_t)t / kKv4Tile) + i, last_tile)); };
+  auto record = [&](Kv4Place at) { return kv4_record(p.cache, at, kv4_tile_bytes(D)); };
+  Kv4TileRegs<D> T[NH][2];
+  auto fetch_k = [&](int64_t r0, int64_t r1) {
+#pragma unroll
+    for (int j = 0; j < NH; ++j) {
+      kv4_load_k<D, true>(scalar_base(kbase + r0 + j * p.cache.s_head), at, T[j][0]);
+      kv4_load_k<D, true>(scalar_base(kbase + r1 + j * p.cache.s_head), at, T[j][1]);
+    }
+  };
+  auto fetch_v = [&](int64_t r0, int64_t r1) {
+#pragma unroll
+    for (int j = 0; j < NH; ++j) {
+      kv4_load_v<D, true>(scalar_base(vbase + r0 + j * p.cache.s_head), at, T[j][0]);
+      kv4_load_v<D, true>(scalar_base(vbase + r1 + j * p.cache.s_head), at, T[j][1]);
+    }
   };
 
-  for (int t0 = lo + wave * kKv4Step; t0 < hi; t0 += kWaves * kKv4Step) {
-    const int64_t r0 = record(t0 / kKv4Tile), r1 = record(t0 / kKv4Tile + 1);
-    f32x4 S[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
-    Kv4TileRegs<D> T[NH][2];
+  constexpr int kStride = W * kKv4Step;
+  int t0 = lo + wave * kKv4Step;
+  // the table entries of the next step, asked for a step ahead of the loads that need them: waiting for an
+  // entry in front of its loads would put one more trip to memory into every step
+  Kv4Place n0{}, n1{};
+  if (t0 < hi) {
+    const Kv4Place a0 = place(t0, 0), a1 = place(t0, 1);
+    n0 = place(min(t0 + kStride, hi - 1), 0), n1 = place(min(t0 + kStride, hi - 1), 1);
+    const int64_t r0 = record(a0), r1 = record(a1);
+    fetch_k(r0, r1);
+    fetch_v(r0, r1);
+  }
+  // K registers are refilled for the next step as soon as the scores are made, V registers as soon as the
+  // weights have met them: each load has the other half of a step to arrive.  The last step refills them
+  // with the tile it has just read: a branch around the loads would make the compiler wait for all of them.
+  for (; t0 < hi; t0 += kStride) {
+    f32x4 S[2];
 #pragma unroll
     for (int j = 0; j < NH; ++j) {
-      if (j < nh) {
-        kv4_load_k<D>(p.cache.k + r0 + j * p.cache.s_head, lane, T[j][0]);
-        kv4_load_k<D>(p.cache.k + r1 + j * p.cache.s_head, lane, T[j][1]);
-      }
-    }
 #pragma unroll
-    for (int j = 0; j < NH; ++j) {
-      if (j < nh) {
-        kv4_load_v<D>(p.cache.v + r0 + j * p.cache.s_head, lane, T[j][0]);
-        kv4_load_v<D>(p.cache.v + r1 + j * p.cache.s_head, lane, T[j][1]);
-      }
-    }
+      for (int i = 0; i < 2; ++i) {
+        f32x4 c = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < NH; ++j) {
-      if (j < nh) {
+        for (int s = 0; s < KS; ++s) {
+          const bf16x8_t a = kv4_k_frag(T[j][i].k[s], kv4_k_scale<D>(T[j][i], at, s));
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          f32x4 c = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int s = 0; s < KS; ++s) {
-            const bf16x8_t a = kv4_k_frag(T[j][i].k[s], kv4_scale(T[j][i].ks, D == 256 ? s / 4 : 0));
-#pragma unroll
-            for (int n = 0; n < NP; ++n) c = mfma_bf16(a, qf[s][n], c);
-          }
+          for (int n = 0; n < NP; ++n) c = mfma_bf16(a, qf[s][n], c);
+        }
+        if (j == 0) S[i] = c;
+        else
 #pragma unroll
           for (int e = 0; e < 4; ++e) S[i][e] = my_j == j ? c[e] : S[i][e];
-        }
       }
     }
-    // tokens 4 g + e of each tile, in powers of two
-    float x[8];
+    const int64_t r0 = record(n0), r1 = record(n1);
+    fetch_k(r0, r1);
+    const int after = min(t0 + 2 * kStride, hi - 1);
+    n0 = place(after, 0), n1 = place(after, 1);
+    float x[8];   // tokens 4 g + e of each tile
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = S[e >> 2][e & 3] * p.scale2;
+    for (int e = 0; e < 8; ++e) x[e] = S[e >> 2][e & 3];
     if (t0 + kKv4Step > hi) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
+      for (int e = 0; e < 8; ++e)
         if (t0 + (e >> 2) * kKv4Tile + 4 * g + (e & 3) >= hi) x[e] = -INFINITY;
-      }
+      // rows behind the context hold whatever was there: their codes count as 0 and their scales as 1
 #pragma unroll
-      for (int j = 0; j < NH; ++j) {
-        if (j < nh) {
+      for (int i = 0; i < 2; ++i) {
+        const int live = hi - (t0 + i * kKv4Tile + 4 * g);   // of this lane's four tokens
+        const uint32_t keep = live >= 4 ? ~0u : (live <= 0 ? 0u : (1u << (8 * live)) - 1u);
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            // rows behind the context hold whatever was there: their codes count as 0 and their scales as 1
-            const int live = hi - (t0 + i * kKv4Tile + 4 * g);   // tokens of this lane's four that count
-            const uint32_t keep = live >= 4 ? ~0u : (live <= 0 ? 0u : (1u << (8 * live)) - 1u);
+        for (int j = 0; j < NH; ++j)
 #pragma unroll
-            for (int s = 0; s < KS; ++s) {
-              T[j][i].v[s] &= keep;
-              T[j][i].vs[s] = (T[j][i].vs[s] & keep) | (0x7f7f7f7fu & ~keep);
-            }
+          for (int s = 0; s < KS; ++s) {
+            T[j][i].v[s] &= keep;
+            T[j][i].vs[s] = (T[j][i].vs[s] & keep) | (0x7f7f7f7fu & ~keep);
           }
-        }
       }
     }
-    float top = x[0];
-#pragma unroll
-    for (int e = 1; e < 8; ++e) top = fmaxf(top, x[e]);
-    if (__ballot(top > m + kKv4Raise)) {
+    float top = fmaxf(fmaxf(x[0], x[1]), x[2]);
+    top = fmaxf(fmaxf(top, x[3]), x[4]);
+    top = fmaxf(fmaxf(top, x[5]), fmaxf(x[6], x[7]));
+    if (__ballot(top > m + p.raise)) {
       top = fmaxf(top, __shfl_xor(top, 16));
       top = fmaxf(top, __shfl_xor(top, 32));
-      const float mn = fmaxf(m, top), f = fast_exp2(m - mn);
+      const float mn = fmaxf(m, top), f = fast_exp2((m - mn) * p.scale2);
       m = mn;
-      l *= f;
+      m2 = fmaxf(mn * p.scale2, kKv4Floor);
+      sum *= f;
 #pragma unroll
       for (int j = 0; j < NH; ++j)
 #pragma unroll
@@ -158,35 +178,30 @@ __global__ void __launch_bounds__(256) kv4_decode_kernel(const Kv4DecodeParams p
         }
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      x[e] = fast_exp2(x[e] - m);
-      l += x[e];
-    }
+    for (int e = 0; e < 8; ++e) x[e] = fast_exp2(__builtin_fmaf(x[e], p.scale2, -m2));
     bf16x8_t pf[NP];
     bf16_pieces<NP>(x, pf);
 #pragma unroll
-    for (int j = 0; j < NH; ++j) {
-      if (j < nh) {
+    for (int n = 0; n < NP; ++n) sum = mfma_bf16(ones, pf[n], sum);   // every row: the column's sum of weights
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          bf16x8_t ev, od;
-          kv4_v_frags(T[j][0].v[s], T[j][1].v[s], T[j][0].vs[s], T[j][1].vs[s], ev, od);
+    for (int j = 0; j < NH; ++j)
 #pragma unroll
-          for (int n = 0; n < NP; ++n) {
-            acc[j][s][0] = mfma_bf16(ev, pf[n], acc[j][s][0]);
-            acc[j][s][1] = mfma_bf16(od, pf[n], acc[j][s][1]);
-          }
+      for (int s = 0; s < KS; ++s) {
+        bf16x8_t ev, od;
+        kv4_v_frags(T[j][0].v[s], T[j][1].v[s], T[j][0].vs[s], T[j][1].vs[s], ev, od);
+#pragma unroll
+        for (int n = 0; n < NP; ++n) {
+          acc[j][s][0] = mfma_bf16(ev, pf[n], acc[j][s][0]);
+          acc[j][s][1] = mfma_bf16(od, pf[n], acc[j][s][1]);
         }
       }
-    }
+    fetch_v(r0, r1);
   }
 
   // the lane's column: dims 32 s + 8 g .. + 8 (even and odd rows of the two accumulators alternate)
-  l += __shfl_xor(l, 16);
-  l += __shfl_xor(l, 32);
   if (g == 0) {
-    s_m[wave][col] = m;
-    s_l[wave][col] = l;
+    s_m[wave][col] = m2;
+    s_l[wave][col] = sum[0];
   }
 #pragma unroll
   for (int s = 0; s < KS; ++s) {
@@ -206,16 +221,16 @@ __global__ void __launch_bounds__(256) kv4_decode_kernel(const Kv4DecodeParams p
   __syncthreads();
   // columns x pieces of eight dims over the workgroup's threads
   constexpr int P = D / 8;
-  for (int item = threadIdx.x; item < 16 * P; item += 256) {
+  for (int item = threadIdx.x; item < 16 * P; item += W * 64) {
     const int c = item / P, d = (item % P) * 8;
     const int j = c / p.gc, qi = qc * p.gc + c % p.gc;
-    if (j >= nh || qi >= p.G) continue;
+    if (j >= NH || qi >= p.G) continue;
     float M = s_m[0][c];
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) M = fmaxf(M, s_m[w][c]);
+    for (int w = 1; w < W; ++w) M = fmaxf(M, s_m[w][c]);
     float L = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
+    for (int w = 0; w < W; ++w) {
       const float f = fast_exp2(s_m[w][c] - M);
       L = __builtin_fmaf(s_l[w][c], f, L);
 #pragma unroll
@@ -239,75 +254,114 @@ __global__ void __launch_bounds__(256) kv4_decode_kernel(const Kv4DecodeParams p
   }
 }
 
-// Joins the splits of a row: thread = eight dims.
+// Joins the splits of a row, one workgroup each: a thread owns eight dims and every SL-th split (the
+// records of a long row lie a memory latency apart when one thread walks them all: 32 splits of 128
+// dims took 25 us that way), then the threads of the same dims meet in LDS.
 template <class Tag, int D>
 __global__ void __launch_bounds__(256)
-kv4_merge_kernel(char* out, const float* ws_acc, const float* ws_ml, const int32_t* ctx_lens, int rows, int Hq,
-                 int max_ctx, int nsplit, int tps) {
-  constexpr int P = D / 8;
-  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t row = idx / P;
-  const int d = (int)(idx % P) * 8;
-  if (row >= rows) return;
+kv4_merge_kernel(char* out, const float* ws_acc, const float* ws_ml, const int32_t* ctx_lens, int Hq, int max_ctx,
+                 int nsplit, int tps) {
+  constexpr int P = D / 8, SL = 256 / P;
+  __shared__ float s_m[SL][P], s_l[SL][P], s_o[SL][P][9];   // (9: neighbouring threads on neighbouring banks)
+  const int64_t row = blockIdx.x;
+  const int piece = threadIdx.x % P, sl = threadIdx.x / P;
   const int ctx = min(ctx_lens[row / Hq], max_ctx);
   const int n = ctx <= 0 ? 0 : min(nsplit, (ctx + tps - 1) / tps);
   float M = kKv4Floor, L = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < n; ++s) {
-    const float ms = ws_ml[(row * nsplit + s) * 2], ls = ws_ml[(row * nsplit + s) * 2 + 1];
-    const float* a = ws_acc + (row * nsplit + s) * D + d;
-    const f32x4 lo = *reinterpret_cast<const f32x4*>(a), hi = *reinterpret_cast<const f32x4*>(a + 4);
+  auto join = [&](float ms, float ls, const float (&x)[8]) {
     const float Mn = fmaxf(M, ms), fo = fast_exp2(M - Mn), fn = fast_exp2(ms - Mn);
     M = Mn;
     L = __builtin_fmaf(ls, fn, L * fo);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      o[e] = __builtin_fmaf(lo[e], fn, o[e] * fo);
-      o[4 + e] = __builtin_fmaf(hi[e], fn, o[4 + e] * fo);
+    for (int e = 0; e < 8; ++e) o[e] = __builtin_fmaf(x[e], fn, o[e] * fo);
+  };
+#pragma unroll 2
+  for (int s = sl; s < n; s += SL) {
+    float x[8];
+    load8<F32>(reinterpret_cast<const char*>(ws_acc + (row * nsplit + s) * D + piece * 8), x);
+    join(ws_ml[(row * nsplit + s) * 2], ws_ml[(row * nsplit + s) * 2 + 1], x);
+  }
+  for (int half = SL / 2; half > 0; half /= 2) {
+    if (sl >= half && sl < 2 * half) {
+      s_m[sl][piece] = M;
+      s_l[sl][piece] = L;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s_o[sl][piece][e] = o[e];
+    }
+    __syncthreads();
+    if (sl < half) {
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = s_o[sl + half][piece][e];
+      join(s_m[sl + half][piece], s_l[sl + half][piece], x);
     }
   }
-  const float inv = n > 0 ? 1.f / L : 0.f;
+  if (sl != 0) return;
+  const float inv = n > 0 ? 1.f / L : 0.f;   // no token at all: zeros
 #pragma unroll
   for (int e = 0; e < 8; ++e) o[e] *= inv;
-  store8<Tag>(out + (row * D + d) * Tag::kBytes, o);
+  store8<Tag>(out + (row * D + piece * 8) * Tag::kBytes, o);
 }
 
 struct Kv4Plan {
-  int NH, gc, qchunks, hgroups, nsplit, tps;
+  int NH, W, gc, qchunks, hgroups, nsplit, tps;
   size_t ws_bytes;
 };
 
-// Host arithmetic only.
+// Host arithmetic only.  Figures: us per call, 8 heads of 64 in bf16 unless said otherwise.
 int make_plan(const char* what, int B, int Hq, int Hkv, int D, int max_ctx, int dtype, Kv4Plan* pl) {
   if (!kv4_dtype_ok(dtype)) return fail(MI355_EINVAL, "%s: dtype %d", what, dtype);
   if (!kv4_head_dim_ok(D)) return fail(MI355_EUNSUPPORTED, "%s: head_dim %d (the 4-bit cache holds 32, 64, 128 or 256)", what, D);
-  if (B < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || max_ctx < 0)
+  if (B < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || max_ctx < 0 || max_ctx > kKv4MaxContext)
     return fail(MI355_EINVAL, "%s: bad shape (B=%d Hq=%d Hkv=%d max_context=%d)", what, B, Hq, Hkv, max_ctx);
   const int G = Hq / Hkv;
   pl->gc = std::min(G, 16);
   pl->qchunks = (G + 15) / 16;
+  // kv heads per wave: more of them share a step's softmax and read longer runs of a block, but make fewer, longer
+  // workgroups.  `units` counts (kv head, 128 tokens) pieces of the whole call.  256 x 2048: 61 / 56 / 53.7 with 1 / 2 / 4
+  // heads; 16 x 4000: 14.7 / 14.4 / 14.5; 32 x 1000: 9.0 / 11.3.  The accumulators of NH heads take NH D / 2 registers:
+  // NH D <= 256 leaves room for two waves per SIMD.
+  const int64_t rounds128 = ((int64_t)max_ctx + 127) / 128, units = (int64_t)std::max(B, 1) * Hkv * pl->qchunks * rounds128;
   pl->NH = 1;
-  pl->hgroups = (Hkv + pl->NH - 1) / pl->NH;
+  while (pl->NH * 2 <= 256 / D && pl->NH * 2 * pl->gc <= 16 && Hkv % (pl->NH * 2) == 0 && units >= 4096 * pl->NH) pl->NH *= 2;
+  pl->hgroups = Hkv / pl->NH;
   const int64_t groups = (int64_t)std::max(B, 1) * pl->hgroups * pl->qchunks;
-  const int steps = std::max(1, (max_ctx + kWaves * kKv4Step - 1) / (kWaves * kKv4Step));   // rounds of a workgroup's four waves
-  int64_t want = std::max<int64_t>(1, (1024 + groups - 1) / groups);
-  want = std::min<int64_t>(want, steps);
-  const int per = (int)((steps + want - 1) / want);
-  pl->tps = per * kWaves * kKv4Step;
-  pl->nsplit = (steps + per - 1) / per;
+  // More workgroups than the chip's 256 CUs: four waves each.  Fewer: eight waves each as long as that leaves a wave few
+  // steps (1 x 500: 6.6, in two splits and their merge 8.5; 32 x 1000: 9.0 against 10.4 with four waves), else the context
+  // is split over workgroups, two per CU (1 x 8000: 9.5; 4 sequences to 65536, 32/8 heads of 128, fp16: 45 against 67 with
+  // one per CU; head_dim 256 takes one per CU: 16 x 2000, 4 heads of 256: 15.1 against 16.0), none shorter than 256 tokens.
+  int64_t want = 1;
+  pl->W = 4;
+  if (groups <= 256) {
+    if (max_ctx <= 1024 || groups > 192) pl->W = 8;
+    else want = std::min<int64_t>(((D == 256 ? 256 : 512) + groups - 1) / groups, ((int64_t)max_ctx + 255) / 256);
+  }
+  const int64_t round = pl->W * kKv4Step;                                             // tokens of a workgroup's waves at once
+  const int64_t rounds = std::max<int64_t>(1, ((int64_t)max_ctx + round - 1) / round), per = (rounds + want - 1) / want;
+  pl->tps = (int)(per * round);
+  pl->nsplit = (int)((rounds + per - 1) / per);
   pl->ws_bytes = pl->nsplit > 1 ? (size_t)B * Hq * pl->nsplit * (D + 2) * sizeof(float) : 0;
   return 0;
 }
 
+template <class Tag, int D, int NH>
+void launch_heads(const Kv4DecodeParams& p, int W, hipStream_t s) {
+  const dim3 grid((unsigned)((int64_t)p.B * p.hgroups * p.qchunks * p.nsplit));
+  if (W == 4) hipLaunchKernelGGL((kv4_decode_kernel<Tag, D, NH, 4>), grid, dim3(256), 0, s, p);
+  else hipLaunchKernelGGL((kv4_decode_kernel<Tag, D, NH, 8>), grid, dim3(512), 0, s, p);
+}
 template <class Tag, int D>
 int launch(const Kv4DecodeParams& p, const Kv4Plan& pl, hipStream_t s) {
-  const int64_t wgs = (int64_t)p.B * p.hgroups * p.qchunks * p.nsplit;
-  const dim3 grid((unsigned)wgs), block(256);
-  hipLaunchKernelGGL((kv4_decode_kernel<Tag, D, 1>), grid, block, 0, s, p);
+  switch (pl.NH) {
+    case 8: if constexpr (D <= 32) launch_heads<Tag, D, 8>(p, pl.W, s); break;
+    case 4: if constexpr (D <= 64) launch_heads<Tag, D, 4>(p, pl.W, s); break;
+    case 2: if constexpr (D <= 128) launch_heads<Tag, D, 2>(p, pl.W, s); break;
+    default: launch_heads<Tag, D, 1>(p, pl.W, s);
+  }
   if (int rc = check_launch("kv4_decode_kernel")) return rc;
   if (p.nsplit > 1) {
-    const int rows = p.B * p.Hq;
-    hipLaunchKernelGGL((kv4_merge_kernel<Tag, D>), dim3((unsigned)ceil_div64((int64_t)rows * (D / 8), 256)), block, 0, s,
-                       p.out, p.ws_acc, p.ws_ml, p.ctx, rows, p.Hq, p.max_ctx, p.nsplit, p.tps);
+    hipLaunchKernelGGL((kv4_merge_kernel<Tag, D>), dim3((unsigned)(p.B * p.Hq)), dim3(256), 0, s, p.out, p.ws_acc, p.ws_ml,
+                       p.ctx, p.Hq, p.max_ctx, p.nsplit, p.tps);
     return check_launch("kv4_merge_kernel");
   }
   return 0;
@@ -359,8 +413,7 @@ extern "C" int mi355_paged_decode_kv4(void* out, const void* q, int64_t q_stride
   Kv4DecodeParams p;
   p.out = static_cast<char*>(out);
   p.q = static_cast<const char*>(q);
-  p.cache = Kv4Cache{static_cast<char*>(const_cast<void*>(k_cache)), static_cast<char*>(const_cast<void*>(v_cache)),
-                     stride_block, stride_head, num_blocks, block_size / kKv4Tile};
+  p.cache = kv4_cache(k_cache, v_cache, stride_block, stride_head, num_blocks, block_size / kKv4Tile);
   p.bt = block_tables;
   p.ctx = context_lens;
   p.ws_acc = static_cast<float*>(workspace);
@@ -377,7 +430,9 @@ extern "C" int mi355_paged_decode_kv4(void* out, const void* q, int64_t q_stride
   p.max_ctx = max_context;
   p.nsplit = pl.nsplit;
   p.tps = pl.tps;
-  p.scale2 = scale * 1.44269504088896340736f;
+  p.flip = scale < 0.f;
+  p.scale2 = std::max(std::fabs(scale) * 1.44269504088896340736f, 1e-30f);   // (a scale of 0: all weights 1 to 30 digits)
+  p.raise = kKv4Raise / p.scale2;
   hipStream_t s = static_cast<hipStream_t>(stream);
   switch (dtype) {
     case MI355_F32: return launch<F32>(p, pl, D, s);

@@ -31,6 +31,7 @@ __global__ void __launch_bounds__(256) kv4_prefill_kernel(const Kv4PrefillParams
   constexpr int NP = Kv4Pieces<Tag>::n, KS = D / 32, EB = Tag::kBytes;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, col = lane & 15;
+  Kv4Lane<D> at(lane);
   int idx = blockIdx.x;
   const int h = idx % p.Hkv;
   idx /= p.Hkv;
@@ -75,9 +76,7 @@ __global__ void __launch_bounds__(256) kv4_prefill_kernel(const Kv4PrefillParams
   const int last_tile = max(last_lim, 0) / kKv4Tile;
   auto record = [&](int tile) -> int64_t {
     tile = min(tile, last_tile);
-    int id = table[tile / p.cache.tpb];
-    id = id < 0 ? 0 : (id >= p.cache.num_blocks ? p.cache.num_blocks - 1 : id);
-    return (int64_t)id * p.cache.s_blk + (int64_t)h * p.cache.s_head + (tile % p.cache.tpb) * kv4_tile_bytes(D);
+    return kv4_record(p.cache, kv4_place(p.cache, table, tile), kv4_tile_bytes(D)) + (int64_t)h * p.cache.s_head;
   };
 
   for (int t0 = 0; t0 <= last_lim; t0 += kKv4Step) {
@@ -85,8 +84,8 @@ __global__ void __launch_bounds__(256) kv4_prefill_kernel(const Kv4PrefillParams
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int64_t r = record(t0 / kKv4Tile + i);
-      kv4_load_k<D>(p.cache.k + r, lane, T[i]);
-      kv4_load_v<D>(p.cache.v + r, lane, T[i]);
+      kv4_load_k<D, false>(scalar_base(p.cache.k + r), at, T[i]);
+      kv4_load_v<D, false>(scalar_base(p.cache.v + r), at, T[i]);
     }
     const bool masked = t0 + kKv4Step - 1 > first_lim;
     f32x4 S[MC][2];
@@ -96,7 +95,7 @@ __global__ void __launch_bounds__(256) kv4_prefill_kernel(const Kv4PrefillParams
       for (int mc = 0; mc < MC; ++mc) S[mc][i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
-        const bf16x8_t a = kv4_k_frag(T[i].k[s], kv4_scale(T[i].ks, D == 256 ? s / 4 : 0));
+        const bf16x8_t a = kv4_k_frag(T[i].k[s], kv4_k_scale<D>(T[i], at, s));
 #pragma unroll
         for (int mc = 0; mc < MC; ++mc)
 #pragma unroll
@@ -251,7 +250,8 @@ extern "C" int mi355_paged_prefill_kv4(void* out, const void* q, int64_t q_strid
   if (int rc = kv4_check_cache("paged_prefill_kv4", k_cache, v_cache, Hkv, D, block_size, num_blocks, stride_block, stride_head))
     return rc;
   if (!kv4_dtype_ok(dtype)) return fail(MI355_EINVAL, "paged_prefill_kv4: dtype %d", dtype);
-  if (nseg < 0 || max_q_len < 0 || Hq <= 0 || Hq % Hkv || max_blocks <= 0 || max_context <= 0)
+  if (nseg < 0 || max_q_len < 0 || Hq <= 0 || Hq % Hkv || max_blocks <= 0 || max_context <= 0 ||
+      (max_context > kKv4MaxContext && (int64_t)max_blocks * block_size > kKv4MaxContext))
     return fail(MI355_EINVAL, "paged_prefill_kv4: bad shape (nseg=%d max_q_len=%d Hq=%d Hkv=%d max_blocks=%d max_context=%d)",
                 nseg, max_q_len, Hq, Hkv, max_blocks, max_context);
   if ((int64_t)max_context > (int64_t)max_blocks * block_size) max_context = max_blocks * block_size;
@@ -262,8 +262,7 @@ extern "C" int mi355_paged_prefill_kv4(void* out, const void* q, int64_t q_strid
   Kv4PrefillParams p;
   p.out = static_cast<char*>(out);
   p.q = static_cast<const char*>(q);
-  p.cache = Kv4Cache{static_cast<char*>(const_cast<void*>(k_cache)), static_cast<char*>(const_cast<void*>(v_cache)),
-                     stride_block, stride_head, num_blocks, block_size / kKv4Tile};
+  p.cache = kv4_cache(k_cache, v_cache, stride_block, stride_head, num_blocks, block_size / kKv4Tile);
   p.bt = block_tables;
   p.seg_q0 = seg_q_start;
   p.seg_len = seg_len;

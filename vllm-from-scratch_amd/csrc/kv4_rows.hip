@@ -365,8 +365,7 @@ extern "C" int mi355_rope_kv4_write(void* q_out, const void* q, const void* k, c
   p.cos = cos_rows;
   p.sin = sin_rows;
   p.slots = slots;
-  p.cache = Kv4Cache{static_cast<char*>(k_cache), static_cast<char*>(v_cache), stride_block, stride_head, num_blocks,
-                     block_size / kKv4Tile};
+  p.cache = kv4_cache(k_cache, v_cache, stride_block, stride_head, num_blocks, block_size / kKv4Tile);
   p.num_slots = (int64_t)num_blocks * block_size;
   p.bs_shift = ilog2_exact(block_size);
   p.Hq = Hq;
@@ -389,8 +388,7 @@ extern "C" int mi355_kv4_read_slots(void* k_out, void* v_out, const void* k_cach
   p.k_out = static_cast<char*>(k_out);
   p.v_out = static_cast<char*>(v_out);
   p.slots = slots;
-  p.cache = Kv4Cache{static_cast<char*>(const_cast<void*>(k_cache)), static_cast<char*>(const_cast<void*>(v_cache)),
-                     stride_block, stride_head, num_blocks, block_size / kKv4Tile};
+  p.cache = kv4_cache(k_cache, v_cache, stride_block, stride_head, num_blocks, block_size / kKv4Tile);
   p.rows = (int64_t)T * 2 * Hkv;
   p.num_slots = (int64_t)num_blocks * block_size;
   p.Hkv = Hkv;
