@@ -1,10 +1,16 @@
 // Attention of several new query tokens per sequence over the 4-bit KV cache (their K / V rows are in
 // it already): query j of a segment attends to positions 0 .. pos0 + j.
 //
-// The query rows of a (segment, kv head) are its (token, query head of the group) pairs; a wave owns
-// MC tiles of 16 of them (the columns of its score tiles) and walks the context in steps of 32
-// tokens.  A step's K and V are converted to bf16 once (exact) and serve the wave's MC tiles.
+// The query rows of a (segment, kv head) are its (token, query head of the group) pairs.  A workgroup
+// of four waves owns 4 x MC tiles of 16 of them (a tile is the 16 columns of a score tile) and walks the
+// context in stages of SUB steps of 32 tokens.  Per stage each wave converts a quarter of the K and V
+// codes to bf16 (exact) and leaves them in LDS as the operands of the matrix instruction; every wave
+// reads them all back, once per MC tiles.  Conversion is what the format costs beside attention in
+// bf16: 130 vector instructions per 32 tokens of 128 dims, as many as two tiles' softmax, so it is done
+// once per workgroup and not once per wave.  Codes travel from memory one stage ahead in registers,
+// operands one stage ahead in LDS (two buffers, one barrier per stage).
 #include <algorithm>
+#include <cmath>
 
 #include "kv4.h"
 
@@ -12,6 +18,22 @@ namespace mi355 {
 namespace {
 
 constexpr int kWaves = 4;
+
+// How a stage is cut: steps per stage, and the part of it each of the four waves converts -- NB V blocks
+// of one step, and K operands [first, first + KF) of KT tiles.
+template <int D>
+struct Stage {
+  static constexpr int KS = D / 32;
+  static constexpr int SUB = D == 256 ? 1 : D == 128 ? 2 : 4;
+  static constexpr int NB = KS < 2 ? KS : 2;
+  static constexpr int KT = D <= 64 ? 2 : 1, KF = D <= 64 ? KS : 4;
+  static constexpr int kTokens = SUB * kKv4Step;
+  static __device__ __forceinline__ int v_step(int w) { return D == 256 ? 0 : D == 128 ? w / 2 : w; }
+  static __device__ __forceinline__ int v_block(int w) { return D == 256 ? 2 * w : D == 128 ? 2 * (w & 1) : 0; }
+  static __device__ __forceinline__ int k_step(int w) { return v_step(w); }
+  static __device__ __forceinline__ int k_tile(int w) { return D == 256 ? w / 2 : D == 128 ? (w & 1) : 0; }   // (the first of KT)
+  static __device__ __forceinline__ int k_first(int w) { return D == 256 ? 4 * (w & 1) : 0; }
+};
 
 struct Kv4PrefillParams {
   char* out;
@@ -23,32 +45,42 @@ struct Kv4PrefillParams {
   const int32_t* seg_pos0;
   int64_t q_stride;   // elements
   int nseg, Hq, Hkv, G, max_blocks, max_ctx, row_tiles;
-  float scale2;
+  float scale2, raise;   // |scale| * log2(e); kKv4Raise in units of a raw score
+  int flip;              // a negative scale: the queries are negated
 };
 
+// Between two waves' uses of LDS; global loads may stay in flight across it.
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 template <class Tag, int D, int MC>
-__global__ void __launch_bounds__(256) kv4_prefill_kernel(const Kv4PrefillParams p) {
-  constexpr int NP = Kv4Pieces<Tag>::n, KS = D / 32, EB = Tag::kBytes;
+__global__ void __launch_bounds__(256, 2) kv4_prefill_kernel(const Kv4PrefillParams p) {
+  typedef Stage<D> St;
+  constexpr int NP = Kv4Pieces<Tag>::n, KS = D / 32, EB = Tag::kBytes, SUB = St::SUB, NB = St::NB, KT = St::KT, KF = St::KF;
+  __shared__ bf16x8_t s_k[2][SUB][2][KS][64], s_v[2][SUB][KS][2][64];
+  __shared__ uint32_t s_nan[2][SUB][KS];   // tokens of a step whose V block was NaN (masked stages only)
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, col = lane & 15;
-  Kv4Lane<D> at(lane);
   int idx = blockIdx.x;
-  const int h = idx % p.Hkv;
+  const int h = idx % p.Hkv;   // (kv heads on neighbouring XCDs: the row tiles of one head share an L2 where Hkv is a multiple of 8)
   idx /= p.Hkv;
   const int seg = idx % p.nseg;
   const int rt = p.row_tiles - 1 - idx / p.nseg;   // the longest contexts first
   const int len = p.seg_len[seg], pos0 = p.seg_pos0[seg], q0 = p.seg_q0[seg];
-  const int rows = len * p.G;
-  const int row0 = (rt * kWaves + wave) * MC * 16;
-  if (row0 >= rows) return;   // (no barrier below)
+  const int rows = len * p.G, wg_row0 = rt * kWaves * MC * 16;
+  if (wg_row0 >= rows) return;
+  const int row0 = wg_row0 + wave * MC * 16;
 
-  int lim[MC];       // last position the column attends to
+  int lim[MC];       // last position the column attends to; -1: none
   int64_t orow[MC];  // its row of out (and of q), -1: none
   bf16x8_t qf[MC][KS][NP];
 #pragma unroll
   for (int mc = 0; mc < MC; ++mc) {
-    const int r = row0 + mc * 16 + col;
-    const int tok = min(r, rows - 1) / p.G, hq = h * p.G + min(r, rows - 1) % p.G;
+    const int r = row0 + mc * 16 + col, rr = min(r, rows - 1);
+    const int tok = rr / p.G, hq = h * p.G + rr % p.G;
     lim[mc] = min(pos0 + tok, p.max_ctx - 1);
     orow[mc] = r < rows ? (int64_t)(q0 + tok) * p.Hq + hq : -1;
     const char* src = p.q + ((int64_t)(q0 + tok) * p.q_stride + (int64_t)hq * D + g * (D / 4)) * EB;
@@ -56,144 +88,217 @@ __global__ void __launch_bounds__(256) kv4_prefill_kernel(const Kv4PrefillParams
     for (int s = 0; s < KS; ++s) {
       float x[8];
       load8<Tag>(src + s * 8 * EB, x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = p.flip ? -x[e] : x[e];
       bf16_pieces<NP>(x, qf[mc][s]);
     }
   }
-  const int first_lim = min(pos0 + row0 / p.G, p.max_ctx - 1);                                  // of the wave's first row
-  const int last_lim = min(pos0 + min(row0 + MC * 16 - 1, rows - 1) / p.G, p.max_ctx - 1);      // of its last one
+  auto limit = [&](int r) { return min(pos0 + min(r, rows - 1) / p.G, p.max_ctx - 1); };
+  const int wave_first = limit(row0), wave_last = row0 < rows ? limit(row0 + MC * 16 - 1) : -1;
+  const int wg_first = limit(wg_row0), wg_last = limit(wg_row0 + kWaves * MC * 16 - 1);
 
-  f32x4 acc[MC][KS][2];
-  float m[MC], l[MC];
+  f32x4 acc[MC][KS][2], sum[MC];
+  float m[MC], m2[MC];   // running maximum of the raw scores, and times the scale
 #pragma unroll
   for (int mc = 0; mc < MC; ++mc) {
-    m[mc] = kKv4Floor;
-    l[mc] = 0.f;
+    m[mc] = m2[mc] = kKv4Floor;
+    sum[mc] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int s = 0; s < KS; ++s) acc[mc][s][0] = acc[mc][s][1] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
+  bf16x8_t ones;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) ones[e] = (__bf16)1.f;
 
+  // ---- this wave's part of a stage
   const int32_t* table = p.bt + (int64_t)seg * p.max_blocks;
-  const int last_tile = max(last_lim, 0) / kKv4Tile;
-  auto record = [&](int tile) -> int64_t {
-    tile = min(tile, last_tile);
-    return kv4_record(p.cache, kv4_place(p.cache, table, tile), kv4_tile_bytes(D)) + (int64_t)h * p.cache.s_head;
+  const int last_tile = max(wg_last, 0) / kKv4Tile;
+  const int vstep = St::v_step(wave), vblk = St::v_block(wave), kstep = St::k_step(wave), ktile = St::k_tile(wave),
+            kfirst = St::k_first(wave);
+  uint32_t o_k, o_ks, o_v, o_vs, turn;   // the lane's places in a record
+  {
+    Kv4Lane<D> at(lane);
+    o_k = at.k + 4 * kfirst;
+    o_ks = at.ks;
+    o_v = at.v + 4 * vblk;
+    o_vs = at.vs + 4 * vblk;
+    turn = D == 256 && kfirst ? (at.turn + 8) & 31 : at.turn;
+  }
+  uint32_t rk[KT][KF], rks[KT], rv[2][NB], rvs[2][NB];
+  const char* const kbase = p.cache.k + (int64_t)h * p.cache.s_head;
+  const char* const vbase = p.cache.v + (int64_t)h * p.cache.s_head;
+  static_assert(KT == 2 || KT == 1, "");
+  Kv4Place n0{}, n1{};   // the next stage's records (of the step this wave converts), asked for a stage ahead
+  auto place = [&](int t0) {
+    const int tile = (int)((uint32_t)(t0 + vstep * kKv4Step) / kKv4Tile);
+    n0 = kv4_place(p.cache, table, min(tile, last_tile));
+    n1 = kv4_place(p.cache, table, min(tile + 1, last_tile));
   };
-
-  for (int t0 = 0; t0 <= last_lim; t0 += kKv4Step) {
-    Kv4TileRegs<D> T[2];
+  auto fetch = [&]() {
+    const int64_t r0 = kv4_record(p.cache, n0, kv4_tile_bytes(D)), r1 = kv4_record(p.cache, n1, kv4_tile_bytes(D));
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int64_t r = record(t0 / kKv4Tile + i);
-      kv4_load_k<D, false>(scalar_base(p.cache.k + r), at, T[i]);
-      kv4_load_v<D, false>(scalar_base(p.cache.v + r), at, T[i]);
+      gptr rec = scalar_base(vbase + (i ? r1 : r0));
+      load_words<false>(rec + lane_offset(o_v), rv[i]);
+      load_words<false>(rec + lane_offset(o_vs), rvs[i]);
     }
-    const bool masked = t0 + kKv4Step - 1 > first_lim;
-    f32x4 S[MC][2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-#pragma unroll
-      for (int mc = 0; mc < MC; ++mc) S[mc][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        const bf16x8_t a = kv4_k_frag(T[i].k[s], kv4_k_scale<D>(T[i], at, s));
-#pragma unroll
-        for (int mc = 0; mc < MC; ++mc)
-#pragma unroll
-          for (int n = 0; n < NP; ++n) S[mc][i] = mfma_bf16(a, qf[mc][s][n], S[mc][i]);
-      }
+    for (int i = 0; i < KT; ++i) {
+      gptr rec = scalar_base(kbase + ((KT == 2 ? i : ktile) ? r1 : r0));
+      uint32_t w[1];
+      load_words<false>(rec + lane_offset(o_k), rk[i]);
+      load_words<false>(rec + lane_offset(o_ks), w);
+      rks[i] = w[0];
     }
-    if (masked) {
-      // A value row some column must not see enters with weight 0, and 0 * NaN is NaN: rows behind the
-      // wave's last position count as 0, and NaN blocks are taken out of the product and added to the
-      // columns that do see them.
+  };
+  // Codes in registers -> operands in LDS, for the stage that starts at token t0.
+  auto convert = [&](int t0, int buf) {
+    if (t0 + St::kTokens - 1 > wg_first) {
+      // Some column must not see some of these value rows; they enter its product with weight 0, and 0 * NaN is
+      // NaN.  Rows behind the workgroup's last position count as 0; NaN blocks become 0 here and are put back,
+      // for the columns that see them, where the stage is used.
+      uint32_t nan[NB];
+#pragma unroll
+      for (int b = 0; b < NB; ++b) nan[b] = 0;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int first = t0 + i * kKv4Tile + 4 * g, live = last_lim + 1 - first;
+        const int live = wg_last + 1 - (t0 + vstep * kKv4Step + i * kKv4Tile + 4 * g);   // of this lane's four tokens
         const uint32_t keep = live >= 4 ? ~0u : (live <= 0 ? 0u : (1u << (8 * live)) - 1u);
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          uint32_t vs = (T[i].vs[s] & keep) | (0x7f7f7f7fu & ~keep);
-          T[i].v[s] &= keep;
-          uint32_t nan = 0;
+        for (int b = 0; b < NB; ++b) {
+          uint32_t vs = (rvs[i][b] & keep) | (0x7f7f7f7fu & ~keep), bad = 0;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) nan |= ((vs >> (8 * j)) & 0xffu) == 255u ? 0xffu << (8 * j) : 0u;
-          if (__ballot(nan != 0)) {
-            vs = (vs & ~nan) | (0x7f7f7f7fu & nan);
-            T[i].v[s] &= ~nan;
+          for (int j = 0; j < 4; ++j) {
+            const bool is_nan = ((vs >> (8 * j)) & 0xffu) == 255u;
+            const uint64_t all = __ballot(is_nan);   // lanes 0, 16, 32, 48 speak for tokens j, 4 + j, 8 + j, 12 + j
+            nan[b] |= (uint32_t)((all & 1) | (all >> 16 & 1) << 4 | (all >> 32 & 1) << 8 | (all >> 48 & 1) << 12) << (16 * i + j);
+            bad |= is_nan ? 0xffu << (8 * j) : 0u;
+          }
+          rv[i][b] &= keep & ~bad;
+          rvs[i][b] = (vs & ~bad) | (0x7f7f7f7fu & bad);
+        }
+      }
+      if (lane == 0) {
 #pragma unroll
-            for (int mc = 0; mc < MC; ++mc) {
-              // (a lane's scales are those of ITS four tokens; the column needs all sixteen of the tile)
-              int hit = 0;
+        for (int b = 0; b < NB; ++b) s_nan[buf][vstep][vblk + b] = nan[b];
+      }
+    }
 #pragma unroll
-              for (int gg = 0; gg < 4; ++gg) {
-                const uint32_t other = (uint32_t)__shfl((int)nan, gg * 16);
+    for (int i = 0; i < KT; ++i) {
+      const float sc = u2f(__builtin_amdgcn_alignbit(rks[i], rks[i], turn));
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                  hit |= ((other >> (8 * j)) & 1u) && t0 + i * kKv4Tile + 4 * gg + j <= lim[mc] ? 1 : 0;
-              }
-              if (hit) {
+      for (int f = 0; f < KF; ++f) s_k[buf][kstep][KT == 2 ? i : ktile][kfirst + f][lane] = kv4_k_frag(rk[i][f], sc);
+    }
 #pragma unroll
-                for (int e = 0; e < 4; ++e) acc[mc][s][0][e] = acc[mc][s][1][e] = __builtin_nanf("");
+    for (int b = 0; b < NB; ++b) {
+      bf16x8_t ev, od;
+      kv4_v_frags(rv[0][b], rv[1][b], rvs[0][b], rvs[1][b], ev, od);
+      s_v[buf][vstep][vblk + b][0][lane] = ev;
+      s_v[buf][vstep][vblk + b][1][lane] = od;
+    }
+  };
+
+  if (wg_last >= 0) {
+    place(0);
+    fetch();
+    place(St::kTokens);
+    convert(0, 0);
+    fetch();
+    place(2 * St::kTokens);
+    int buf = 0;
+    for (int t0 = 0; t0 <= wg_last; t0 += St::kTokens, buf ^= 1) {
+      lds_barrier();
+      convert(t0 + St::kTokens, buf ^ 1);   // (behind the last stage: the last tile again, read by nobody)
+      fetch();
+      place(min(t0 + 3 * St::kTokens, wg_last));
+      const bool wg_masked = t0 + St::kTokens - 1 > wg_first;
+#pragma unroll
+      for (int sub = 0; sub < SUB; ++sub) {
+        const int ts = t0 + sub * kKv4Step;
+        if (ts > wave_last) break;
+        const bool masked = ts + kKv4Step - 1 > wave_first;
+        f32x4 S[MC][2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+          for (int mc = 0; mc < MC; ++mc) S[mc][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int s = 0; s < KS; ++s) {
+            const bf16x8_t a = s_k[buf][sub][i][s][lane];
+#pragma unroll
+            for (int mc = 0; mc < MC; ++mc)
+#pragma unroll
+              for (int n = 0; n < NP; ++n) S[mc][i] = mfma_bf16(a, qf[mc][s][n], S[mc][i]);
+          }
+        }
+        if (wg_masked) {
+#pragma unroll
+          for (int s = 0; s < KS; ++s) {
+            const uint32_t nan = __builtin_amdgcn_readfirstlane(s_nan[buf][sub][s]);
+            if (nan) {
+#pragma unroll
+              for (int mc = 0; mc < MC; ++mc) {
+                const int seen = lim[mc] + 1 - ts;   // tokens of the step the column sees
+                const uint32_t sees = seen >= 32 ? ~0u : (seen <= 0 ? 0u : (1u << seen) - 1u);
+                if (nan & sees) {
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) acc[mc][s][0][e] = acc[mc][s][1][e] = __builtin_nanf("");
+                }
               }
             }
           }
-          T[i].vs[s] = vs;
         }
-      }
-    }
-    bf16x8_t pf[MC][NP];
+        bf16x8_t pf[MC][NP];
 #pragma unroll
-    for (int mc = 0; mc < MC; ++mc) {
-      float x[8];
+        for (int mc = 0; mc < MC; ++mc) {
+          float x[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = S[mc][e >> 2][e & 3] * p.scale2;
-      if (masked) {
+          for (int e = 0; e < 8; ++e) x[e] = S[mc][e >> 2][e & 3];
+          if (masked) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (t0 + (e >> 2) * kKv4Tile + 4 * g + (e & 3) > lim[mc]) x[e] = -INFINITY;
-      }
-      float top = x[0];
+            for (int e = 0; e < 8; ++e)
+              if (ts + (e >> 2) * kKv4Tile + 4 * g + (e & 3) > lim[mc]) x[e] = -INFINITY;
+          }
+          float top = fmaxf(fmaxf(x[0], x[1]), x[2]);
+          top = fmaxf(fmaxf(top, x[3]), x[4]);
+          top = fmaxf(fmaxf(top, x[5]), fmaxf(x[6], x[7]));
+          if (__ballot(top > m[mc] + p.raise)) {
+            top = fmaxf(top, __shfl_xor(top, 16));
+            top = fmaxf(top, __shfl_xor(top, 32));
+            const float mn = fmaxf(m[mc], top), f = fast_exp2((m[mc] - mn) * p.scale2);
+            m[mc] = mn;
+            m2[mc] = fmaxf(mn * p.scale2, kKv4Floor);
+            sum[mc] *= f;
 #pragma unroll
-      for (int e = 1; e < 8; ++e) top = fmaxf(top, x[e]);
-      if (__ballot(top > m[mc] + kKv4Raise)) {
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
-        const float mn = fmaxf(m[mc], top), f = fast_exp2(m[mc] - mn);
-        m[mc] = mn;
-        l[mc] *= f;
+            for (int s = 0; s < KS; ++s) {
+              acc[mc][s][0] *= f;
+              acc[mc][s][1] *= f;
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = fast_exp2(__builtin_fmaf(x[e], p.scale2, -m2[mc]));
+          bf16_pieces<NP>(x, pf[mc]);
+#pragma unroll
+          for (int n = 0; n < NP; ++n) sum[mc] = mfma_bf16(ones, pf[mc][n], sum[mc]);   // every row: the column's sum of weights
+        }
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
-          acc[mc][s][0] *= f;
-          acc[mc][s][1] *= f;
+          const bf16x8_t ev = s_v[buf][sub][s][0][lane], od = s_v[buf][sub][s][1][lane];
+#pragma unroll
+          for (int mc = 0; mc < MC; ++mc)
+#pragma unroll
+            for (int n = 0; n < NP; ++n) {
+              acc[mc][s][0] = mfma_bf16(ev, pf[mc][n], acc[mc][s][0]);
+              acc[mc][s][1] = mfma_bf16(od, pf[mc][n], acc[mc][s][1]);
+            }
         }
       }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        x[e] = fast_exp2(x[e] - m[mc]);
-        l[mc] += x[e];
-      }
-      bf16_pieces<NP>(x, pf[mc]);
-    }
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      bf16x8_t ev, od;
-      kv4_v_frags(T[0].v[s], T[1].v[s], T[0].vs[s], T[1].vs[s], ev, od);
-#pragma unroll
-      for (int mc = 0; mc < MC; ++mc)
-#pragma unroll
-        for (int n = 0; n < NP; ++n) {
-          acc[mc][s][0] = mfma_bf16(ev, pf[mc][n], acc[mc][s][0]);
-          acc[mc][s][1] = mfma_bf16(od, pf[mc][n], acc[mc][s][1]);
-        }
     }
   }
 
 #pragma unroll
   for (int mc = 0; mc < MC; ++mc) {
-    float L = l[mc];
-    L += __shfl_xor(L, 16);
-    L += __shfl_xor(L, 32);
-    const float inv = lim[mc] >= 0 ? 1.f / L : 0.f;   // a query before position 0 sees nothing: zeros
+    const float inv = lim[mc] >= 0 ? 1.f / sum[mc][0] : 0.f;   // a query before position 0 sees nothing: zeros
     if (orow[mc] < 0) continue;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
@@ -275,7 +380,9 @@ extern "C" int mi355_paged_prefill_kv4(void* out, const void* q, int64_t q_strid
   p.max_blocks = max_blocks;
   p.max_ctx = max_context;
   p.row_tiles = 0;
-  p.scale2 = scale * 1.44269504088896340736f;
+  p.flip = scale < 0.f;
+  p.scale2 = std::max(std::fabs(scale) * 1.44269504088896340736f, 1e-30f);   // (a scale of 0: all weights 1 to 30 digits)
+  p.raise = kKv4Raise / p.scale2;
   hipStream_t s = static_cast<hipStream_t>(stream);
   switch (dtype) {
     case MI355_F32: return launch<F32>(p, D, max_q_len, s);
