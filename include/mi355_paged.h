@@ -523,14 +523,20 @@ size_t mi355_paged_decode_kv4_workspace_bytes(int32_t B, int32_t Hq, int32_t Hkv
  * mi355_paged_prefill over the 4-bit cache: query token j of segment s attends to positions
  * 0 .. seg_pos0[s] + j, whose rows (the segment's own among them) are in the cache.  Rows of out
  * outside every segment are left as they are; a segment may be empty.  A value row that a query must
- * not see never reaches it, NaN or not.  Precision as in mi355_paged_decode_kv4.
+ * not see never reaches it, NaN or not.  Precision as in mi355_paged_decode_kv4.  total_rows: the tokens
+ * q and out hold; every segment lies within them.
  */
 int mi355_paged_prefill_kv4(void* out, const void* q, int64_t q_stride_tok, const void* k_cache,
                             const void* v_cache, const int32_t* block_tables, const int32_t* seg_q_start,
-                            const int32_t* seg_len, const int32_t* seg_pos0, int32_t nseg, int32_t max_q_len,
-                            int32_t Hq, int32_t Hkv, int32_t D, int32_t block_size, int32_t max_blocks,
-                            int32_t num_blocks, int32_t max_context, int64_t stride_block, int64_t stride_head,
-                            float scale, int32_t dtype, void* workspace, size_t workspace_bytes, void* stream);
+                            const int32_t* seg_len, const int32_t* seg_pos0, int32_t nseg, int32_t total_rows,
+                            int32_t max_q_len, int32_t Hq, int32_t Hkv, int32_t D, int32_t block_size,
+                            int32_t max_blocks, int32_t num_blocks, int32_t max_context, int64_t stride_block,
+                            int64_t stride_head, float scale, int32_t dtype, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
+/* Scratch bytes mi355_paged_prefill_kv4 needs for this shape (max_context after its clamp; total_rows =
+ * tokens of q): few query rows behind a long context are split over workgroups.  Nothing is kept in it
+ * between calls, and calls that may overlap on the GPU must not share it. */
 size_t mi355_paged_prefill_kv4_workspace_bytes(int32_t nseg, int32_t total_rows, int32_t max_q_len, int32_t Hq,
                                                int32_t Hkv, int32_t D, int32_t max_context, int32_t dtype);
 

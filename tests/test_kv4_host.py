@@ -1,7 +1,6 @@
 """The 4-bit KV cache without a GPU: the checker's format against hand-worked values, the host-side
 arithmetic of rope_frequencies, and every refusal of the C entry points (argument checks come before
 any device work)."""
-import ctypes
 import math
 
 import numpy as np
@@ -106,7 +105,7 @@ WRITE = dict(q_out=P, q=P, k=P, v=P, qs=1536, ks=1536, vs=1536, cos=P, sin=P, R=
 READ = dict(ko=P, vo=P, kc=P, vc=P, slots=P, T=4, Hkv=8, D=64, BS=16, NB=10, sb=8 * 544, sh=544, dtype=1, stream=None)
 DECODE = dict(out=P, q=P, qs=512, kc=P, vc=P, bt=P, ctx=P, B=2, Hq=8, Hkv=8, D=64, BS=16, mb=4, NB=10, max_ctx=64,
               sb=8 * 544, sh=544, scale=0.125, dtype=1, ws=P, wsb=1 << 30, stream=None)
-CHUNK = dict(out=P, q=P, qs=512, kc=P, vc=P, bt=P, q0=P, ln=P, pos=P, nseg=2, max_q=8, Hq=8, Hkv=8, D=64, BS=16, mb=4,
+CHUNK = dict(out=P, q=P, qs=512, kc=P, vc=P, bt=P, q0=P, ln=P, pos=P, nseg=2, rows=16, max_q=8, Hq=8, Hkv=8, D=64, BS=16, mb=4,
              NB=10, max_ctx=64, sb=8 * 544, sh=544, scale=0.125, dtype=1, ws=P, wsb=1 << 30, stream=None)
 CACHE = [(dict(kc=None), -1), (dict(vc=None), -1), (dict(kc=P + 8), -1), (dict(D=16), -2), (dict(D=96), -2), (dict(BS=8), -2),
          (dict(BS=24), -2), (dict(BS=0), -2), (dict(NB=0), -1), (dict(Hkv=0), -1), (dict(sh=540), -1), (dict(sb=8), -1),
@@ -128,11 +127,13 @@ REFUSED = (
         (dict(out=None), -1), (dict(q=None), -1), (dict(bt=None), -1), (dict(ctx=None), -1), (dict(qs=504), -1), (dict(qs=516), -1),
         (dict(q=P + 8), -1), (dict(Hq=12), -1), (dict(Hq=0), -1), (dict(B=-1), -1), (dict(mb=0), -1), (dict(max_ctx=-1), -1),
         (dict(max_ctx=100000, mb=7000, ws=None), -3), (dict(max_ctx=100000, mb=7000, wsb=64), -3),
-        (dict(max_ctx=100000, mb=7000, ws=P + 4), -3)]] +
+        (dict(max_ctx=100000, mb=7000, ws=P + 4), -3), (dict(max_ctx=1 << 30, mb=1 << 27), -1)]] +
     [('mi355_paged_prefill_kv4', CHUNK, c, r) for c, r in CACHE + [
         (dict(out=None), -1), (dict(q=None), -1), (dict(bt=None), -1), (dict(q0=None), -1), (dict(ln=None), -1), (dict(pos=None), -1),
         (dict(qs=504), -1), (dict(q=P + 8), -1), (dict(Hq=12), -1), (dict(nseg=-1), -1), (dict(max_q=-1), -1), (dict(mb=0), -1),
-        (dict(max_ctx=0), -1), (dict(max_q=1 << 30, Hq=64, qs=4096), -1)]])
+        (dict(max_ctx=0), -1), (dict(max_q=1 << 30, Hq=64, qs=4096), -1), (dict(rows=-1), -1),
+        (dict(max_ctx=100000, mb=7000, ws=None), -3), (dict(max_ctx=100000, mb=7000, wsb=64), -3),
+        (dict(max_ctx=100000, mb=7000, ws=P + 4), -3), (dict(max_ctx=1 << 30, mb=1 << 27), -1)]])
 
 
 @pytest.mark.parametrize('name,good,change,want', REFUSED, ids=lambda v: str(v)[:40])
@@ -156,7 +157,8 @@ def test_workspace_queries_are_host_arithmetic():
     assert lib.mi355_paged_decode_kv4_workspace_bytes(1, 8, 8, 64, 37, 1) == 0            # one split
     assert lib.mi355_paged_decode_kv4_workspace_bytes(1, 8, 8, 64, 100000, 1) > 0
     assert lib.mi355_paged_decode_kv4_workspace_bytes(1, 8, 8, 48, 100000, 1) == 0        # refused: the call says why
-    assert ctypes.c_size_t(lib.mi355_paged_prefill_kv4_workspace_bytes(1, 8, 8, 8, 8, 64, 100000, 1)).value >= 0
+    assert lib.mi355_paged_prefill_kv4_workspace_bytes(1, 8, 8, 8, 8, 64, 100000, 1) > 0
+    assert lib.mi355_paged_prefill_kv4_workspace_bytes(8, 8192, 1024, 8, 8, 64, 1024, 1) == 0
 
 
 def test_ops_refuse_host_tensors():

@@ -260,4 +260,55 @@ __device__ __forceinline__ float kv4_k_scale(const Kv4TileRegs<D>& t, const Kv4L
   return u2f(__builtin_amdgcn_alignbit(t.ks, t.ks, turn));
 }
 
+// Joins a row's `n` split records of D + 4 floats (unnormalised sums, running maximum, sum of weights)
+// and stores the row.  A thread owns eight dims and every SL-th split, SL * D / 8 threads a row; with
+// SL > 1 the row is the whole workgroup's (256 threads) and its threads of the same dims meet in LDS.
+// The records of a row lie a memory latency apart when one thread walks them (32 splits of 128 dims:
+// 25 us), but a workgroup per row is too much for thousands of rows of a few splits (12 prompts of 64
+// dims in two splits: 162 us in all, 48 unsplit): kv4_split_lanes picks by the number of splits.
+constexpr int kKv4WalkedSplits = 8;
+template <int D>
+constexpr int kv4_split_lanes(bool walked) { return walked ? 1 : 256 / (D / 8); }
+template <class Tag, int D, int SL>
+__device__ inline void kv4_join_splits(char* out, const float* ws, int n) {
+  constexpr int P = D / 8;
+  __shared__ float s_m[SL][P], s_l[SL][P], s_o[SL][P][9];   // (9: neighbouring threads on neighbouring banks)
+  const int piece = threadIdx.x % P, sl = SL == 1 ? 0 : threadIdx.x / P;
+  float M = kKv4Floor, L = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  auto join = [&](float ms, float ls, const float (&x)[8]) {
+    const float Mn = fmaxf(M, ms), fo = fast_exp2(M - Mn), fn = fast_exp2(ms - Mn);
+    M = Mn;
+    L = __builtin_fmaf(ls, fn, L * fo);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = __builtin_fmaf(x[e], fn, o[e] * fo);
+  };
+#pragma unroll 4
+  for (int s = sl; s < n; s += SL) {
+    const float* rec = ws + (int64_t)s * (D + 4);
+    float x[8];
+    load8<F32>(reinterpret_cast<const char*>(rec + piece * 8), x);
+    join(rec[D], rec[D + 1], x);
+  }
+  for (int half = SL / 2; half > 0; half /= 2) {
+    if (sl >= half && sl < 2 * half) {
+      s_m[sl][piece] = M;
+      s_l[sl][piece] = L;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s_o[sl][piece][e] = o[e];
+    }
+    __syncthreads();
+    if (sl < half) {
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = s_o[sl + half][piece][e];
+      join(s_m[sl + half][piece], s_l[sl + half][piece], x);
+    }
+  }
+  if (sl != 0) return;
+  const float inv = n > 0 ? 1.f / L : 0.f;   // no token at all: zeros
+#pragma unroll
+  for (int e = 0; e < 8; ++e) o[e] = n > 0 ? o[e] * inv : 0.f;
+  store8<Tag>(out + piece * 8 * Tag::kBytes, o);
+}
+
 }  // namespace mi355

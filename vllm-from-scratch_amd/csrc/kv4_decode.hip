@@ -25,8 +25,7 @@ struct Kv4DecodeParams {
   Kv4Cache cache;
   const int32_t* bt;
   const int32_t* ctx;
-  float* ws_acc;   // [B * Hq][nsplit][D]
-  float* ws_ml;    // [B * Hq][nsplit][2]
+  float* ws;   // [B * Hq][nsplit][D + 4]: unnormalised sums, running maximum, sum of weights
   int64_t q_stride;   // elements
   int B, Hq, Hkv, G /* query heads per kv head */, gc /* of them per workgroup */, qchunks, hgroups;
   int max_blocks, max_ctx, nsplit, tps /* tokens per split */;
@@ -243,64 +242,28 @@ __global__ void __launch_bounds__(W * 64) kv4_decode_kernel(const Kv4DecodeParam
       for (int e = 0; e < 8; ++e) o[e] = ctx > 0 ? o[e] * inv : 0.f;
       store8<Tag>(p.out + (row * D + d) * EB, o);
     } else {
-      float* dst = p.ws_acc + (row * p.nsplit + sp) * D + d;
-      *reinterpret_cast<f32x4*>(dst) = f32x4{o[0], o[1], o[2], o[3]};
-      *reinterpret_cast<f32x4*>(dst + 4) = f32x4{o[4], o[5], o[6], o[7]};
-      if (d == 0) {
-        p.ws_ml[(row * p.nsplit + sp) * 2] = M;
-        p.ws_ml[(row * p.nsplit + sp) * 2 + 1] = L;
-      }
+      float* rec = p.ws + (row * p.nsplit + sp) * (D + 4);
+      *reinterpret_cast<f32x4*>(rec + d) = f32x4{o[0], o[1], o[2], o[3]};
+      *reinterpret_cast<f32x4*>(rec + d + 4) = f32x4{o[4], o[5], o[6], o[7]};
+      if (d == 0) *reinterpret_cast<f32x4*>(rec + D) = f32x4{M, L, 0.f, 0.f};
     }
   }
 }
 
-// Joins the splits of a row, one workgroup each: a thread owns eight dims and every SL-th split (the
-// records of a long row lie a memory latency apart when one thread walks them all: 32 splits of 128
-// dims took 25 us that way), then the threads of the same dims meet in LDS.
-template <class Tag, int D>
+template <class Tag, int D, int SL>
 __global__ void __launch_bounds__(256)
-kv4_merge_kernel(char* out, const float* ws_acc, const float* ws_ml, const int32_t* ctx_lens, int Hq, int max_ctx,
-                 int nsplit, int tps) {
-  constexpr int P = D / 8, SL = 256 / P;
-  __shared__ float s_m[SL][P], s_l[SL][P], s_o[SL][P][9];   // (9: neighbouring threads on neighbouring banks)
-  const int64_t row = blockIdx.x;
-  const int piece = threadIdx.x % P, sl = threadIdx.x / P;
+kv4_merge_kernel(char* out, const float* ws, const int32_t* ctx_lens, int rows, int Hq, int max_ctx, int nsplit, int tps) {
+  const int64_t row = (int64_t)blockIdx.x * (256 / (SL * D / 8)) + (SL == 1 ? threadIdx.x / (D / 8) : 0);
+  if (row >= rows) return;
   const int ctx = min(ctx_lens[row / Hq], max_ctx);
-  const int n = ctx <= 0 ? 0 : min(nsplit, (ctx + tps - 1) / tps);
-  float M = kKv4Floor, L = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  auto join = [&](float ms, float ls, const float (&x)[8]) {
-    const float Mn = fmaxf(M, ms), fo = fast_exp2(M - Mn), fn = fast_exp2(ms - Mn);
-    M = Mn;
-    L = __builtin_fmaf(ls, fn, L * fo);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] = __builtin_fmaf(x[e], fn, o[e] * fo);
-  };
-#pragma unroll 2
-  for (int s = sl; s < n; s += SL) {
-    float x[8];
-    load8<F32>(reinterpret_cast<const char*>(ws_acc + (row * nsplit + s) * D + piece * 8), x);
-    join(ws_ml[(row * nsplit + s) * 2], ws_ml[(row * nsplit + s) * 2 + 1], x);
-  }
-  for (int half = SL / 2; half > 0; half /= 2) {
-    if (sl >= half && sl < 2 * half) {
-      s_m[sl][piece] = M;
-      s_l[sl][piece] = L;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) s_o[sl][piece][e] = o[e];
-    }
-    __syncthreads();
-    if (sl < half) {
-      float x[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = s_o[sl + half][piece][e];
-      join(s_m[sl + half][piece], s_l[sl + half][piece], x);
-    }
-  }
-  if (sl != 0) return;
-  const float inv = n > 0 ? 1.f / L : 0.f;   // no token at all: zeros
-#pragma unroll
-  for (int e = 0; e < 8; ++e) o[e] *= inv;
-  store8<Tag>(out + (row * D + piece * 8) * Tag::kBytes, o);
+  kv4_join_splits<Tag, D, SL>(out + row * D * Tag::kBytes, ws + row * nsplit * (D + 4),
+                              ctx <= 0 ? 0 : min(nsplit, (ctx + tps - 1) / tps));
+}
+template <class Tag, int D, int SL>
+void launch_merge(const Kv4DecodeParams& p, hipStream_t s) {
+  const int rows = p.B * p.Hq;
+  hipLaunchKernelGGL((kv4_merge_kernel<Tag, D, SL>), dim3((unsigned)ceil_div64(rows, 256 / (SL * D / 8))), dim3(256), 0, s,
+                     p.out, p.ws, p.ctx, rows, p.Hq, p.max_ctx, p.nsplit, p.tps);
 }
 
 struct Kv4Plan {
@@ -340,7 +303,7 @@ int make_plan(const char* what, int B, int Hq, int Hkv, int D, int max_ctx, int 
   const int64_t rounds = std::max<int64_t>(1, ((int64_t)max_ctx + round - 1) / round), per = (rounds + want - 1) / want;
   pl->tps = (int)(per * round);
   pl->nsplit = (int)((rounds + per - 1) / per);
-  pl->ws_bytes = pl->nsplit > 1 ? (size_t)B * Hq * pl->nsplit * (D + 2) * sizeof(float) : 0;
+  pl->ws_bytes = pl->nsplit > 1 ? (size_t)B * Hq * pl->nsplit * (D + 4) * sizeof(float) : 0;
   return 0;
 }
 
@@ -360,8 +323,8 @@ int launch(const Kv4DecodeParams& p, const Kv4Plan& pl, hipStream_t s) {
   }
   if (int rc = check_launch("kv4_decode_kernel")) return rc;
   if (p.nsplit > 1) {
-    hipLaunchKernelGGL((kv4_merge_kernel<Tag, D>), dim3((unsigned)(p.B * p.Hq)), dim3(256), 0, s, p.out, p.ws_acc, p.ws_ml,
-                       p.ctx, p.Hq, p.max_ctx, p.nsplit, p.tps);
+    if (p.nsplit <= kKv4WalkedSplits) launch_merge<Tag, D, kv4_split_lanes<D>(true)>(p, s);
+    else launch_merge<Tag, D, kv4_split_lanes<D>(false)>(p, s);
     return check_launch("kv4_merge_kernel");
   }
   return 0;
@@ -416,8 +379,7 @@ extern "C" int mi355_paged_decode_kv4(void* out, const void* q, int64_t q_stride
   p.cache = kv4_cache(k_cache, v_cache, stride_block, stride_head, num_blocks, block_size / kKv4Tile);
   p.bt = block_tables;
   p.ctx = context_lens;
-  p.ws_acc = static_cast<float*>(workspace);
-  p.ws_ml = p.ws_acc ? p.ws_acc + (size_t)B * Hq * pl.nsplit * D : nullptr;
+  p.ws = static_cast<float*>(workspace);
   p.q_stride = q_stride_seq;
   p.B = B;
   p.Hq = Hq;

@@ -24,14 +24,13 @@ constexpr int kWaves = 4;
 template <int D>
 struct Stage {
   static constexpr int KS = D / 32;
-  static constexpr int SUB = D == 256 ? 1 : D == 128 ? 2 : 4;
-  static constexpr int NB = KS < 2 ? KS : 2;
-  static constexpr int KT = D <= 64 ? 2 : 1, KF = D <= 64 ? KS : 4;
+  static constexpr int SUB = D == 256 ? 1 : D == 32 ? 4 : 2;
+  static constexpr int NB = D <= 64 ? 1 : 2;
+  static constexpr int KT = D == 32 ? 2 : 1, KF = D <= 64 ? KS : 4;
   static constexpr int kTokens = SUB * kKv4Step;
-  static __device__ __forceinline__ int v_step(int w) { return D == 256 ? 0 : D == 128 ? w / 2 : w; }
-  static __device__ __forceinline__ int v_block(int w) { return D == 256 ? 2 * w : D == 128 ? 2 * (w & 1) : 0; }
-  static __device__ __forceinline__ int k_step(int w) { return v_step(w); }
-  static __device__ __forceinline__ int k_tile(int w) { return D == 256 ? w / 2 : D == 128 ? (w & 1) : 0; }   // (the first of KT)
+  static __device__ __forceinline__ int step(int w) { return D == 256 ? 0 : D == 32 ? w : w / 2; }
+  static __device__ __forceinline__ int v_block(int w) { return D == 256 ? 2 * w : D == 32 ? 0 : NB * (w & 1); }
+  static __device__ __forceinline__ int k_tile(int w) { return D == 256 ? w / 2 : D == 32 ? 0 : w & 1; }   // (the first of KT)
   static __device__ __forceinline__ int k_first(int w) { return D == 256 ? 4 * (w & 1) : 0; }
 };
 
@@ -44,7 +43,8 @@ struct Kv4PrefillParams {
   const int32_t* seg_len;
   const int32_t* seg_pos0;
   int64_t q_stride;   // elements
-  int nseg, Hq, Hkv, G, max_blocks, max_ctx, row_tiles;
+  float* ws;   // [total rows * Hq][nsplit][D + 4]: unnormalised sums, running maximum, sum of weights
+  int nseg, Hq, Hkv, G, max_blocks, max_ctx, row_tiles, nsplit, tps /* tokens per split, whole stages */;
   float scale2, raise;   // |scale| * log2(e); kKv4Raise in units of a raw score
   int flip;              // a negative scale: the queries are negated
 };
@@ -60,11 +60,14 @@ template <class Tag, int D, int MC>
 __global__ void __launch_bounds__(256, 2) kv4_prefill_kernel(const Kv4PrefillParams p) {
   typedef Stage<D> St;
   constexpr int NP = Kv4Pieces<Tag>::n, KS = D / 32, EB = Tag::kBytes, SUB = St::SUB, NB = St::NB, KT = St::KT, KF = St::KF;
+  constexpr int KA = KS < 4 ? KS : 4, VA = KS < 2 ? KS : 2;   // operands read ahead of their use
   __shared__ bf16x8_t s_k[2][SUB][2][KS][64], s_v[2][SUB][KS][2][64];
   __shared__ uint32_t s_nan[2][SUB][KS];   // tokens of a step whose V block was NaN (masked stages only)
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, col = lane & 15;
   int idx = blockIdx.x;
+  const int sp = idx % p.nsplit;
+  idx /= p.nsplit;
   const int h = idx % p.Hkv;   // (kv heads on neighbouring XCDs: the row tiles of one head share an L2 where Hkv is a multiple of 8)
   idx /= p.Hkv;
   const int seg = idx % p.nseg;
@@ -95,7 +98,9 @@ __global__ void __launch_bounds__(256, 2) kv4_prefill_kernel(const Kv4PrefillPar
   }
   auto limit = [&](int r) { return min(pos0 + min(r, rows - 1) / p.G, p.max_ctx - 1); };
   const int wave_first = limit(row0), wave_last = row0 < rows ? limit(row0 + MC * 16 - 1) : -1;
-  const int wg_first = limit(wg_row0), wg_last = limit(wg_row0 + kWaves * MC * 16 - 1);
+  const int wg_first = limit(wg_row0), wg_end = limit(wg_row0 + kWaves * MC * 16 - 1);
+  const int lo = sp * p.tps, wg_last = min(wg_end, lo + p.tps - 1);   // this workgroup's tokens: lo .. wg_last
+  if (lo > wg_last && sp > 0) return;                                 // (the rows' own limits tell which splits are empty)
 
   f32x4 acc[MC][KS][2], sum[MC];
   float m[MC], m2[MC];   // running maximum of the raw scores, and times the scale
@@ -113,7 +118,7 @@ __global__ void __launch_bounds__(256, 2) kv4_prefill_kernel(const Kv4PrefillPar
   // ---- this wave's part of a stage
   const int32_t* table = p.bt + (int64_t)seg * p.max_blocks;
   const int last_tile = max(wg_last, 0) / kKv4Tile;
-  const int vstep = St::v_step(wave), vblk = St::v_block(wave), kstep = St::k_step(wave), ktile = St::k_tile(wave),
+  const int vstep = St::step(wave), vblk = St::v_block(wave), kstep = vstep, ktile = St::k_tile(wave),
             kfirst = St::k_first(wave);
   uint32_t o_k, o_ks, o_v, o_vs, turn;   // the lane's places in a record
   {
@@ -198,15 +203,15 @@ __global__ void __launch_bounds__(256, 2) kv4_prefill_kernel(const Kv4PrefillPar
     }
   };
 
-  if (wg_last >= 0) {
-    place(0);
+  if (wg_last >= lo) {
+    place(lo);
     fetch();
-    place(St::kTokens);
-    convert(0, 0);
+    place(lo + St::kTokens);
+    convert(lo, 0);
     fetch();
-    place(2 * St::kTokens);
+    place(lo + 2 * St::kTokens);
     int buf = 0;
-    for (int t0 = 0; t0 <= wg_last; t0 += St::kTokens, buf ^= 1) {
+    for (int t0 = lo; t0 <= wg_last; t0 += St::kTokens, buf ^= 1) {
       lds_barrier();
       convert(t0 + St::kTokens, buf ^ 1);   // (behind the last stage: the last tile again, read by nobody)
       fetch();
@@ -218,19 +223,32 @@ __global__ void __launch_bounds__(256, 2) kv4_prefill_kernel(const Kv4PrefillPar
         if (ts > wave_last) break;
         const bool masked = ts + kKv4Step - 1 > wave_first;
         f32x4 S[MC][2];
+        bf16x8_t kf[2][KA];   // K operands, read 2 KA ahead
+#pragma unroll
+        for (int f = 0; f < 2 * KA; ++f) kf[f / KA][f % KA] = s_k[buf][sub][f / KS][f % KS][lane];
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
 #pragma unroll
           for (int mc = 0; mc < MC; ++mc) S[mc][i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int s = 0; s < KS; ++s) {
-            const bf16x8_t a = s_k[buf][sub][i][s][lane];
+            const int f = i * KS + s;
+            const bf16x8_t a = kf[f / KA % 2][f % KA];
+            if (f + 2 * KA < 2 * KS) kf[f / KA % 2][f % KA] = s_k[buf][sub][(f + 2 * KA) / KS][(f + 2 * KA) % KS][lane];
 #pragma unroll
             for (int mc = 0; mc < MC; ++mc)
 #pragma unroll
               for (int n = 0; n < NP; ++n) S[mc][i] = mfma_bf16(a, qf[mc][s][n], S[mc][i]);
           }
         }
+        bf16x8_t vf[VA][2];   // V operands of the first blocks, on their way during the softmax
+#pragma unroll
+        for (int s = 0; s < VA; ++s) {
+          vf[s][0] = s_v[buf][sub][s][0][lane];
+          vf[s][1] = s_v[buf][sub][s][1][lane];
+        }
+        __builtin_amdgcn_sched_barrier(0);
         if (wg_masked) {
 #pragma unroll
           for (int s = 0; s < KS; ++s) {
@@ -283,7 +301,11 @@ __global__ void __launch_bounds__(256, 2) kv4_prefill_kernel(const Kv4PrefillPar
         }
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
-          const bf16x8_t ev = s_v[buf][sub][s][0][lane], od = s_v[buf][sub][s][1][lane];
+          const bf16x8_t ev = vf[s % VA][0], od = vf[s % VA][1];
+          if (s + VA < KS) {
+            vf[s % VA][0] = s_v[buf][sub][s + VA][0][lane];
+            vf[s % VA][1] = s_v[buf][sub][s + VA][1][lane];
+          }
 #pragma unroll
           for (int mc = 0; mc < MC; ++mc)
 #pragma unroll
@@ -298,8 +320,19 @@ __global__ void __launch_bounds__(256, 2) kv4_prefill_kernel(const Kv4PrefillPar
 
 #pragma unroll
   for (int mc = 0; mc < MC; ++mc) {
-    const float inv = lim[mc] >= 0 ? 1.f / sum[mc][0] : 0.f;   // a query before position 0 sees nothing: zeros
     if (orow[mc] < 0) continue;
+    if (p.nsplit > 1) {
+      float* rec = p.ws + (orow[mc] * p.nsplit + sp) * (D + 4);
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const f32x4 e = acc[mc][s][0], o = acc[mc][s][1];
+        *reinterpret_cast<f32x4*>(rec + 32 * s + 8 * g) = f32x4{e[0], o[0], e[1], o[1]};
+        *reinterpret_cast<f32x4*>(rec + 32 * s + 8 * g + 4) = f32x4{e[2], o[2], e[3], o[3]};
+      }
+      if (g == 0) *reinterpret_cast<f32x4*>(rec + D) = f32x4{m2[mc], sum[mc][0], 0.f, 0.f};
+      continue;
+    }
+    const float inv = lim[mc] >= 0 ? 1.f / sum[mc][0] : 0.f;   // a query before position 0 sees nothing: zeros
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       const f32x4 e = acc[mc][s][0], o = acc[mc][s][1];
@@ -311,23 +344,90 @@ __global__ void __launch_bounds__(256, 2) kv4_prefill_kernel(const Kv4PrefillPar
   }
 }
 
+// Joins the splits of the segments' query rows; items are (segment, token, query head).
+template <class Tag, int D, int SL>
+__global__ void __launch_bounds__(256) kv4_prefill_merge_kernel(const Kv4PrefillParams p, int max_q_len, int64_t items) {
+  const int64_t item = (int64_t)blockIdx.x * (256 / (SL * D / 8)) + (SL == 1 ? threadIdx.x / (D / 8) : 0);
+  if (item >= items) return;
+  const int hq = (int)(item % p.Hq);
+  const int64_t st = item / p.Hq;
+  const int tok = (int)(st % max_q_len), seg = (int)(st / max_q_len);
+  if (tok >= p.seg_len[seg]) return;
+  const int lim = min(p.seg_pos0[seg] + tok, p.max_ctx - 1);
+  const int64_t row = (int64_t)(p.seg_q0[seg] + tok) * p.Hq + hq;
+  kv4_join_splits<Tag, D, SL>(p.out + row * D * Tag::kBytes, p.ws + row * p.nsplit * (D + 4),
+                              lim < 0 ? 0 : min(lim / p.tps + 1, p.nsplit));
+}
+template <class Tag, int D, int SL>
+void launch_merge(const Kv4PrefillParams& p, int max_q_len, hipStream_t s) {
+  const int64_t items = (int64_t)p.nseg * max_q_len * p.Hq;
+  hipLaunchKernelGGL((kv4_prefill_merge_kernel<Tag, D, SL>), dim3((unsigned)ceil_div64(items, 256 / (SL * D / 8))), dim3(256), 0,
+                     s, p, max_q_len, items);
+}
+
+struct Kv4PrefillPlan {
+  int MC, row_tiles, nsplit, tps;
+  size_t ws_bytes;
+};
+
+// Host arithmetic only.
+int make_plan(const char* what, int nseg, int total_rows, int max_q_len, int Hq, int Hkv, int D, int max_ctx, int dtype,
+              Kv4PrefillPlan* pl) {
+  if (!kv4_dtype_ok(dtype)) return fail(MI355_EINVAL, "%s: dtype %d", what, dtype);
+  if (!kv4_head_dim_ok(D)) return fail(MI355_EUNSUPPORTED, "%s: head_dim %d (the 4-bit cache holds 32, 64, 128 or 256)", what, D);
+  if (nseg < 0 || total_rows < 0 || max_q_len < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || max_ctx <= 0 || max_ctx > kKv4MaxContext)
+    return fail(MI355_EINVAL, "%s: bad shape (nseg=%d total_rows=%d max_q_len=%d Hq=%d Hkv=%d max_context=%d)", what, nseg,
+                total_rows, max_q_len, Hq, Hkv, max_ctx);
+  const int64_t rows = (int64_t)max_q_len * (Hq / Hkv), heads = (int64_t)std::max(nseg, 1) * Hkv;
+  if (rows > INT32_MAX) return fail(MI355_EINVAL, "%s: max_q_len %d", what, max_q_len);
+  // Two tiles of 16 rows per wave use every converted operand twice, one tile makes twice the workgroups.  Figures: us, two /
+  // one.  head_dim 64: 8 prompts of 4096 168 / 193, 16 uneven chunks to 1024 46 / 42; head_dim 128: 8 prompts of 1024
+  // 37 / 42, 4 of 300 with 32/8 heads 32 / 38, 4 of 300 with 8 heads 28 / 22; 2 of 256 behind 3000, split, 51 / 56.
+  // Two tiles' registers at head_dim 256 (fp32: 128) would leave one wave per SIMD.
+  const bool narrow = D == 256 || (dtype == MI355_F32 && D == 128);
+  const int64_t wgs2 = heads * ceil_div64(rows, kWaves * 32);
+  pl->MC = !narrow && (wgs2 >= (D == 128 ? 256 : 1024) || (D == 128 && wgs2 >= 128 && max_ctx >= 2048)) ? 2 : 1;
+  pl->row_tiles = (int)ceil_div64(rows, kWaves * pl->MC * 16);
+  const int64_t wgs = heads * pl->row_tiles;
+  const int stage = kKv4Step * (D == 256 ? 1 : D == 32 ? 4 : 2);
+  const int64_t stages = ceil_div64(max_ctx, stage);
+  // Few workgroups behind a long context: the context is split until there are two per CU, no split shorter than 256 tokens
+  // (16 tokens behind 30000, 32/8 heads of 128: 524 -> 29; 8 chunks to 45 behind 900: 17.4 -> 12.6).  The merge costs about
+  // 5 us and the rows' partial sums: 500 tokens, 32/8 heads of 128, 16.3 unsplit, 22.8 in two.
+  int64_t want = 1;
+  if ((wgs <= 128 && max_ctx >= 768) || (wgs <= 256 && max_ctx >= 2048))
+    want = std::min<int64_t>(512 / std::max<int64_t>(wgs, 1), ceil_div64(max_ctx, 256));
+  const int64_t per = ceil_div64(stages, std::min(want, stages));
+  pl->tps = (int)(per * stage);
+  pl->nsplit = (int)ceil_div64(stages, per);
+  pl->ws_bytes = pl->nsplit > 1 ? (size_t)total_rows * Hq * pl->nsplit * (D + 4) * sizeof(float) : 0;
+  if (wgs * pl->nsplit > INT32_MAX || (int64_t)nseg * max_q_len * Hq > INT32_MAX)
+    return fail(MI355_EINVAL, "%s: too many workgroups (nseg=%d max_q_len=%d Hq=%d)", what, nseg, max_q_len, Hq);
+  return 0;
+}
+
 template <class Tag, int D>
-int launch(const Kv4PrefillParams& p0, int max_q_len, hipStream_t s) {
-  constexpr int MC = D == 256 ? 1 : 2;
-  Kv4PrefillParams p = p0;
-  p.row_tiles = (int)ceil_div64((int64_t)max_q_len * p.G, kWaves * MC * 16);
-  const int64_t wgs = (int64_t)p.row_tiles * p.nseg * p.Hkv;
-  if (wgs > INT32_MAX) return fail(MI355_EINVAL, "paged_prefill_kv4: too many workgroups");
-  hipLaunchKernelGGL((kv4_prefill_kernel<Tag, D, MC>), dim3((unsigned)wgs), dim3(256), 0, s, p);
-  return check_launch("kv4_prefill_kernel");
+int launch(const Kv4PrefillParams& p, const Kv4PrefillPlan& pl, int max_q_len, hipStream_t s) {
+  const dim3 grid((unsigned)((int64_t)p.row_tiles * p.nseg * p.Hkv * p.nsplit)), block(256);
+  if constexpr (D < 256 && !(Tag::kCode == MI355_F32 && D == 128)) {
+    if (pl.MC == 2) hipLaunchKernelGGL((kv4_prefill_kernel<Tag, D, 2>), grid, block, 0, s, p);
+  }
+  if (pl.MC == 1) hipLaunchKernelGGL((kv4_prefill_kernel<Tag, D, 1>), grid, block, 0, s, p);
+  if (int rc = check_launch("kv4_prefill_kernel")) return rc;
+  if (p.nsplit > 1) {
+    if (p.nsplit <= kKv4WalkedSplits) launch_merge<Tag, D, kv4_split_lanes<D>(true)>(p, max_q_len, s);
+    else launch_merge<Tag, D, kv4_split_lanes<D>(false)>(p, max_q_len, s);
+    return check_launch("kv4_prefill_merge_kernel");
+  }
+  return 0;
 }
 template <class Tag>
-int launch(const Kv4PrefillParams& p, int D, int max_q_len, hipStream_t s) {
+int launch(const Kv4PrefillParams& p, const Kv4PrefillPlan& pl, int D, int max_q_len, hipStream_t s) {
   switch (D) {
-    case 32: return launch<Tag, 32>(p, max_q_len, s);
-    case 64: return launch<Tag, 64>(p, max_q_len, s);
-    case 128: return launch<Tag, 128>(p, max_q_len, s);
-    default: return launch<Tag, 256>(p, max_q_len, s);
+    case 32: return launch<Tag, 32>(p, pl, max_q_len, s);
+    case 64: return launch<Tag, 64>(p, pl, max_q_len, s);
+    case 128: return launch<Tag, 128>(p, pl, max_q_len, s);
+    default: return launch<Tag, 256>(p, pl, max_q_len, s);
   }
 }
 
@@ -339,31 +439,34 @@ using namespace mi355;
 extern "C" size_t mi355_paged_prefill_kv4_workspace_bytes(int32_t nseg, int32_t total_rows, int32_t max_q_len,
                                                           int32_t Hq, int32_t Hkv, int32_t D, int32_t max_context,
                                                           int32_t dtype) {
-  return 0;
+  Kv4PrefillPlan pl;
+  if (nseg == 0 || max_q_len == 0) return 0;
+  if (make_plan("paged_prefill_kv4", nseg, total_rows, max_q_len, Hq, Hkv, D, max_context, dtype, &pl)) return 0;
+  return pl.ws_bytes;
 }
 
 extern "C" int mi355_paged_prefill_kv4(void* out, const void* q, int64_t q_stride_tok, const void* k_cache,
                                        const void* v_cache, const int32_t* block_tables, const int32_t* seg_q_start,
                                        const int32_t* seg_len, const int32_t* seg_pos0, int32_t nseg,
-                                       int32_t max_q_len, int32_t Hq, int32_t Hkv, int32_t D, int32_t block_size,
-                                       int32_t max_blocks, int32_t num_blocks, int32_t max_context,
-                                       int64_t stride_block, int64_t stride_head, float scale, int32_t dtype,
-                                       void* workspace, size_t workspace_bytes, void* stream) {
+                                       int32_t total_rows, int32_t max_q_len, int32_t Hq, int32_t Hkv, int32_t D,
+                                       int32_t block_size, int32_t max_blocks, int32_t num_blocks,
+                                       int32_t max_context, int64_t stride_block, int64_t stride_head, float scale,
+                                       int32_t dtype, void* workspace, size_t workspace_bytes, void* stream) {
   if (nseg == 0 || max_q_len == 0) return 0;
   if (!out || !q || !block_tables || !seg_q_start || !seg_len || !seg_pos0)
     return fail(MI355_EINVAL, "paged_prefill_kv4: null pointer argument");
   if (int rc = kv4_check_cache("paged_prefill_kv4", k_cache, v_cache, Hkv, D, block_size, num_blocks, stride_block, stride_head))
     return rc;
-  if (!kv4_dtype_ok(dtype)) return fail(MI355_EINVAL, "paged_prefill_kv4: dtype %d", dtype);
-  if (nseg < 0 || max_q_len < 0 || Hq <= 0 || Hq % Hkv || max_blocks <= 0 || max_context <= 0 ||
-      (max_context > kKv4MaxContext && (int64_t)max_blocks * block_size > kKv4MaxContext))
-    return fail(MI355_EINVAL, "paged_prefill_kv4: bad shape (nseg=%d max_q_len=%d Hq=%d Hkv=%d max_blocks=%d max_context=%d)",
-                nseg, max_q_len, Hq, Hkv, max_blocks, max_context);
+  if (max_blocks <= 0) return fail(MI355_EINVAL, "paged_prefill_kv4: max_blocks %d", max_blocks);
   if ((int64_t)max_context > (int64_t)max_blocks * block_size) max_context = max_blocks * block_size;
-  if ((int64_t)max_q_len * (Hq / Hkv) > INT32_MAX) return fail(MI355_EINVAL, "paged_prefill_kv4: max_q_len %d", max_q_len);
+  Kv4PrefillPlan pl;
+  if (int rc = make_plan("paged_prefill_kv4", nseg, total_rows, max_q_len, Hq, Hkv, D, max_context, dtype, &pl)) return rc;
   const int epl = dtype == MI355_F32 ? 4 : 8;
   if (q_stride_tok % epl || q_stride_tok < (int64_t)Hq * D || (((uintptr_t)q | (uintptr_t)out) & 15))
     return fail(MI355_EINVAL, "paged_prefill_kv4: query rows must be 16-byte aligned and a token's heads packed");
+  if (pl.ws_bytes && (!workspace || workspace_bytes < pl.ws_bytes || ((uintptr_t)workspace & 15)))
+    return fail(MI355_EWORKSPACE, "paged_prefill_kv4: workspace of %zu bytes needed (16-byte aligned), %zu given", pl.ws_bytes,
+                workspace ? workspace_bytes : (size_t)0);
   Kv4PrefillParams p;
   p.out = static_cast<char*>(out);
   p.q = static_cast<const char*>(q);
@@ -379,14 +482,17 @@ extern "C" int mi355_paged_prefill_kv4(void* out, const void* q, int64_t q_strid
   p.G = Hq / Hkv;
   p.max_blocks = max_blocks;
   p.max_ctx = max_context;
-  p.row_tiles = 0;
+  p.row_tiles = pl.row_tiles;
+  p.nsplit = pl.nsplit;
+  p.tps = pl.tps;
+  p.ws = static_cast<float*>(workspace);
   p.flip = scale < 0.f;
   p.scale2 = std::max(std::fabs(scale) * 1.44269504088896340736f, 1e-30f);   // (a scale of 0: all weights 1 to 30 digits)
   p.raise = kKv4Raise / p.scale2;
   hipStream_t s = static_cast<hipStream_t>(stream);
   switch (dtype) {
-    case MI355_F32: return launch<F32>(p, D, max_q_len, s);
-    case MI355_BF16: return launch<BF16>(p, D, max_q_len, s);
-    default: return launch<F16>(p, D, max_q_len, s);
+    case MI355_F32: return launch<F32>(p, pl, D, max_q_len, s);
+    case MI355_BF16: return launch<BF16>(p, pl, D, max_q_len, s);
+    default: return launch<F16>(p, pl, D, max_q_len, s);
   }
 }

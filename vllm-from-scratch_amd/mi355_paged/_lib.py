@@ -91,7 +91,7 @@ SIGNATURES = {
     'mi355_paged_decode_kv4_workspace_bytes': (c_size_t, [c_int32, c_int32, c_int32, c_int32, c_int32, c_int32]),
     'mi355_paged_prefill_kv4': (c_int, [
         c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32,
-        c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int64, c_int64, c_float, c_int32,
+        c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int64, c_int64, c_float, c_int32,
         c_void_p, c_size_t, c_void_p]),
     'mi355_paged_prefill_kv4_workspace_bytes': (c_size_t, [
         c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32]),

@@ -1014,7 +1014,7 @@ def paged_prefill_kv4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
         rc = lib.mi355_paged_prefill_kv4(
             out.data_ptr(), q.data_ptr(), _stride(q, 0), k_cache.data_ptr(), v_cache.data_ptr(),
             block_tables.data_ptr(), seg_q_start.data_ptr(), seg_len.data_ptr(), seg_pos0.data_ptr(), nseg,
-            int(max_q_len), Hq, Hkv, D, BS, width, NB, max_context, sb, sh, float(scale), code,
+            T, int(max_q_len), Hq, Hkv, D, BS, width, NB, max_context, sb, sh, float(scale), code,
             ws.data_ptr() if ws is not None else None, ws_bytes, stream)
     if rc:
         _lib.check(rc, 'mi355_paged_prefill_kv4')
