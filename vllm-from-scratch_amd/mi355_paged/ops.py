@@ -782,17 +782,30 @@ def kv4_cache_shape(num_blocks: int, kv_heads: int, block_size: int, head_dim: i
 
 def _kv4_geometry(k_cache: torch.Tensor, v_cache: torch.Tensor):
     """(num_blocks, kv_heads, block_size, head_dim, block stride, head stride) of a pair of cache tensors."""
-    shape = k_cache.shape
+    shape, strides = k_cache.shape, k_cache.stride()
     if k_cache.dtype != torch.uint8 or v_cache.dtype != torch.uint8:
         raise TypeError("4-bit caches are uint8 tensors")
     if len(shape) != 4 or shape != v_cache.shape or (shape[3] * 2) % 17 or shape[3] * 2 // 17 not in KV4_HEAD_DIMS:
         raise ValueError(f"4-bit caches must share the shape kv4_cache_shape gives, got {tuple(shape)} and "
                          f"{tuple(v_cache.shape)}")
-    sb, sh = _stride(k_cache, 0), _stride(k_cache, 1)
-    if k_cache.stride(3) != 1 or _stride(k_cache, 2) != shape[3] or v_cache.stride(3) != 1 or \
-            _stride(v_cache, 2) != shape[3] or _stride(v_cache, 0) != sb or _stride(v_cache, 1) != sh:
-        raise ValueError("4-bit caches must share strides, with the tiles of a head contiguous")
-    return shape[0], shape[1], shape[2] * KV4_TILE, shape[3] * 2 // 17, sb, sh
+    blocks, heads, tiles, record = shape
+    if strides != v_cache.stride() or strides[3] != 1 or strides[2] != record or blocks == 1 or heads == 1:
+        # (a dim of size 1 may carry any stride)
+        strides = tuple(_stride(k_cache, d) for d in range(4))
+        if strides != tuple(_stride(v_cache, d) for d in range(4)) or strides[3] != 1 or strides[2] != record:
+            raise ValueError("4-bit caches must share strides, with the tiles of a head contiguous")
+    return blocks, heads, tiles * KV4_TILE, record * 2 // 17, strides[0], strides[1]
+
+
+def _packed_rows(t: torch.Tensor) -> int:
+    """Token stride of [T, H, D] whose head rows are contiguous and packed D apart."""
+    if t.dim() != 3:
+        raise ValueError("expected [T, H, D]")
+    T, H, D = t.shape
+    st, sh, sd = t.stride()
+    if sd != 1 or (H != 1 and sh != D):
+        raise ValueError("expected [T, H, D] with heads packed D apart and contiguous head rows")
+    return st if T != 1 else H * D
 
 
 def rope_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional[dict] = None):
@@ -872,12 +885,12 @@ def rope_rotate(x: torch.Tensor, cos: Optional[torch.Tensor], sin: Optional[torc
     Pairs are (i, i + rotary_dim / 2), or neighbours (2 i, 2 i + 1) when `interleaved`."""
     dev = require_device(x, cos, sin, out)
     lib = _lib.load()
-    x = _head_rows(x)
+    stride = _packed_rows(x)
     T, H, D = x.shape
     R = _angle_rows(cos, sin, T)
-    out = _checked_out(out, (T, H, D), x.dtype, dev)
+    out = torch.empty((T, H, D), dtype=x.dtype, device=dev) if out is None else _checked_out(out, (T, H, D), x.dtype, dev)
     with _on(dev):
-        rc = lib.mi355_rope_rotate(out.data_ptr(), x.data_ptr(), _stride(x, 0), cos.data_ptr() if R else None,
+        rc = lib.mi355_rope_rotate(out.data_ptr(), x.data_ptr(), stride, cos.data_ptr() if R else None,
                                    sin.data_ptr() if R else None, R, int(interleaved), T, H, D, dtype_code(x),
                                    _stream(dev))
     if rc:
@@ -893,21 +906,22 @@ def rope_kv4_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: Optio
     are read only and may be views of one projection output; cos = sin = None: nothing is rotated."""
     dev = require_device(q, k, v, cos, sin, slots, k_cache, v_cache, out)
     lib = _lib.load()
-    q, k, v = _head_rows(q), _head_rows(k), _head_rows(v)
+    q_stride, k_stride, v_stride = _packed_rows(q), _packed_rows(k), _packed_rows(v)
     T, Hq, D = q.shape
     NB, Hkv, BS, cache_dim, sb, sh = _kv4_geometry(k_cache, v_cache)
-    if k.dtype != q.dtype or v.dtype != q.dtype:
+    dtype = q.dtype
+    if k.dtype != dtype or v.dtype != dtype:
         raise TypeError("q, k and v must share one dtype")
-    if k.shape != (T, Hkv, D) or v.shape != k.shape or cache_dim != D:
+    if k.shape != (T, Hkv, D) or v.shape != (T, Hkv, D) or cache_dim != D:
         raise ValueError("k and v must be [T, kv_heads, head_dim] matching q and the caches")
     if slots.dtype != torch.int64 or slots.numel() != T:
         raise TypeError("slots must be int64 [T]")
     slots = slots.contiguous()
     R = _angle_rows(cos, sin, T)
-    out = _checked_out(out, (T, Hq, D), q.dtype, dev)
+    out = torch.empty((T, Hq, D), dtype=dtype, device=dev) if out is None else _checked_out(out, (T, Hq, D), dtype, dev)
     with _on(dev):
         rc = lib.mi355_rope_kv4_write(
-            out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), _stride(q, 0), _stride(k, 0), _stride(v, 0),
+            out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), q_stride, k_stride, v_stride,
             cos.data_ptr() if R else None, sin.data_ptr() if R else None, R, int(interleaved), slots.data_ptr(),
             k_cache.data_ptr(), v_cache.data_ptr(), T, Hq, Hkv, D, BS, NB, sb, sh, dtype_code(q), _stream(dev))
     if rc:
@@ -945,8 +959,9 @@ def paged_decode_kv4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     q's dtype; a context of 0 gives zeros."""
     dev = require_device(q, k_cache, v_cache, block_tables, context_lens, out)
     lib = _lib.load()
-    if q.dim() != 3 or q.stride(2) != 1 or _stride(q, 1) != q.shape[2]:
+    if q.dim() != 3 or q.stride(2) != 1 or q.stride(1) != q.shape[2]:
         q = q.contiguous()
+    q_stride = _packed_rows(q)
     B, Hq, D = q.shape
     NB, Hkv, BS, cache_dim, sb, sh = _kv4_geometry(k_cache, v_cache)
     if cache_dim != D:
@@ -956,8 +971,8 @@ def paged_decode_kv4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     if block_tables.dim() != 2 or block_tables.shape[0] != B or context_lens.numel() != B:
         raise ValueError("block_tables must be [B, max_blocks] and context_lens [B]")
     block_tables, context_lens = block_tables.contiguous(), context_lens.contiguous()
-    out = _checked_out(out, (B, Hq, D), q.dtype, dev)
     code = dtype_code(q)
+    out = torch.empty((B, Hq, D), dtype=q.dtype, device=dev) if out is None else _checked_out(out, (B, Hq, D), q.dtype, dev)
     if scale is None:
         scale = 1.0 / math.sqrt(D)
     width = block_tables.shape[1]
@@ -967,7 +982,7 @@ def paged_decode_kv4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         need = lib.mi355_paged_decode_kv4_workspace_bytes(B, Hq, Hkv, D, max_context, code)
         ws, ws_bytes = _workspace(dev, need, stream)
         rc = lib.mi355_paged_decode_kv4(
-            out.data_ptr(), q.data_ptr(), _stride(q, 0), k_cache.data_ptr(), v_cache.data_ptr(),
+            out.data_ptr(), q.data_ptr(), q_stride, k_cache.data_ptr(), v_cache.data_ptr(),
             block_tables.data_ptr(), context_lens.data_ptr(), B, Hq, Hkv, D, BS, width, NB, max_context, sb, sh,
             float(scale), code, ws.data_ptr() if ws is not None else None, ws_bytes, stream)
     if rc:
@@ -985,7 +1000,7 @@ def paged_prefill_kv4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     max_context their host-side bounds.  Rows of `out` outside every segment are left untouched."""
     dev = require_device(q, k_cache, v_cache, block_tables, seg_q_start, seg_len, seg_pos0, out)
     lib = _lib.load()
-    q = _head_rows(q)
+    q_stride = _packed_rows(q)
     T, Hq, D = q.shape
     NB, Hkv, BS, cache_dim, sb, sh = _kv4_geometry(k_cache, v_cache)
     if cache_dim != D:
@@ -999,10 +1014,10 @@ def paged_prefill_kv4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
         raise ValueError("block_tables must be [nseg, max_blocks]; the segment vectors [nseg]")
     block_tables = block_tables.contiguous()
     seg_q_start, seg_len, seg_pos0 = seg_q_start.contiguous(), seg_len.contiguous(), seg_pos0.contiguous()
-    out = _checked_out(out, (T, Hq, D), q.dtype, dev)
+    code = dtype_code(q)
+    out = torch.empty((T, Hq, D), dtype=q.dtype, device=dev) if out is None else _checked_out(out, (T, Hq, D), q.dtype, dev)
     if T == 0:
         return out
-    code = dtype_code(q)
     if scale is None:
         scale = 1.0 / math.sqrt(D)
     width = block_tables.shape[1]
@@ -1012,7 +1027,7 @@ def paged_prefill_kv4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
         need = lib.mi355_paged_prefill_kv4_workspace_bytes(nseg, T, int(max_q_len), Hq, Hkv, D, max_context, code)
         ws, ws_bytes = _workspace(dev, need, stream)
         rc = lib.mi355_paged_prefill_kv4(
-            out.data_ptr(), q.data_ptr(), _stride(q, 0), k_cache.data_ptr(), v_cache.data_ptr(),
+            out.data_ptr(), q.data_ptr(), q_stride, k_cache.data_ptr(), v_cache.data_ptr(),
             block_tables.data_ptr(), seg_q_start.data_ptr(), seg_len.data_ptr(), seg_pos0.data_ptr(), nseg,
             T, int(max_q_len), Hq, Hkv, D, BS, width, NB, max_context, sb, sh, float(scale), code,
             ws.data_ptr() if ws is not None else None, ws_bytes, stream)
