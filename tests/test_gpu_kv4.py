@@ -529,3 +529,90 @@ def test_captured_and_replayed(ops, device, decode):
         other = _step(ops, fresh[0])
     side.synchronize()
     assert torch.equal(other, _step(ops, fresh[0]))
+
+
+# ------------------------------------------------------------------ the engine over a 4-bit cache
+@pytest.mark.parametrize('rotary', [None, dict(dim=32, interleaved=True, scaling={'kind': 'yarn', 'factor': 4, 'original': 64})])
+def test_engine_layer_steps(ops, device, rotary):
+    """Two steps of an attention layer (prompts, then a decode token beside a later chunk) against float64 on the
+    layer's own projections: which rows are rotated how, where they are cached and who attends to what."""
+    import mini_vllm as mv
+    torch.manual_seed(3)
+    H, D, BS = 4, 64, 16
+    pos_cfg = mv.RotaryPositions(D, **(rotary or {}))
+    layer = mv.SelfAttention(H * D, H, D, pos_cfg).to(device)
+    kc, vc = (torch.full(ops.kv4_cache_shape(8, H, BS, D), 255, dtype=torch.uint8, device=device) for _ in range(2))
+    okc, ovc = kc.cpu().numpy(), vc.cpu().numpy()
+    tables = [[5, 2, 0], [1, 7, 3]]
+    steps = [([0, 0], [20, 17], [True, True]), ([20, 17], [1, 14], [False, True])]       # starts, lengths, prefill?
+    for starts, lens, prefill in steps:
+        pos = np.concatenate([np.arange(s, s + n) for s, n in zip(starts, lens)])
+        slots = np.concatenate([[t[p // BS] * BS + p % BS for p in range(s, s + n)] for t, s, n in zip(tables, starts, lens)])
+        plan = mv.build_attn_plan(pos.tolist(), lens, prefill, tables, device, append_ok=True, from_cache=True)
+        x = torch.randn(len(pos), H * D, device=device)
+        with torch.no_grad():
+            got = layer(x, torch.from_numpy(pos).cuda(), (kc, vc), torch.from_numpy(slots).cuda(), lens, prefill, plan)
+            qkv = layer.qkv(x).double().cpu().numpy()
+        q, k, v = (t.reshape(len(pos), H, D) for t in np.split(qkv, 3, -1))
+        cos, sin = (t.double().cpu().numpy() for t in pos_cfg.angles(torch.from_numpy(pos).cuda()))
+        for form, (cache, rows) in enumerate(((okc, orc.rotate(k, cos, sin, pos_cfg.interleaved)), (ovc, v))):
+            code, byte = orc.quantise(rows)
+            for t, slot in enumerate(slots):
+                for h in range(H):
+                    orc.write_row(cache[slot // BS, h, slot % BS // 16], slot % 16, code[t, h], byte[t, h], bool(form))
+        np.testing.assert_array_equal(kc.cpu().numpy(), okc)
+        np.testing.assert_array_equal(vc.cpu().numpy(), ovc)
+        rot = orc.rotate(q, cos, sin, pos_cfg.interleaved)
+        total = [s + n for s, n in zip(starts, lens)]
+        want, size, big = _attend_all(np.split(rot, [lens[0]]), okc, ovc, np.array(tables), total, D ** -0.5,
+                                      [list(range(s, s + n)) for s, n in zip(starts, lens)])
+        # per attention output: the kernel's bound and one rounding of the rotated query; then a product of H D terms
+        bound = _attention_bound(size, big, want, D, max(total), torch.float32) + 8 * U * big * size
+        w = layer.out_proj.weight.detach().double().cpu().numpy()
+        a = want.reshape(len(pos), -1)
+        _near(got, a @ w.T, bound.reshape(len(pos), -1) @ np.abs(w).T + (H * D + 2) * U * (np.abs(a) @ np.abs(w).T))
+
+
+def _generate(mv, graphs, dtype, **kw):
+    torch.manual_seed(7)
+    eng = mv.MiniVLLM(vocab_size=300, hidden_size=128, num_layers=2, num_heads=4, intermediate_size=256, num_kv_blocks=64,
+                      block_size=16, max_num_seqs=8, max_num_batched_tokens=64, device='cuda', dtype=dtype,
+                      decode_graphs=graphs, **kw)
+    rng = np.random.default_rng(1)
+    for n in (5, 90, 33, 1, 130):
+        eng.add_request(rng.integers(1, 300, n).tolist(), max_new_tokens=12, temperature=0.0)
+    out = {}
+    while eng.scheduler.has_unfinished:
+        for rid, tok in eng.step():
+            out.setdefault(rid, []).append(tok)
+    return out, eng
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('kw', [dict(kv_cache_dtype='mxfp4'), dict(kv_cache_dtype='mxfp4', rotary=dict(dim=16, interleaved=True)),
+                                dict(rotary=dict(scaling={'kind': 'linear', 'factor': 2.0}))], ids=str)
+def test_engine_generates_the_same_with_and_without_graphs(device, dtype, kw):
+    """Chunked prompts, mixed and pure decode steps: replayed steps give what eager ones give, to the token."""
+    import mini_vllm as mv
+    a, eng = _generate(mv, True, dtype, **kw)
+    b, _ = _generate(mv, False, dtype, **kw)
+    assert a == b and all(len(v) == 12 or v[-1] == 0 for v in a.values()) and len(a) == 5
+    assert eng._launches > 0 and torch.isfinite(eng.last_logits.float()).all()
+    if 'kv_cache_dtype' in kw:
+        assert eng.model.k_cache.dtype == torch.uint8
+
+
+def test_engine_rotary_settings_equal_the_table_where_they_mean_the_same(device):
+    """rotary={} is the reference's rotation, with angles formed in double instead of taken from a float table: at
+    positions below 150 an angle differs by at most 150 * 2^-24 = 9e-6, a score by a few times that, and two layers
+    of this model turn it into logits within 1e-3 of each other."""
+    import mini_vllm as mv
+    logits = []
+    for kw in ({}, dict(rotary={})):
+        torch.manual_seed(7)
+        model = mv.MiniTransformer(300, 128, 2, 4, 256, 16, 16, **kw).to(device)
+        n = 140
+        pos = torch.arange(n, device=device)
+        with torch.no_grad():
+            logits.append(model(torch.arange(1, n + 1, device=device), pos, pos, [n], [True], block_tables=[list(range(9))]))
+    torch.testing.assert_close(logits[0], logits[1], atol=1e-3, rtol=1e-3)

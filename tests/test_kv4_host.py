@@ -167,3 +167,42 @@ def test_ops_refuse_host_tensors():
         ops.kv4_read_slots(k, k, torch.zeros(1, dtype=torch.int64))
     with pytest.raises(RuntimeError, match='HIP device'):
         ops.rope_angles(torch.zeros(1, dtype=torch.int64), torch.zeros(4, dtype=torch.float64))
+
+
+# ------------------------------------------------------------------ the engine's arguments
+@pytest.mark.parametrize('kw', [dict(kv_cache_dtype='mxfp4'), dict(rotary={}), dict(kv_cache_dtype='mxfp4', device='cuda', reference_compat=True),
+                                dict(kv_cache_dtype='fp4', device='cuda')])
+def test_engine_refuses_settings_it_does_not_serve(kw):
+    import mini_vllm
+    with pytest.raises(ValueError):
+        mini_vllm.MiniVLLM(**kw)
+
+
+@pytest.mark.parametrize('kw,match', [(dict(num_heads=8), 'head_dim'), (dict(block_size=8), 'tiles of 16'), (dict(rotary=dict(dim=24)), 'multiple of 16'),
+                                      (dict(rotary=dict(dim=64)), 'head_dim'), (dict(rotary=dict(scaling={'kind': 'x'})), 'scaling kind'),
+                                      (dict(kv_cache_dtype='int4'), 'mxfp4')])
+def test_model_refuses_what_the_cache_does_not_hold(kw, match):
+    import mini_vllm
+    args = dict(vocab_size=50, hidden_size=128, num_layers=1, num_heads=4, intermediate_size=64, num_kv_blocks=4, block_size=16,
+                kv_cache_dtype='mxfp4')
+    with pytest.raises(ValueError, match=match):
+        mini_vllm.MiniTransformer(**dict(args, **kw))
+
+
+def test_model_holds_the_caches_it_announces():
+    import mini_vllm
+    m = mini_vllm.MiniTransformer(50, 128, 2, 4, 64, 6, 32, kv_cache_dtype='mxfp4')
+    assert m.k_cache.shape == m.v_cache.shape == (2, 6, 4, 2, 17 * 32 // 2) and m.k_cache.dtype == torch.uint8
+    assert m.to(torch.bfloat16).k_cache.dtype == torch.uint8
+    plain = mini_vllm.MiniTransformer(50, 128, 2, 4, 64, 6, 32)
+    assert plain.k_cache.shape == (2, 6, 32, 4, 32) and plain.k_cache.dtype == torch.float32
+
+
+def test_plan_keeps_prompts_on_the_cache():
+    import mini_vllm
+    args = dict(positions=list(range(5)) + [7] + [0], seq_lens=[5, 1, 1], is_prefill=[True, False, True],
+                block_tables=[[0], [1], [2]], device='cpu', append_ok=True)
+    plan = mini_vllm.build_attn_plan(**args, from_cache=True)
+    assert plan.causal_tokens == 0 and plan.append_tokens == 5 and plan.append_meta.tolist() == [[0], [5], [0]]
+    assert plan.paged_rows == 2 and plan.paged_context.tolist() == [8, 1] and not plan.pure_decode
+    assert mini_vllm.build_attn_plan(**args).causal_tokens == 6

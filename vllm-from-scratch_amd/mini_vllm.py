@@ -581,6 +581,8 @@ class AttnPlan:
     # paged_context[r] = its position + 1 cached rows): RoPE, cache write and attention of a layer
     # can then be ONE launch (ops.paged_decode_append with rope tables)
     pure_decode: bool = False
+    # cos / sin rows of the step's positions (RotaryPositions), made by the first layer that asks and shared by the rest
+    angles: Optional[tuple] = None
 
 
 def build_attn_plan(positions: Sequence[int], seq_lens: Sequence[int], is_prefill: Sequence[bool],
@@ -588,13 +590,15 @@ def build_attn_plan(positions: Sequence[int], seq_lens: Sequence[int], is_prefil
                     reference_compat: bool = False,
                     device_tables: Optional[DeviceBlockTables] = None,
                     table_rows: Optional[Sequence[int]] = None,
-                    append_ok=False) -> AttnPlan:
+                    append_ok=False, from_cache: bool = False) -> AttnPlan:
     """block_tables: per-request lists of block ids (host), or None for the reference's
     semantics.  When device_tables / table_rows are given (one row id per request) the paged
     rows' tables are gathered on the device instead of being rebuilt from the host lists.
     append_ok: the paged-prefill kernel covers this model, so prompt chunks that do not start
     at position 0 become append segments instead of one paged-decode row per token; a callable
-    (n_q, context) -> bool decides per segment (contexts beyond what that kernel stages)."""
+    (n_q, context) -> bool decides per segment (contexts beyond what that kernel stages).
+    from_cache: prompts attend to their cached rows even where they start at position 0 (a 4-bit
+    cache: every token then sees the same rounded rows, however the prompt was cut)."""
     causal_tok: List[int] = []
     cu = [0]
     max_len = 0
@@ -613,7 +617,7 @@ def build_attn_plan(positions: Sequence[int], seq_lens: Sequence[int], is_prefil
         n_q = n if prefill else 1
         pure_decode = pure_decode and not prefill
         start = int(positions[tok]) if n > 0 else 0
-        if prefill and (compat or start == 0):
+        if prefill and (compat or (start == 0 and not from_cache)):
             causal_tok.extend(range(tok, tok + n_q))
             cu.append(cu[-1] + n_q)
             max_len = max(max_len, n_q)
@@ -742,6 +746,31 @@ def paged_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_ca
     return out.to(home)
 
 
+def kv4_attention_step(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, plan: AttnPlan,
+                       scale: float) -> torch.Tensor:
+    """Attention of one layer of one step over a 4-bit cache that holds the step's rows already.
+    q [T, H, D] (rotated); returns [T, H, D]."""
+    sel = plan.paged_index
+    if plan.causal_tokens:
+        raise RuntimeError("mini_vllm: a step over a 4-bit cache needs a plan built with from_cache=True")
+    out = None
+    if plan.paged_rows:
+        rows = q if sel is None else q[sel]
+        if sel is not None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        part = ops.paged_decode_kv4(rows, k_cache, v_cache, plan.paged_tables, plan.paged_context, plan.max_context,
+                                    scale=scale, out=out[sel] if isinstance(sel, slice) else None)
+        if sel is None:
+            out = part
+        elif not isinstance(sel, slice):
+            out[sel] = part
+    if plan.append_tokens:
+        meta = plan.append_meta
+        out = ops.paged_prefill_kv4(q, k_cache, v_cache, plan.append_tables, meta[0], meta[1], meta[2],
+                                    plan.max_append_len, plan.max_append_context, scale=scale, out=out)
+    return out
+
+
 # ---------------------------------------------------------------------------
 # model
 # ---------------------------------------------------------------------------
@@ -807,15 +836,38 @@ class RotaryEmbedding(nn.Module):
         return self.cos_cached[positions], self.sin_cached[positions]
 
 
+class RotaryPositions:
+    """How a model turns positions into rotations where the table of RotaryEmbedding does not do: which dims
+    rotate (the first `dim` of a head), in which pairs (`interleaved`: neighbours, else halves), and a
+    long-context `scaling` of the frequencies (ops.rope_frequencies).  Angles are formed in double for the
+    positions at hand, so there is no last position."""
+
+    def __init__(self, head_dim: int, dim: Optional[int] = None, base: float = 10000.0, interleaved: bool = False,
+                 scaling: Optional[dict] = None):
+        self.dim = head_dim if dim is None else dim
+        if self.dim <= 0 or self.dim > head_dim or self.dim % 16:
+            raise ValueError(f"rotary dim {self.dim} must be a multiple of 16 up to head_dim {head_dim}")
+        if head_dim not in ops.KV4_HEAD_DIMS:
+            raise ValueError(f"rotary settings and 4-bit caches serve head_dim {ops.KV4_HEAD_DIMS}, not {head_dim}")
+        self.interleaved = interleaved
+        self.inv_freq, self.factor = ops.rope_frequencies(self.dim, base, scaling)
+
+    def angles(self, positions: torch.Tensor):
+        if self.inv_freq.device != positions.device:
+            self.inv_freq = self.inv_freq.to(positions.device)
+        return ops.rope_angles(positions, self.inv_freq, self.factor)
+
+
 class SelfAttention(nn.Module):
     """Multi-head attention over a paged KV cache (05_mini_vllm/mini_vllm.py:377-487).
     The projections and RoPE are torch ops; the KV write and both attention branches
     are kernel launches driven by an AttnPlan."""
 
-    def __init__(self, hidden_size: int, num_heads: int, head_dim: int):
+    def __init__(self, hidden_size: int, num_heads: int, head_dim: int, rotary: Optional[RotaryPositions] = None):
         super().__init__()
         self.num_heads = num_heads
         self.head_dim = head_dim
+        self.rotary = rotary             # None: the table in self.rope
         self.scale = head_dim ** -0.5
         self.qkv = nn.Linear(hidden_size, 3 * num_heads * head_dim, bias=False)
         self.out_proj = nn.Linear(num_heads * head_dim, hidden_size, bias=False)
@@ -829,6 +881,18 @@ class SelfAttention(nn.Module):
         qkv = self.qkv(x)
         q, k, v = (t.view(T, H, D) for t in qkv.chunk(3, dim=-1))
         k_cache, v_cache = kv_cache
+        if self.rotary is not None:
+            if plan.angles is None:
+                plan.angles = self.rotary.angles(positions)
+            cos, sin = plan.angles
+            if k_cache.dtype == torch.uint8:
+                q = ops.rope_kv4_write(q, k, v, cos, sin, slot_mapping, k_cache, v_cache, self.rotary.interleaved)
+                attn = kv4_attention_step(q, k_cache, v_cache, plan, self.scale)
+            else:
+                q = ops.rope_rotate(q, cos, sin, self.rotary.interleaved)
+                k = ops.rope_rotate(k, cos, sin, self.rotary.interleaved)
+                attn = paged_attention_step(q, k, v, k_cache, v_cache, slot_mapping, plan, self.scale)
+            return self.out_proj(attn.reshape(plan.total_tokens, H * D).to(x.dtype))
         cos_t, sin_t = self.rope.cos_cached, self.rope.sin_cached
         per32 = 32 // x.element_size()      # the fused kernel moves two 16-byte pieces per half row
         fusable = (_kernel_rows(qkv, cos_t, sin_t) and k_cache.is_cuda and k_cache.dtype == x.dtype and D % per32 == 0
@@ -890,9 +954,10 @@ class FFN(nn.Module):
 
 
 class TransformerLayer(nn.Module):
-    def __init__(self, hidden_size: int, num_heads: int, intermediate_size: int):
+    def __init__(self, hidden_size: int, num_heads: int, intermediate_size: int,
+                 rotary: Optional[RotaryPositions] = None):
         super().__init__()
-        self.attn = SelfAttention(hidden_size, num_heads, hidden_size // num_heads)
+        self.attn = SelfAttention(hidden_size, num_heads, hidden_size // num_heads, rotary)
         self.ffn = FFN(hidden_size, intermediate_size)
         self.norm1 = RMSNorm(hidden_size)
         self.norm2 = RMSNorm(hidden_size)
@@ -918,23 +983,34 @@ class TransformerLayer(nn.Module):
 class MiniTransformer(nn.Module):
     """Small pre-norm transformer that owns its paged KV buffers
     k_cache / v_cache [layers, blocks, block_size, heads, head_dim]
-    (05_mini_vllm/mini_vllm.py:517-585)."""
+    (05_mini_vllm/mini_vllm.py:517-585).  kv_cache_dtype 'mxfp4': the buffers are 4-bit caches, uint8
+    [layers, blocks, heads, block_size / 16, 17 * head_dim / 2] (ops.kv4_cache_shape); rotary: the
+    arguments of RotaryPositions, None for the reference's table."""
 
     def __init__(self, vocab_size: int, hidden_size: int, num_layers: int, num_heads: int,
-                 intermediate_size: int, num_kv_blocks: int, block_size: int):
+                 intermediate_size: int, num_kv_blocks: int, block_size: int,
+                 kv_cache_dtype: Optional[str] = None, rotary: Optional[dict] = None):
         super().__init__()
+        if kv_cache_dtype not in (None, 'mxfp4'):
+            raise ValueError(f"kv_cache_dtype {kv_cache_dtype!r}: None (the model's dtype) or 'mxfp4'")
         self.hidden_size = hidden_size
         self.num_layers = num_layers
         self.block_size = block_size
         head_dim = hidden_size // num_heads
+        self.head_dim = head_dim
+        self.kv4 = kv_cache_dtype == 'mxfp4'
+        positions = RotaryPositions(head_dim, **(rotary or {})) if self.kv4 or rotary is not None else None
         self.embedding = nn.Embedding(vocab_size, hidden_size)
         self.layers = nn.ModuleList(
-            TransformerLayer(hidden_size, num_heads, intermediate_size) for _ in range(num_layers))
+            TransformerLayer(hidden_size, num_heads, intermediate_size, positions) for _ in range(num_layers))
         self.norm = RMSNorm(hidden_size)
         self.lm_head = nn.Linear(hidden_size, vocab_size, bias=False)
-        cache_shape = (num_layers, num_kv_blocks, block_size, num_heads, head_dim)
-        self.register_buffer('k_cache', torch.zeros(cache_shape))
-        self.register_buffer('v_cache', torch.zeros(cache_shape))
+        cache_shape, cache_dtype = (num_layers, num_kv_blocks, block_size, num_heads, head_dim), None
+        if self.kv4:
+            cache_shape = (num_layers,) + ops.kv4_cache_shape(num_kv_blocks, num_heads, block_size, head_dim)
+            cache_dtype = torch.uint8
+        self.register_buffer('k_cache', torch.zeros(cache_shape, dtype=cache_dtype))
+        self.register_buffer('v_cache', torch.zeros(cache_shape, dtype=cache_dtype))
 
     def forward(self, token_ids: torch.Tensor, positions: torch.Tensor, slot_mapping: torch.Tensor,
                 seq_lens: List[int], is_prefill: List[bool],
@@ -953,14 +1029,14 @@ class MiniTransformer(nn.Module):
         token_ids, positions, slot_mapping = (t.to(home) for t in (token_ids, positions, slot_mapping))
         if positions_host is None:
             positions_host = positions.tolist()
-        head_dim = self.k_cache.shape[-1]
-        append_ok = self.k_cache.is_cuda and ops.paged_prefill_supported(self.k_cache.dtype, head_dim)
-        if append_ok:
+        head_dim = self.head_dim
+        append_ok = self.kv4 or (self.k_cache.is_cuda and ops.paged_prefill_supported(self.k_cache.dtype, head_dim))
+        if append_ok and not self.kv4:
             dtype, bs = self.k_cache.dtype, self.block_size
             append_ok = lambda n_q, context: ops.paged_prefill_serves(dtype, head_dim, bs, n_q, context)
         plan = build_attn_plan(positions_host, seq_lens, is_prefill, block_tables,
                                _compute_device(self.k_cache), reference_compat, device_tables, table_rows,
-                               append_ok=append_ok)
+                               append_ok=append_ok, from_cache=self.kv4)
         last, offset = [], 0
         for n in seq_lens:
             offset += n
@@ -1238,12 +1314,20 @@ class MiniVLLM:
                  enable_chunked_prefill: bool = True, device: str = 'cpu',
                  reference_compat: bool = False, dtype: Optional[torch.dtype] = None,
                  decode_graphs: bool = True, enable_prefix_caching: bool = False,
-                 decode_lookahead: bool = True, pipeline_steps: bool = True, fused_decode_step: bool = True):
+                 decode_lookahead: bool = True, pipeline_steps: bool = True, fused_decode_step: bool = True,
+                 kv_cache_dtype: Optional[str] = None, rotary: Optional[dict] = None):
         """The first eleven arguments are the reference's (05_mini_vllm/mini_vllm.py:649-662); the
         rest select this implementation's execution modes, every one of which gives every request
         the same tokens.  fused_decode_step: in a step of decode tokens only, RoPE, the cache write
-        and attention of a layer are one launch (False: RoPE + cache write, then attention)."""
+        and attention of a layer are one launch (False: RoPE + cache write, then attention).
+        Two further arguments change the model itself, on a HIP device only: kv_cache_dtype 'mxfp4' keeps
+        keys and values in 4 bits (17/64 of a 16-bit cache's bytes; head_dim 32 / 64 / 128 / 256, block_size
+        a multiple of 16), and rotary gives the positions' rotation other settings than the reference's table
+        (RotaryPositions: dim, base, interleaved, scaling)."""
         self.device = torch.device(device)
+        if (kv_cache_dtype is not None or rotary is not None) and (self.device.type != 'cuda' or reference_compat):
+            raise ValueError("kv_cache_dtype and rotary need device='cuda' and true-context attention "
+                             "(not reference_compat)")
         self.reference_compat = reference_compat
         # replay pure-decode steps as HIP graphs (device-resident engines only)
         self.decode_graphs = decode_graphs and self.device.type == 'cuda' and not reference_compat
@@ -1273,7 +1357,8 @@ class MiniVLLM:
         self.model = MiniTransformer(vocab_size=vocab_size, hidden_size=hidden_size,
                                      num_layers=num_layers, num_heads=num_heads,
                                      intermediate_size=intermediate_size,
-                                     num_kv_blocks=num_kv_blocks, block_size=block_size).to(self.device)
+                                     num_kv_blocks=num_kv_blocks, block_size=block_size,
+                                     kv_cache_dtype=kv_cache_dtype, rotary=rotary).to(self.device)
         if dtype is not None:
             self.model = self.model.to(dtype)
         for layer in self.model.layers:
@@ -1331,8 +1416,9 @@ class MiniVLLM:
         max_q = max((len(scheduled[i].tokens) for i in chunks), default=1)
         max_ctx = max(item.start + len(item.tokens) for item in scheduled)
         cache = self.model.k_cache
-        if not ops.paged_prefill_serves(cache.dtype, cache.shape[-1], self.model.block_size,
-                                        _bucket_pow(max(max_q, 1), 4, 16), _bucket_pow(max_ctx, 2, 256)):
+        if not self.model.kv4 and not ops.paged_prefill_serves(
+                cache.dtype, cache.shape[-1], self.model.block_size,
+                _bucket_pow(max(max_q, 1), 4, 16), _bucket_pow(max_ctx, 2, 256)):
             return None
         step = self._mixed_step(total, len(scheduled), max_q, max_ctx)
         T, S = step.T, step.S
@@ -1557,8 +1643,9 @@ class MiniVLLM:
         if ok is None:
             cache = self.model.k_cache
             ok = self._mixed_ok = (cache.is_cuda and self.model.embedding.weight.is_cuda
-                                   and ops.paged_prefill_supported(cache.dtype, cache.shape[-1])
-                                   and cache.dtype == self.model.embedding.weight.dtype)
+                                   and (self.model.kv4
+                                        or (ops.paged_prefill_supported(cache.dtype, cache.shape[-1])
+                                            and cache.dtype == self.model.embedding.weight.dtype)))
         return ok
 
     def step(self):
