@@ -524,7 +524,7 @@ size_t mi355_paged_decode_kv4_workspace_bytes(int32_t B, int32_t Hq, int32_t Hkv
  * 0 .. seg_pos0[s] + j, whose rows (the segment's own among them) are in the cache.  Rows of out
  * outside every segment are left as they are; a segment may be empty.  A value row that a query must
  * not see never reaches it, NaN or not.  Precision as in mi355_paged_decode_kv4.  total_rows: the tokens
- * q and out hold; every segment lies within them.
+ * q and out hold; what a segment has behind them (or behind its first max_q_len) is left out.
  */
 int mi355_paged_prefill_kv4(void* out, const void* q, int64_t q_stride_tok, const void* k_cache,
                             const void* v_cache, const int32_t* block_tables, const int32_t* seg_q_start,

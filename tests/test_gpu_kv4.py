@@ -419,6 +419,55 @@ def test_chunk_long_context_few_rows(ops, device, dtype):
         _near(out, want, _attention_bound(size, big, want, D, 7005, dtype))
 
 
+WIDE = [
+    # Hq, Hkv, D, BS, chunk lengths, first positions: enough rows for each way the kernel cuts them up
+    (8, 8, 64, 16, [2048] * 8, [0] * 8),
+    (8, 8, 64, 16, [300, 7, 400, 0, 220, 399, 350, 1], [0, 600, 0, 0, 90, 0, 17, 0]),
+    (8, 8, 64, 16, [512, 500, 512, 512, 480, 512], [1300, 0, 1290, 1300, 1000, 1777]),
+    (32, 8, 128, 16, [300, 290, 300, 300], [0, 0, 11, 0]),
+    (32, 8, 128, 16, [256, 250, 256], [1600, 1607, 0]),
+    (8, 8, 128, 16, [512, 100, 512, 512, 512], [0, 0, 0, 0, 0]),
+    (4, 2, 256, 16, [200, 100], [700, 0]),
+    (8, 8, 32, 16, [512, 510, 512, 512, 333, 512], [1300, 0, 1290, 1300, 1000, 1777]),
+]
+
+
+@pytest.mark.parametrize('dtype', ALL)
+@pytest.mark.parametrize('Hq,Hkv,D,BS,lens,pos0', WIDE, ids=lambda v: str(v))
+def test_many_rows(ops, device, dtype, Hq, Hkv, D, BS, lens, pos0):
+    """Up to 40 queries of each chunk at random, the first and the last among them."""
+    rng = np.random.default_rng(Hq + D + sum(lens))
+    total = [n + p for n, p in zip(lens, pos0)]
+    kc, vc, tables = _cache(rng, total, Hkv, D, BS)
+    start = [int(x) for x in np.cumsum([0] + lens)[:-1]]
+    q, qv = _cast(rng.standard_normal((sum(lens), Hq, D)) * 1.5, dtype)
+    meta = torch.tensor([start, lens, pos0], dtype=torch.int32, device=device)
+    out = ops.paged_prefill_kv4(q, *(torch.from_numpy(a).cuda() for a in (kc, vc, tables)), meta[0], meta[1], meta[2],
+                                max(lens), max(total))
+    pick = [sorted({j for j in (0, n - 1) if n} | set(rng.integers(0, n, n // 4 and min(n // 4, 40)).tolist())) for n in lens]
+    want, size, big = _attend_all([qv[[s + j for j in p]] for s, p in zip(start, pick)], kc, vc, tables, total, D ** -0.5,
+                                  [[p0 + j for j in p] for p0, p in zip(pos0, pick)])
+    rows = torch.tensor([s + j for s, p in zip(start, pick) for j in p]).cuda()
+    _near(out[rows], want, _attention_bound(size, big, want, D, max(total), dtype))
+
+
+@pytest.mark.parametrize('ctx', [40, 3000])
+def test_chunk_rows_outside_the_tensors_are_left_out(ops, device, ctx):
+    rng = np.random.default_rng(2)
+    Hq, Hkv, D, BS, rows = 4, 2, 64, 16, 20
+    kc, vc, tables = _cache(rng, [ctx] * 4, Hkv, D, BS)
+    big, qv = _cast(rng.standard_normal((rows + 12, Hq, D)), torch.bfloat16)
+    out = torch.full((rows + 12, Hq, D), 7.0, dtype=torch.bfloat16, device=device)
+    start, lens, pos0 = [0, 14, 25, -3], [4, 9, 5, 2], [ctx - 4, ctx - 9, 0, 0]
+    meta = torch.tensor([start, lens, pos0], dtype=torch.int32, device=device)
+    ops.paged_prefill_kv4(big[:rows], *(torch.from_numpy(a).cuda() for a in (kc, vc, tables)), meta[0], meta[1], meta[2], 9, ctx,
+                          out=out[:rows])
+    assert bool((out[4:14] == 7.0).all()) and bool((out[rows:] == 7.0).all())
+    want, size, most = _attend_all([qv[:4], qv[14:20]], kc, vc, tables, [ctx] * 2, D ** -0.5,
+                                   [[ctx - 4 + j for j in range(4)], [ctx - 9 + j for j in range(6)]])
+    _near(out[[0, 1, 2, 3, 14, 15, 16, 17, 18, 19]], want, _attention_bound(size, most, want, D, ctx, torch.bfloat16))
+
+
 def test_chunk_nan_reaches_only_the_queries_that_see_it(ops, device):
     """A NaN key or value at a position of the chunk itself: the queries before it stay finite, whatever
     else shares their tiles."""

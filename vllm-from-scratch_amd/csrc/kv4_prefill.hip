@@ -9,6 +9,9 @@
 // bf16: 130 vector instructions per 32 tokens of 128 dims, as many as two tiles' softmax, so it is done
 // once per workgroup and not once per wave.  Codes travel from memory one stage ahead in registers,
 // operands one stage ahead in LDS (two buffers, one barrier per stage).
+// A stage is a chain -- scores, softmax, values, barrier -- that eight waves of a CU overlap and four do not.
+// Where there are few workgroups each gets a second team of four waves for the same rows; the teams take
+// the stages in turn and are joined through LDS.
 #include <algorithm>
 #include <cmath>
 
@@ -44,10 +47,15 @@ struct Kv4PrefillParams {
   const int32_t* seg_pos0;
   int64_t q_stride;   // elements
   float* ws;   // [total rows * Hq][nsplit][D + 4]: unnormalised sums, running maximum, sum of weights
-  int nseg, Hq, Hkv, G, max_blocks, max_ctx, row_tiles, nsplit, tps /* tokens per split, whole stages */;
+  int nseg, total_rows, Hq, Hkv, G, max_blocks, max_ctx, row_tiles, nsplit, tps /* tokens per split, whole stages */;
   float scale2, raise;   // |scale| * log2(e); kKv4Raise in units of a raw score
   int flip;              // a negative scale: the queries are negated
 };
+
+// Rows of a segment; none outside the tensors, whatever the segment says.
+__device__ __forceinline__ int segment_rows(const Kv4PrefillParams& p, int q0, int len) {
+  return q0 < 0 || q0 >= p.total_rows ? 0 : min(len, p.total_rows - q0);
+}
 
 // Between two waves' uses of LDS; global loads may stay in flight across it.
 __device__ __forceinline__ void lds_barrier() {
@@ -56,14 +64,21 @@ __device__ __forceinline__ void lds_barrier() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-template <class Tag, int D, int MC>
-__global__ void __launch_bounds__(256, 2) kv4_prefill_kernel(const Kv4PrefillParams p) {
+template <class Tag, int D, int MC, int TEAMS>
+__global__ void __launch_bounds__(256 * TEAMS, 2) kv4_prefill_kernel(const Kv4PrefillParams p) {
   typedef Stage<D> St;
   constexpr int NP = Kv4Pieces<Tag>::n, KS = D / 32, EB = Tag::kBytes, SUB = St::SUB, NB = St::NB, KT = St::KT, KF = St::KF;
   constexpr int KA = KS < 4 ? KS : 4, VA = KS < 2 ? KS : 2;   // operands read ahead of their use
-  __shared__ bf16x8_t s_k[2][SUB][2][KS][64], s_v[2][SUB][KS][2][64];
-  __shared__ uint32_t s_nan[2][SUB][KS];   // tokens of a step whose V block was NaN (masked stages only)
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  struct Shared {   // one team's
+    bf16x8_t k[2][SUB][2][KS][64], v[2][SUB][KS][2][64];
+    uint32_t nan[2][SUB][KS];   // tokens of a step whose V block was NaN (masked stages only)
+  };
+  constexpr int kRow = D + 4;   // a column's sums, maximum and sum of weights on their way from team 1 to team 0
+  constexpr int kShared = TEAMS * (int)sizeof(Shared), kJoin = TEAMS > 1 ? kWaves * MC * 16 * kRow * 4 : 0;
+  __shared__ __attribute__((aligned(16))) char s_mem[kShared > kJoin ? kShared : kJoin];
+  const int lane = threadIdx.x & 63, wg_wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int team = TEAMS > 1 ? wg_wave / kWaves : 0, wave = TEAMS > 1 ? wg_wave % kWaves : wg_wave;
+  Shared& sh = reinterpret_cast<Shared*>(s_mem)[team];
   const int g = lane >> 4, col = lane & 15;
   int idx = blockIdx.x;
   const int sp = idx % p.nsplit;
@@ -72,7 +87,7 @@ __global__ void __launch_bounds__(256, 2) kv4_prefill_kernel(const Kv4PrefillPar
   idx /= p.Hkv;
   const int seg = idx % p.nseg;
   const int rt = p.row_tiles - 1 - idx / p.nseg;   // the longest contexts first
-  const int len = p.seg_len[seg], pos0 = p.seg_pos0[seg], q0 = p.seg_q0[seg];
+  const int q0 = p.seg_q0[seg], pos0 = p.seg_pos0[seg], len = segment_rows(p, q0, p.seg_len[seg]);
   const int rows = len * p.G, wg_row0 = rt * kWaves * MC * 16;
   if (wg_row0 >= rows) return;
   const int row0 = wg_row0 + wave * MC * 16;
@@ -97,9 +112,10 @@ __global__ void __launch_bounds__(256, 2) kv4_prefill_kernel(const Kv4PrefillPar
     }
   }
   auto limit = [&](int r) { return min(pos0 + min(r, rows - 1) / p.G, p.max_ctx - 1); };
-  const int wave_first = limit(row0), wave_last = row0 < rows ? limit(row0 + MC * 16 - 1) : -1;
+  const int wave_first = limit(row0);
   const int wg_first = limit(wg_row0), wg_end = limit(wg_row0 + kWaves * MC * 16 - 1);
   const int lo = sp * p.tps, wg_last = min(wg_end, lo + p.tps - 1);   // this workgroup's tokens: lo .. wg_last
+  const int wave_last = row0 < rows ? min(limit(row0 + MC * 16 - 1), wg_last) : -1;
   if (lo > wg_last && sp > 0) return;                                 // (the rows' own limits tell which splits are empty)
 
   f32x4 acc[MC][KS][2], sum[MC];
@@ -185,37 +201,39 @@ __global__ void __launch_bounds__(256, 2) kv4_prefill_kernel(const Kv4PrefillPar
       }
       if (lane == 0) {
 #pragma unroll
-        for (int b = 0; b < NB; ++b) s_nan[buf][vstep][vblk + b] = nan[b];
+        for (int b = 0; b < NB; ++b) sh.nan[buf][vstep][vblk + b] = nan[b];
       }
     }
 #pragma unroll
     for (int i = 0; i < KT; ++i) {
       const float sc = u2f(__builtin_amdgcn_alignbit(rks[i], rks[i], turn));
 #pragma unroll
-      for (int f = 0; f < KF; ++f) s_k[buf][kstep][KT == 2 ? i : ktile][kfirst + f][lane] = kv4_k_frag(rk[i][f], sc);
+      for (int f = 0; f < KF; ++f) sh.k[buf][kstep][KT == 2 ? i : ktile][kfirst + f][lane] = kv4_k_frag(rk[i][f], sc);
     }
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       bf16x8_t ev, od;
       kv4_v_frags(rv[0][b], rv[1][b], rvs[0][b], rvs[1][b], ev, od);
-      s_v[buf][vstep][vblk + b][0][lane] = ev;
-      s_v[buf][vstep][vblk + b][1][lane] = od;
+      sh.v[buf][vstep][vblk + b][0][lane] = ev;
+      sh.v[buf][vstep][vblk + b][1][lane] = od;
     }
   };
 
   if (wg_last >= lo) {
-    place(lo);
+    constexpr int kStride = TEAMS * St::kTokens;   // the teams take stages in turn
+    const int first = lo + team * St::kTokens;
+    place(first);
     fetch();
-    place(lo + St::kTokens);
-    convert(lo, 0);
+    place(first + kStride);
+    convert(first, 0);
     fetch();
-    place(lo + 2 * St::kTokens);
+    place(first + 2 * kStride);
     int buf = 0;
-    for (int t0 = lo; t0 <= wg_last; t0 += St::kTokens, buf ^= 1) {
+    for (int t0 = first; t0 - team * St::kTokens <= wg_last; t0 += kStride, buf ^= 1) {
       lds_barrier();
-      convert(t0 + St::kTokens, buf ^ 1);   // (behind the last stage: the last tile again, read by nobody)
+      convert(t0 + kStride, buf ^ 1);   // (behind the last stage: the last tile again, read by nobody)
       fetch();
-      place(min(t0 + 3 * St::kTokens, wg_last));
+      place(min(t0 + 3 * kStride, wg_last));
       const bool wg_masked = t0 + St::kTokens - 1 > wg_first;
 #pragma unroll
       for (int sub = 0; sub < SUB; ++sub) {
@@ -225,7 +243,7 @@ __global__ void __launch_bounds__(256, 2) kv4_prefill_kernel(const Kv4PrefillPar
         f32x4 S[MC][2];
         bf16x8_t kf[2][KA];   // K operands, read 2 KA ahead
 #pragma unroll
-        for (int f = 0; f < 2 * KA; ++f) kf[f / KA][f % KA] = s_k[buf][sub][f / KS][f % KS][lane];
+        for (int f = 0; f < 2 * KA; ++f) kf[f / KA][f % KA] = sh.k[buf][sub][f / KS][f % KS][lane];
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -235,7 +253,7 @@ __global__ void __launch_bounds__(256, 2) kv4_prefill_kernel(const Kv4PrefillPar
           for (int s = 0; s < KS; ++s) {
             const int f = i * KS + s;
             const bf16x8_t a = kf[f / KA % 2][f % KA];
-            if (f + 2 * KA < 2 * KS) kf[f / KA % 2][f % KA] = s_k[buf][sub][(f + 2 * KA) / KS][(f + 2 * KA) % KS][lane];
+            if (f + 2 * KA < 2 * KS) kf[f / KA % 2][f % KA] = sh.k[buf][sub][(f + 2 * KA) / KS][(f + 2 * KA) % KS][lane];
 #pragma unroll
             for (int mc = 0; mc < MC; ++mc)
 #pragma unroll
@@ -245,14 +263,14 @@ __global__ void __launch_bounds__(256, 2) kv4_prefill_kernel(const Kv4PrefillPar
         bf16x8_t vf[VA][2];   // V operands of the first blocks, on their way during the softmax
 #pragma unroll
         for (int s = 0; s < VA; ++s) {
-          vf[s][0] = s_v[buf][sub][s][0][lane];
-          vf[s][1] = s_v[buf][sub][s][1][lane];
+          vf[s][0] = sh.v[buf][sub][s][0][lane];
+          vf[s][1] = sh.v[buf][sub][s][1][lane];
         }
         __builtin_amdgcn_sched_barrier(0);
         if (wg_masked) {
 #pragma unroll
           for (int s = 0; s < KS; ++s) {
-            const uint32_t nan = __builtin_amdgcn_readfirstlane(s_nan[buf][sub][s]);
+            const uint32_t nan = __builtin_amdgcn_readfirstlane(sh.nan[buf][sub][s]);
             if (nan) {
 #pragma unroll
               for (int mc = 0; mc < MC; ++mc) {
@@ -303,8 +321,8 @@ __global__ void __launch_bounds__(256, 2) kv4_prefill_kernel(const Kv4PrefillPar
         for (int s = 0; s < KS; ++s) {
           const bf16x8_t ev = vf[s % VA][0], od = vf[s % VA][1];
           if (s + VA < KS) {
-            vf[s % VA][0] = s_v[buf][sub][s + VA][0][lane];
-            vf[s % VA][1] = s_v[buf][sub][s + VA][1][lane];
+            vf[s % VA][0] = sh.v[buf][sub][s + VA][0][lane];
+            vf[s % VA][1] = sh.v[buf][sub][s + VA][1][lane];
           }
 #pragma unroll
           for (int mc = 0; mc < MC; ++mc)
@@ -318,6 +336,40 @@ __global__ void __launch_bounds__(256, 2) kv4_prefill_kernel(const Kv4PrefillPar
     }
   }
 
+  if constexpr (TEAMS > 1) {
+    float* const join = reinterpret_cast<float*>(s_mem) + (wave * MC * 16 + col) * kRow;
+    __syncthreads();   // (nobody reads operands any more)
+    if (team == 1) {
+#pragma unroll
+      for (int mc = 0; mc < MC; ++mc) {
+        float* const row = join + mc * 16 * kRow;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          *reinterpret_cast<f32x4*>(row + 32 * s + 8 * g) = acc[mc][s][0];
+          *reinterpret_cast<f32x4*>(row + 32 * s + 8 * g + 4) = acc[mc][s][1];
+        }
+        if (g == 0) row[D] = m2[mc], row[D + 1] = sum[mc][0];
+      }
+    }
+    __syncthreads();
+    if (team == 1) return;
+#pragma unroll
+    for (int mc = 0; mc < MC; ++mc) {
+      const float* const row = join + mc * 16 * kRow;
+      const float M = fmaxf(m2[mc], row[D]), fa = fast_exp2(m2[mc] - M), fb = fast_exp2(row[D] - M);
+      m2[mc] = M;
+      sum[mc][0] = __builtin_fmaf(row[D + 1], fb, sum[mc][0] * fa);
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const f32x4 e = *reinterpret_cast<const f32x4*>(row + 32 * s + 8 * g), o = *reinterpret_cast<const f32x4*>(row + 32 * s + 8 * g + 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          acc[mc][s][0][i] = __builtin_fmaf(e[i], fb, acc[mc][s][0][i] * fa);
+          acc[mc][s][1][i] = __builtin_fmaf(o[i], fb, acc[mc][s][1][i] * fa);
+        }
+      }
+    }
+  }
 #pragma unroll
   for (int mc = 0; mc < MC; ++mc) {
     if (orow[mc] < 0) continue;
@@ -352,9 +404,10 @@ __global__ void __launch_bounds__(256) kv4_prefill_merge_kernel(const Kv4Prefill
   const int hq = (int)(item % p.Hq);
   const int64_t st = item / p.Hq;
   const int tok = (int)(st % max_q_len), seg = (int)(st / max_q_len);
-  if (tok >= p.seg_len[seg]) return;
+  const int q0 = p.seg_q0[seg];
+  if (tok >= segment_rows(p, q0, p.seg_len[seg])) return;
   const int lim = min(p.seg_pos0[seg] + tok, p.max_ctx - 1);
-  const int64_t row = (int64_t)(p.seg_q0[seg] + tok) * p.Hq + hq;
+  const int64_t row = (int64_t)(q0 + tok) * p.Hq + hq;
   kv4_join_splits<Tag, D, SL>(p.out + row * D * Tag::kBytes, p.ws + row * p.nsplit * (D + 4),
                               lim < 0 ? 0 : min(lim / p.tps + 1, p.nsplit));
 }
@@ -366,7 +419,7 @@ void launch_merge(const Kv4PrefillParams& p, int max_q_len, hipStream_t s) {
 }
 
 struct Kv4PrefillPlan {
-  int MC, row_tiles, nsplit, tps;
+  int MC, teams, row_tiles, nsplit, tps;
   size_t ws_bytes;
 };
 
@@ -380,39 +433,54 @@ int make_plan(const char* what, int nseg, int total_rows, int max_q_len, int Hq,
                 total_rows, max_q_len, Hq, Hkv, max_ctx);
   const int64_t rows = (int64_t)max_q_len * (Hq / Hkv), heads = (int64_t)std::max(nseg, 1) * Hkv;
   if (rows > INT32_MAX) return fail(MI355_EINVAL, "%s: max_q_len %d", what, max_q_len);
-  // Two tiles of 16 rows per wave use every converted operand twice, one tile makes twice the workgroups.  Figures: us, two /
-  // one.  head_dim 64: 8 prompts of 4096 168 / 193, 16 uneven chunks to 1024 46 / 42; head_dim 128: 8 prompts of 1024
-  // 37 / 42, 4 of 300 with 32/8 heads 32 / 38, 4 of 300 with 8 heads 28 / 22; 2 of 256 behind 3000, split, 51 / 56.
+  // Two tiles of 16 rows per wave use every converted operand twice, one tile makes twice the workgroups.  Two teams per
+  // workgroup halve the stages of its walk and fill a chip that has too few workgroups, but take twice its LDS: they pay while
+  // all workgroups fit at once, one per CU, or (deep contexts, up to 64 dims) two.  us, as chosen / the other way:
+  //   two tiles: 8 prompts of 4096, 8 heads of 64 172 / 197; 8 of 1024, 8 of 128 37 / 42; 4 of 300, 32/8 of 128 32 / 37
+  //   one tile: 16 uneven chunks to 1024, 8 of 64 43 / 47; 12 uneven fp16 prompts to 1500 49 / 54; 5 of 512, 8 of 128 17 / 22
+  //   two teams: a prompt of 2000, 8 heads of 64 22 / 29; one of 500, 32/8 of 128 14.4 / 16.3; 2 of 128 behind 2000, 32/8 of
+  //   256 44 / 78; 8 of 512 behind 2000, 8 of 64 38 / 46; two tiles: 4 of 256 behind 3000, 32/8 of 128 67 / 88
+  //   one team: 12 uneven prompts to 400, 8 of 64 10.7 / 12.2; 8 of 4096, 8 of 64 172 / 228; 16 of 100 7.5 / 7.9
   // Two tiles' registers at head_dim 256 (fp32: 128) would leave one wave per SIMD.
   const bool narrow = D == 256 || (dtype == MI355_F32 && D == 128);
-  const int64_t wgs2 = heads * ceil_div64(rows, kWaves * 32);
-  pl->MC = !narrow && (wgs2 >= (D == 128 ? 256 : 1024) || (D == 128 && wgs2 >= 128 && max_ctx >= 2048)) ? 2 : 1;
+  const int64_t all_rows = (int64_t)total_rows * (Hq / Hkv);
+  auto workgroups = [&](int mc) {   // of uneven segments: no more than the rows there are
+    const int64_t per = kWaves * 16 * mc;
+    return std::min(heads * ceil_div64(rows, per), Hkv * (ceil_div64(all_rows, per) + nseg));
+  };
+  const int64_t wgs1 = workgroups(1), wgs2 = workgroups(2);
+  const bool deep = max_ctx >= 1536;
+  pl->MC = !narrow && (D <= 64 ? wgs2 >= 1024 : wgs2 > 256 || (wgs1 > 256 && deep)) ? 2 : 1;
+  pl->teams = 1;
+  if (max_ctx >= 256 && wgs1 <= 256) pl->teams = 2;
+  if (deep && (D <= 64 ? wgs1 <= 512 : pl->MC == 2 && wgs2 <= 256)) pl->teams = 2;
   pl->row_tiles = (int)ceil_div64(rows, kWaves * pl->MC * 16);
-  const int64_t wgs = heads * pl->row_tiles;
   const int stage = kKv4Step * (D == 256 ? 1 : D == 32 ? 4 : 2);
   const int64_t stages = ceil_div64(max_ctx, stage);
-  // Few workgroups behind a long context: the context is split until there are two per CU, no split shorter than 256 tokens
-  // (16 tokens behind 30000, 32/8 heads of 128: 524 -> 29; 8 chunks to 45 behind 900: 17.4 -> 12.6).  The merge costs about
-  // 5 us and the rows' partial sums: 500 tokens, 32/8 heads of 128, 16.3 unsplit, 22.8 in two.
-  int64_t want = 1;
-  if ((wgs <= 128 && max_ctx >= 768) || (wgs <= 256 && max_ctx >= 2048))
-    want = std::min<int64_t>(512 / std::max<int64_t>(wgs, 1), ceil_div64(max_ctx, 256));
+  // Still fewer than one workgroup per CU: the context is split until there is one, no split shorter than 256 tokens (16
+  // tokens behind 30000, 32/8 heads of 128: 348 -> 27; 8 chunks to 45 behind 900: 13.9 -> 12.4).  The merge costs about
+  // 5 us and the rows' partial sums: 128 tokens behind 1000, 32/8 heads of 128, 21.5 unsplit, 22.9 in two.
+  int64_t want = wgs1 <= 256 ? std::min<int64_t>(256 / std::max<int64_t>(wgs1, 1), ceil_div64(max_ctx, 256)) : 1;
+  if (max_ctx - max_ctx / want < 640) want = 1;
   const int64_t per = ceil_div64(stages, std::min(want, stages));
   pl->tps = (int)(per * stage);
   pl->nsplit = (int)ceil_div64(stages, per);
   pl->ws_bytes = pl->nsplit > 1 ? (size_t)total_rows * Hq * pl->nsplit * (D + 4) * sizeof(float) : 0;
-  if (wgs * pl->nsplit > INT32_MAX || (int64_t)nseg * max_q_len * Hq > INT32_MAX)
+  if (heads * pl->row_tiles * pl->nsplit > INT32_MAX || (int64_t)nseg * max_q_len * Hq > INT32_MAX)
     return fail(MI355_EINVAL, "%s: too many workgroups (nseg=%d max_q_len=%d Hq=%d)", what, nseg, max_q_len, Hq);
   return 0;
 }
 
 template <class Tag, int D>
 int launch(const Kv4PrefillParams& p, const Kv4PrefillPlan& pl, int max_q_len, hipStream_t s) {
-  const dim3 grid((unsigned)((int64_t)p.row_tiles * p.nseg * p.Hkv * p.nsplit)), block(256);
+  const dim3 grid((unsigned)((int64_t)p.row_tiles * p.nseg * p.Hkv * p.nsplit)), one(256), two(512);
   if constexpr (D < 256 && !(Tag::kCode == MI355_F32 && D == 128)) {
-    if (pl.MC == 2) hipLaunchKernelGGL((kv4_prefill_kernel<Tag, D, 2>), grid, block, 0, s, p);
+    if (pl.MC == 2 && pl.teams == 1) hipLaunchKernelGGL((kv4_prefill_kernel<Tag, D, 2, 1>), grid, one, 0, s, p);
+    if constexpr (D == 128)
+      if (pl.MC == 2 && pl.teams == 2) hipLaunchKernelGGL((kv4_prefill_kernel<Tag, D, 2, 2>), grid, two, 0, s, p);
   }
-  if (pl.MC == 1) hipLaunchKernelGGL((kv4_prefill_kernel<Tag, D, 1>), grid, block, 0, s, p);
+  if (pl.MC == 1 && pl.teams == 1) hipLaunchKernelGGL((kv4_prefill_kernel<Tag, D, 1, 1>), grid, one, 0, s, p);
+  if (pl.MC == 1 && pl.teams == 2) hipLaunchKernelGGL((kv4_prefill_kernel<Tag, D, 1, 2>), grid, two, 0, s, p);
   if (int rc = check_launch("kv4_prefill_kernel")) return rc;
   if (p.nsplit > 1) {
     if (p.nsplit <= kKv4WalkedSplits) launch_merge<Tag, D, kv4_split_lanes<D>(true)>(p, max_q_len, s);
@@ -477,6 +545,7 @@ extern "C" int mi355_paged_prefill_kv4(void* out, const void* q, int64_t q_strid
   p.seg_pos0 = seg_pos0;
   p.q_stride = q_stride_tok;
   p.nseg = nseg;
+  p.total_rows = total_rows;
   p.Hq = Hq;
   p.Hkv = Hkv;
   p.G = Hq / Hkv;
