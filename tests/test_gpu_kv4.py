@@ -138,6 +138,36 @@ def test_append_rounds_rotates_and_scatters(ops, device, dtype, T, Hq, Hkv, D, B
                 assert not got[t].any()
 
 
+@pytest.mark.parametrize('dtype', ALL)
+@pytest.mark.parametrize('T,Hq,Hkv,D,BS,R,inter', [(12301, 4, 8, 64, 16, 64, False), (3075, 2, 8, 256, 48, 128, True),
+                                                   (24601, 1, 8, 32, 32, 32, False), (6145, 3, 8, 128, 16, 0, False)])
+def test_append_and_read_of_many_rows_equal_those_of_few(ops, device, dtype, T, Hq, Hkv, D, BS, R, inter):
+    """A call long enough for two tokens per thread gives the bytes and values of short calls (which the test above
+    holds against the oracle): slots in runs of either parity, scattered, backwards and outside the cache."""
+    rng = np.random.default_rng(T)
+    (q, k, v), _ = _rows(rng, T, Hq, Hkv, D, dtype)
+    cos, sin, _, _ = _angle_rows(ops, rng, T, R)
+    NB = -(-T // BS) + 9
+    slots = np.arange(T) + 7
+    slots[1000:1501] = slots[1000:1501][rng.permutation(501)]
+    slots[1600:1701] = slots[1600:1701][::-1]
+    slots[2001:3001] = np.roll(slots[2001:3001], 1)
+    slots[[5, 900, 901, T - 1]] = [-1, NB * BS, NB * BS + 1, -2]
+    slots = torch.from_numpy(slots).cuda()
+    caches = [[torch.full(ops.kv4_cache_shape(NB, Hkv, BS, D), 90, dtype=torch.uint8, device=device) for _ in range(2)] for _ in range(2)]
+    whole = ops.rope_kv4_write(q, k, v, cos, sin, slots, *caches[0], interleaved=inter)
+    rk, rv = ops.kv4_read_slots(*caches[0], slots, dtype)
+    for a in range(0, T, 500):
+        b = min(a + 500, T)
+        part = ops.rope_kv4_write(q[a:b], k[a:b], v[a:b], *((cos[a:b], sin[a:b]) if R else (None, None)), slots[a:b], *caches[1],
+                                  interleaved=inter)
+        assert torch.equal(whole[a:b], part)
+    for a in range(0, T, 500):
+        pk, pv = ops.kv4_read_slots(*caches[1], slots[a:a + 500], dtype)
+        assert torch.equal(rk[a:a + 500], pk) and torch.equal(rv[a:a + 500], pv)
+    assert torch.equal(caches[0][0], caches[1][0]) and torch.equal(caches[0][1], caches[1][1])
+
+
 def test_append_values_at_borders_extremes_and_nan(ops, device):
     D, T = 64, 9
     x = np.zeros((T, 1, D))
