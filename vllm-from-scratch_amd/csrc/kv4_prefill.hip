@@ -458,10 +458,12 @@ int make_plan(const char* what, int nseg, int total_rows, int max_q_len, int Hq,
   const int stage = kKv4Step * (D == 256 ? 1 : D == 32 ? 4 : 2);
   const int64_t stages = ceil_div64(max_ctx, stage);
   // Still fewer than one workgroup per CU: the context is split until there is one, no split shorter than 256 tokens (16
-  // tokens behind 30000, 32/8 heads of 128: 348 -> 27; 8 chunks to 45 behind 900: 13.9 -> 12.4).  The merge costs about
-  // 5 us and the rows' partial sums: 128 tokens behind 1000, 32/8 heads of 128, 21.5 unsplit, 22.9 in two.
+  // tokens behind 30000, 32/8 heads of 128: 348 -> 27 us; 8 chunks to 64 behind 2000, 8 heads of 64: 23.2 -> 15.4), if that
+  // takes 800 tokens off a walk.  The merge costs a launch (4.4 us of the host's time) and the rows' partial sums: 8 chunks
+  // to 45 behind 900 take 13.9 in one, 12.4 in four splits and 17 where the host is what they wait for; 128 tokens behind
+  // 1000, 32/8 heads of 128, 21.5 in one, 22.9 in two.
   int64_t want = wgs1 <= 256 ? std::min<int64_t>(256 / std::max<int64_t>(wgs1, 1), ceil_div64(max_ctx, 256)) : 1;
-  if (max_ctx - max_ctx / want < 640) want = 1;
+  if (max_ctx - max_ctx / want < 800) want = 1;
   const int64_t per = ceil_div64(stages, std::min(want, stages));
   pl->tps = (int)(per * stage);
   pl->nsplit = (int)ceil_div64(stages, per);
