@@ -470,8 +470,8 @@ int mi355_rope_angles(float* cos_out, float* sin_out, const int64_t* positions, 
  *   a' = a cos[t][i] - b sin[t][i],  b' = b cos[t][i] + a sin[t][i]      (one rounding per value)
  *   out [T, H, D] contiguous; x [T, H, D], x_stride_tok elements between tokens, heads D apart;
  *   cos_rows / sin_rows [T, rotary_dim / 2] floats, one row per token (mi355_rope_angles);
- *   rotary_dim a multiple of 16 in [0, D] (0: cos_rows / sin_rows may be NULL); out must not
- *   overlap x.  D in {32, 64, 128, 256}.
+ *   rotary_dim a multiple of 16 in [0, D] (0: cos_rows / sin_rows may be NULL); an out that
+ *   overlaps x is refused.  D in {32, 64, 128, 256}.
  */
 int mi355_rope_rotate(void* out, const void* x, int64_t x_stride_tok, const float* cos_rows,
                       const float* sin_rows, int32_t rotary_dim, int32_t interleaved, int32_t T, int32_t H,
@@ -480,7 +480,7 @@ int mi355_rope_rotate(void* out, const void* x, int64_t x_stride_tok, const floa
 /*
  * mi355_rope_rotate of the query rows (to q_out [T, Hq, D]), and the rotated key rows and the value
  * rows rounded into the 4-bit cache at slots[t]: one launch, q / k / v are read only and may be views
- * of one projection output.  Keys are rotated in double and rounded once, to 4 bits, so that the
+ * of one projection output (which q_out must not overlap).  Keys are rotated in double and rounded once, to 4 bits, so that the
  * codes are those of the real product.  Tokens whose slot is negative or >= num_blocks * block_size
  * have no cache write (their query row is rotated all the same); two tokens must not share a slot.
  */

@@ -498,6 +498,45 @@ def test_chunk_rows_outside_the_tensors_are_left_out(ops, device, ctx):
     _near(out[[0, 1, 2, 3, 14, 15, 16, 17, 18, 19]], want, _attention_bound(size, most, want, D, ctx, torch.bfloat16))
 
 
+@pytest.mark.parametrize('ctx', [60, 3000])
+def test_chunk_queries_before_the_first_position_see_nothing(ops, device, ctx):
+    """A negative first position: zeros, whatever the cached rows hold; the queries from position 0 on as ever.  A loose
+    max_q_len and a segment longer than a tight one."""
+    rng = np.random.default_rng(3)
+    Hq, Hkv, D, BS = 4, 2, 64, 16
+    kc, vc, tables = _cache(rng, [ctx, 40, 40], Hkv, D, BS)
+    vc[tables[0, 0], :, 0, orc.scale_place(D, 0, 0, True)] = 255
+    q, qv = _cast(rng.standard_normal((30, Hq, D)), torch.bfloat16)
+    start, lens, pos0 = [0, 10, 20], [6, 10, 9], [-6, -4, 30]
+    meta = torch.tensor([start, lens, pos0], dtype=torch.int32, device=device)
+    args = [torch.from_numpy(a).cuda() for a in (kc, vc, tables)]
+    want, size, most = _attend_all([qv[14:20], qv[20:29]], kc, vc, tables[1:], [40] * 2, D ** -0.5,
+                                   [list(range(6)), [30 + j for j in range(9)]])
+    bound = _attention_bound(size, most, want, D, 40, torch.bfloat16)
+    for longest, rows in ((10, 9), (1 << 30, 9), (7, 7)):
+        out = torch.full((30, Hq, D), 7.0, dtype=torch.bfloat16, device=device)
+        ops.paged_prefill_kv4(q, *args, meta[0], meta[1], meta[2], longest, ctx, out=out)
+        assert not out[:6].any() and not out[10:14].any() and bool((out[6:10] == 7.0).all())
+        got = [j for j in range(14, 20) if j - 10 < longest] + list(range(20, 20 + rows))
+        pick = [j - 14 for j in got]
+        _near(out[got], want[pick], bound[pick])
+        assert bool((out[20 + rows:] == 7.0).all())
+
+
+def test_outputs_that_overlap_their_rows_are_refused(ops, device):
+    from mi355_paged._lib import Mi355Error
+    qkv = torch.randn(1, 3 * 4 * 64, device=device, dtype=torch.bfloat16)
+    q, k, v = (t.view(1, 4, 64) for t in qkv.chunk(3, -1))            # one token: views that are contiguous
+    cos, sin = torch.ones(1, 32, device=device), torch.zeros(1, 32, device=device)
+    caches = [torch.zeros(ops.kv4_cache_shape(2, 4, 16, 64), dtype=torch.uint8, device=device) for _ in range(2)]
+    slots = torch.zeros(1, dtype=torch.int64, device=device)
+    for x in (q, k, v):
+        with pytest.raises(Mi355Error, match='overlaps'):
+            ops.rope_kv4_write(q, k, v, cos, sin, slots, *caches, out=x)
+    with pytest.raises(Mi355Error, match='overlaps'):
+        ops.rope_rotate(q, cos, sin, out=q)
+
+
 def test_chunk_nan_reaches_only_the_queries_that_see_it(ops, device):
     """A NaN key or value at a position of the chunk itself: the queries before it stay finite, whatever
     else shares their tiles."""

@@ -90,6 +90,8 @@ def test_rope_frequencies_refuses(args):
 
 # ------------------------------------------------------------------ refusals (no device is touched)
 P = 4096            # a well aligned address that no refused call reads
+OUT = 1 << 24       # one behind it
+LONG = (1 << 31) - 1
 
 
 def _call(name, good, **change):
@@ -99,8 +101,8 @@ def _call(name, good, **change):
 
 
 ANGLES = dict(cos=P, sin=P, positions=P, freq=P, factor=1.0, T=4, half=8, stream=None)
-ROTATE = dict(out=P, x=P, stride=8 * 64, cos=P, sin=P, R=64, inter=0, T=4, H=8, D=64, dtype=1, stream=None)
-WRITE = dict(q_out=P, q=P, k=P, v=P, qs=1536, ks=1536, vs=1536, cos=P, sin=P, R=64, inter=0, slots=P, kc=P, vc=P, T=4,
+ROTATE = dict(out=OUT, x=P, stride=8 * 64, cos=P, sin=P, R=64, inter=0, T=4, H=8, D=64, dtype=1, stream=None)
+WRITE = dict(q_out=OUT, q=P, k=P, v=P, qs=1536, ks=1536, vs=1536, cos=P, sin=P, R=64, inter=0, slots=P, kc=P, vc=P, T=4,
              Hq=8, Hkv=8, D=64, BS=16, NB=10, sb=8 * 544, sh=544, dtype=1, stream=None)
 READ = dict(ko=P, vo=P, kc=P, vc=P, slots=P, T=4, Hkv=8, D=64, BS=16, NB=10, sb=8 * 544, sh=544, dtype=1, stream=None)
 DECODE = dict(out=P, q=P, qs=512, kc=P, vc=P, bt=P, ctx=P, B=2, Hq=8, Hkv=8, D=64, BS=16, mb=4, NB=10, max_ctx=64,
@@ -112,26 +114,27 @@ CACHE = [(dict(kc=None), -1), (dict(vc=None), -1), (dict(kc=P + 8), -1), (dict(D
          (dict(sh=528), -1), (dict(sb=528), -1), (dict(dtype=3), -1), (dict(sh=-544), -1)]
 REFUSED = (
     [('mi355_rope_angles', ANGLES, c, -1) for c in (dict(cos=None), dict(sin=None), dict(positions=None), dict(freq=None),
-                                                  dict(T=-1), dict(half=0))] +
+                                                  dict(T=-1), dict(half=0), dict(T=LONG))] +
     [('mi355_rope_rotate', ROTATE, c, r) for c, r in (
         (dict(out=None), -1), (dict(x=None), -1), (dict(cos=None), -1), (dict(sin=None), -1), (dict(R=8), -1), (dict(R=80), -1),
         (dict(R=-16), -1), (dict(T=-1), -1), (dict(H=0), -1), (dict(D=48), -2), (dict(dtype=7), -1), (dict(stride=504), -1),
-        (dict(stride=516), -1), (dict(x=P + 4), -1), (dict(out=P + 2), -1), (dict(cos=P + 4), -1))] +
+        (dict(stride=516), -1), (dict(x=P + 4), -1), (dict(out=OUT + 2), -1), (dict(cos=P + 4), -1), (dict(T=LONG), -1),
+        (dict(out=P), -1), (dict(out=P + 4 * 1024 - 16), -1), (dict(x=OUT + 4 * 1024 - 16), -1))] +
     [('mi355_rope_kv4_write', WRITE, c, r) for c, r in CACHE + [
         (dict(q_out=None), -1), (dict(q=None), -1), (dict(k=None), -1), (dict(v=None), -1), (dict(slots=None), -1),
         (dict(ks=504), -1), (dict(vs=1540), -1), (dict(k=P + 2), -1), (dict(Hq=0), -1), (dict(R=24), -1), (dict(cos=None), -1),
-        (dict(T=-3), -1)]] +
+        (dict(T=-3), -1), (dict(T=LONG), -1), (dict(q_out=P), -1), (dict(k=OUT + 2048), -1), (dict(v=OUT - 3 * 3072 - 512), -1)]] +
     [('mi355_kv4_read_slots', READ, c, r) for c, r in CACHE + [
-        (dict(ko=None), -1), (dict(vo=P + 8), -1), (dict(slots=None), -1), (dict(T=-1), -1)]] +
+        (dict(ko=None), -1), (dict(vo=P + 8), -1), (dict(slots=None), -1), (dict(T=-1), -1), (dict(T=LONG), -1)]] +
     [('mi355_paged_decode_kv4', DECODE, c, r) for c, r in CACHE + [
         (dict(out=None), -1), (dict(q=None), -1), (dict(bt=None), -1), (dict(ctx=None), -1), (dict(qs=504), -1), (dict(qs=516), -1),
         (dict(q=P + 8), -1), (dict(Hq=12), -1), (dict(Hq=0), -1), (dict(B=-1), -1), (dict(mb=0), -1), (dict(max_ctx=-1), -1),
         (dict(max_ctx=100000, mb=7000, ws=None), -3), (dict(max_ctx=100000, mb=7000, wsb=64), -3),
-        (dict(max_ctx=100000, mb=7000, ws=P + 4), -3), (dict(max_ctx=1 << 30, mb=1 << 27), -1)]] +
+        (dict(max_ctx=100000, mb=7000, ws=P + 4), -3), (dict(max_ctx=1 << 30, mb=1 << 27), -1), (dict(B=1 << 24), -1)]] +
     [('mi355_paged_prefill_kv4', CHUNK, c, r) for c, r in CACHE + [
         (dict(out=None), -1), (dict(q=None), -1), (dict(bt=None), -1), (dict(q0=None), -1), (dict(ln=None), -1), (dict(pos=None), -1),
         (dict(qs=504), -1), (dict(q=P + 8), -1), (dict(Hq=12), -1), (dict(nseg=-1), -1), (dict(max_q=-1), -1), (dict(mb=0), -1),
-        (dict(max_ctx=0), -1), (dict(max_q=1 << 30, Hq=64, qs=4096), -1), (dict(rows=-1), -1),
+        (dict(max_ctx=0), -1), (dict(max_q=1 << 30, rows=1 << 30, Hq=64, qs=4096), -1), (dict(nseg=1 << 20, rows=1 << 20, max_q=1 << 16), -1), (dict(rows=-1), -1),
         (dict(max_ctx=100000, mb=7000, ws=None), -3), (dict(max_ctx=100000, mb=7000, wsb=64), -3),
         (dict(max_ctx=100000, mb=7000, ws=P + 4), -3), (dict(max_ctx=1 << 30, mb=1 << 27), -1)]])
 
@@ -159,6 +162,8 @@ def test_workspace_queries_are_host_arithmetic():
     assert lib.mi355_paged_decode_kv4_workspace_bytes(1, 8, 8, 48, 100000, 1) == 0        # refused: the call says why
     assert lib.mi355_paged_prefill_kv4_workspace_bytes(1, 8, 8, 8, 8, 64, 100000, 1) > 0
     assert lib.mi355_paged_prefill_kv4_workspace_bytes(8, 8192, 1024, 8, 8, 64, 1024, 1) == 0
+    assert lib.mi355_paged_prefill_kv4_workspace_bytes(1, 8, 1 << 30, 8, 8, 64, 100000, 1) == \
+        lib.mi355_paged_prefill_kv4_workspace_bytes(1, 8, 8, 8, 8, 64, 100000, 1)              # no more rows than there are
 
 
 def test_ops_refuse_host_tensors():

@@ -34,6 +34,8 @@ constexpr float kKv4Floor = -3e38f;   // a running maximum no score has raised y
 constexpr float kKv4Raise = 8.f;      // powers of two a score may pass the running maximum by before it is raised
 
 static inline bool kv4_dtype_ok(int dtype) { return dtype == MI355_F32 || dtype == MI355_BF16 || dtype == MI355_F16; }
+// A launch has fewer than 2^32 threads.
+static inline bool kv4_grid_ok(int64_t workgroups, int threads) { return workgroups <= (int64_t)(UINT32_MAX / (uint32_t)threads); }
 static inline bool kv4_head_dim_ok(int D) { return D == 32 || D == 64 || D == 128 || D == 256; }
 
 // Geometry shared by every kernel over the cache; strides in bytes.
@@ -131,7 +133,7 @@ __device__ __forceinline__ f32x4 mfma_bf16(bf16x8_t a, bf16x8_t b, f32x4 c) {
 
 // N = 1, 2, 3 bf16 pieces of eight floats whose sum is the float to 8, 16, 24 bits: what makes the
 // bf16 matrix instruction exact for bf16, fp16 and fp32 operands against codes that bf16 holds
-// exactly.  (A value beyond bf16's range never occurs: fp32 and bf16 share the exponent.)
+// exactly.  (An fp32 value above bf16's largest, 3.39e38, counts as an infinity.)
 template <int N>
 __device__ __forceinline__ void bf16_pieces(const float (&x)[8], bf16x8_t (&out)[N]) {
   float rest[8];

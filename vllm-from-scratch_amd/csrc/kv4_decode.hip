@@ -18,7 +18,6 @@
 namespace mi355 {
 namespace {
 
-
 struct Kv4DecodeParams {
   char* out;
   const char* q;
@@ -371,7 +370,8 @@ extern "C" int mi355_paged_decode_kv4(void* out, const void* q, int64_t q_stride
   if (pl.ws_bytes && (!workspace || workspace_bytes < pl.ws_bytes || ((uintptr_t)workspace & 15)))
     return fail(MI355_EWORKSPACE, "paged_decode_kv4: workspace of %zu bytes needed (16-byte aligned), %zu given", pl.ws_bytes,
                 workspace ? workspace_bytes : (size_t)0);
-  if ((int64_t)B * pl.hgroups * pl.qchunks * pl.nsplit > INT32_MAX || (int64_t)B * Hq > INT32_MAX)
+  if (!kv4_grid_ok((int64_t)B * pl.hgroups * pl.qchunks * pl.nsplit, pl.W * 64) || (pl.nsplit > 1 && !kv4_grid_ok((int64_t)B * Hq, 256)) ||
+      (int64_t)B * Hq > INT32_MAX)
     return fail(MI355_EINVAL, "paged_decode_kv4: too many workgroups (B=%d Hq=%d)", B, Hq);
   Kv4DecodeParams p;
   p.out = static_cast<char*>(out);

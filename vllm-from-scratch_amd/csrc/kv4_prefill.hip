@@ -47,14 +47,14 @@ struct Kv4PrefillParams {
   const int32_t* seg_pos0;
   int64_t q_stride;   // elements
   float* ws;   // [total rows * Hq][nsplit][D + 4]: unnormalised sums, running maximum, sum of weights
-  int nseg, total_rows, Hq, Hkv, G, max_blocks, max_ctx, row_tiles, nsplit, tps /* tokens per split, whole stages */;
+  int nseg, total_rows, max_q_len, Hq, Hkv, G, max_blocks, max_ctx, row_tiles, nsplit, tps /* tokens per split, whole stages */;
   float scale2, raise;   // |scale| * log2(e); kKv4Raise in units of a raw score
   int flip;              // a negative scale: the queries are negated
 };
 
 // Rows of a segment; none outside the tensors, whatever the segment says.
 __device__ __forceinline__ int segment_rows(const Kv4PrefillParams& p, int q0, int len) {
-  return q0 < 0 || q0 >= p.total_rows ? 0 : min(len, p.total_rows - q0);
+  return q0 < 0 || q0 >= p.total_rows ? 0 : min(min(len, p.max_q_len), p.total_rows - q0);
 }
 
 // Between two waves' uses of LDS; global loads may stay in flight across it.
@@ -398,12 +398,12 @@ __global__ void __launch_bounds__(256 * TEAMS, 2) kv4_prefill_kernel(const Kv4Pr
 
 // Joins the splits of the segments' query rows; items are (segment, token, query head).
 template <class Tag, int D, int SL>
-__global__ void __launch_bounds__(256) kv4_prefill_merge_kernel(const Kv4PrefillParams p, int max_q_len, int64_t items) {
+__global__ void __launch_bounds__(256) kv4_prefill_merge_kernel(const Kv4PrefillParams p, int64_t items) {
   const int64_t item = (int64_t)blockIdx.x * (256 / (SL * D / 8)) + (SL == 1 ? threadIdx.x / (D / 8) : 0);
   if (item >= items) return;
   const int hq = (int)(item % p.Hq);
   const int64_t st = item / p.Hq;
-  const int tok = (int)(st % max_q_len), seg = (int)(st / max_q_len);
+  const int tok = (int)(st % p.max_q_len), seg = (int)(st / p.max_q_len);
   const int q0 = p.seg_q0[seg];
   if (tok >= segment_rows(p, q0, p.seg_len[seg])) return;
   const int lim = min(p.seg_pos0[seg] + tok, p.max_ctx - 1);
@@ -412,10 +412,10 @@ __global__ void __launch_bounds__(256) kv4_prefill_merge_kernel(const Kv4Prefill
                               lim < 0 ? 0 : min(lim / p.tps + 1, p.nsplit));
 }
 template <class Tag, int D, int SL>
-void launch_merge(const Kv4PrefillParams& p, int max_q_len, hipStream_t s) {
-  const int64_t items = (int64_t)p.nseg * max_q_len * p.Hq;
+void launch_merge(const Kv4PrefillParams& p, hipStream_t s) {
+  const int64_t items = (int64_t)p.nseg * p.max_q_len * p.Hq;
   hipLaunchKernelGGL((kv4_prefill_merge_kernel<Tag, D, SL>), dim3((unsigned)ceil_div64(items, 256 / (SL * D / 8))), dim3(256), 0,
-                     s, p, max_q_len, items);
+                     s, p, items);
 }
 
 struct Kv4PrefillPlan {
@@ -431,6 +431,7 @@ int make_plan(const char* what, int nseg, int total_rows, int max_q_len, int Hq,
   if (nseg < 0 || total_rows < 0 || max_q_len < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || max_ctx <= 0 || max_ctx > kKv4MaxContext)
     return fail(MI355_EINVAL, "%s: bad shape (nseg=%d total_rows=%d max_q_len=%d Hq=%d Hkv=%d max_context=%d)", what, nseg,
                 total_rows, max_q_len, Hq, Hkv, max_ctx);
+  max_q_len = std::min(max_q_len, total_rows);
   const int64_t rows = (int64_t)max_q_len * (Hq / Hkv), heads = (int64_t)std::max(nseg, 1) * Hkv;
   if (rows > INT32_MAX) return fail(MI355_EINVAL, "%s: max_q_len %d", what, max_q_len);
   // Two tiles of 16 rows per wave use every converted operand twice, one tile makes twice the workgroups.  Two teams per
@@ -468,13 +469,14 @@ int make_plan(const char* what, int nseg, int total_rows, int max_q_len, int Hq,
   pl->tps = (int)(per * stage);
   pl->nsplit = (int)ceil_div64(stages, per);
   pl->ws_bytes = pl->nsplit > 1 ? (size_t)total_rows * Hq * pl->nsplit * (D + 4) * sizeof(float) : 0;
-  if (heads * pl->row_tiles * pl->nsplit > INT32_MAX || (int64_t)nseg * max_q_len * Hq > INT32_MAX)
+  if (!kv4_grid_ok(heads * pl->row_tiles * pl->nsplit, 256 * pl->teams) ||
+      (pl->nsplit > 1 && !kv4_grid_ok((int64_t)nseg * max_q_len * Hq, 256)))
     return fail(MI355_EINVAL, "%s: too many workgroups (nseg=%d max_q_len=%d Hq=%d)", what, nseg, max_q_len, Hq);
   return 0;
 }
 
 template <class Tag, int D>
-int launch(const Kv4PrefillParams& p, const Kv4PrefillPlan& pl, int max_q_len, hipStream_t s) {
+int launch(const Kv4PrefillParams& p, const Kv4PrefillPlan& pl, hipStream_t s) {
   const dim3 grid((unsigned)((int64_t)p.row_tiles * p.nseg * p.Hkv * p.nsplit)), one(256), two(512);
   if constexpr (D < 256 && !(Tag::kCode == MI355_F32 && D == 128)) {
     if (pl.MC == 2 && pl.teams == 1) hipLaunchKernelGGL((kv4_prefill_kernel<Tag, D, 2, 1>), grid, one, 0, s, p);
@@ -485,19 +487,19 @@ int launch(const Kv4PrefillParams& p, const Kv4PrefillPlan& pl, int max_q_len, h
   if (pl.MC == 1 && pl.teams == 2) hipLaunchKernelGGL((kv4_prefill_kernel<Tag, D, 1, 2>), grid, two, 0, s, p);
   if (int rc = check_launch("kv4_prefill_kernel")) return rc;
   if (p.nsplit > 1) {
-    if (p.nsplit <= kKv4WalkedSplits) launch_merge<Tag, D, kv4_split_lanes<D>(true)>(p, max_q_len, s);
-    else launch_merge<Tag, D, kv4_split_lanes<D>(false)>(p, max_q_len, s);
+    if (p.nsplit <= kKv4WalkedSplits) launch_merge<Tag, D, kv4_split_lanes<D>(true)>(p, s);
+    else launch_merge<Tag, D, kv4_split_lanes<D>(false)>(p, s);
     return check_launch("kv4_prefill_merge_kernel");
   }
   return 0;
 }
 template <class Tag>
-int launch(const Kv4PrefillParams& p, const Kv4PrefillPlan& pl, int D, int max_q_len, hipStream_t s) {
+int launch(const Kv4PrefillParams& p, const Kv4PrefillPlan& pl, int D, hipStream_t s) {
   switch (D) {
-    case 32: return launch<Tag, 32>(p, pl, max_q_len, s);
-    case 64: return launch<Tag, 64>(p, pl, max_q_len, s);
-    case 128: return launch<Tag, 128>(p, pl, max_q_len, s);
-    default: return launch<Tag, 256>(p, pl, max_q_len, s);
+    case 32: return launch<Tag, 32>(p, pl, s);
+    case 64: return launch<Tag, 64>(p, pl, s);
+    case 128: return launch<Tag, 128>(p, pl, s);
+    default: return launch<Tag, 256>(p, pl, s);
   }
 }
 
@@ -510,7 +512,7 @@ extern "C" size_t mi355_paged_prefill_kv4_workspace_bytes(int32_t nseg, int32_t 
                                                           int32_t Hq, int32_t Hkv, int32_t D, int32_t max_context,
                                                           int32_t dtype) {
   Kv4PrefillPlan pl;
-  if (nseg == 0 || max_q_len == 0) return 0;
+  if (nseg == 0 || max_q_len == 0 || total_rows == 0) return 0;
   if (make_plan("paged_prefill_kv4", nseg, total_rows, max_q_len, Hq, Hkv, D, max_context, dtype, &pl)) return 0;
   return pl.ws_bytes;
 }
@@ -522,7 +524,7 @@ extern "C" int mi355_paged_prefill_kv4(void* out, const void* q, int64_t q_strid
                                        int32_t block_size, int32_t max_blocks, int32_t num_blocks,
                                        int32_t max_context, int64_t stride_block, int64_t stride_head, float scale,
                                        int32_t dtype, void* workspace, size_t workspace_bytes, void* stream) {
-  if (nseg == 0 || max_q_len == 0) return 0;
+  if (nseg == 0 || max_q_len == 0 || total_rows == 0) return 0;
   if (!out || !q || !block_tables || !seg_q_start || !seg_len || !seg_pos0)
     return fail(MI355_EINVAL, "paged_prefill_kv4: null pointer argument");
   if (int rc = kv4_check_cache("paged_prefill_kv4", k_cache, v_cache, Hkv, D, block_size, num_blocks, stride_block, stride_head))
@@ -548,6 +550,7 @@ extern "C" int mi355_paged_prefill_kv4(void* out, const void* q, int64_t q_strid
   p.q_stride = q_stride_tok;
   p.nseg = nseg;
   p.total_rows = total_rows;
+  p.max_q_len = std::min(max_q_len, total_rows);
   p.Hq = Hq;
   p.Hkv = Hkv;
   p.G = Hq / Hkv;
@@ -562,8 +565,8 @@ extern "C" int mi355_paged_prefill_kv4(void* out, const void* q, int64_t q_strid
   p.raise = kKv4Raise / p.scale2;
   hipStream_t s = static_cast<hipStream_t>(stream);
   switch (dtype) {
-    case MI355_F32: return launch<F32>(p, pl, D, max_q_len, s);
-    case MI355_BF16: return launch<BF16>(p, pl, D, max_q_len, s);
-    default: return launch<F16>(p, pl, D, max_q_len, s);
+    case MI355_F32: return launch<F32>(p, pl, D, s);
+    case MI355_BF16: return launch<BF16>(p, pl, D, s);
+    default: return launch<F16>(p, pl, D, s);
   }
 }

@@ -372,6 +372,11 @@ int launch_read(ReadParams4& p, int D, hipStream_t s) {
   return two ? launch_read<Tag, 2>(p, D, s) : launch_read<Tag, 1>(p, D, s);
 }
 
+// Whether `out` (contiguous) and the span of rows from x share bytes.
+bool overlaps(const char* out, int64_t out_bytes, const char* x, int64_t stride, int64_t width, int T) {
+  return out < x + ((int64_t)(T - 1) * stride + width) && x < out + out_bytes;
+}
+
 // Query (and, with slots, key / value) rows through kv4_append_kernel.
 int append_impl(const char* what, AppendParams4& p, int T, int D, int rotary_dim, int interleaved, int dtype,
                 hipStream_t s) {
@@ -388,11 +393,16 @@ int append_impl(const char* what, AppendParams4& p, int T, int D, int rotary_dim
   if (p.slots && (p.k_stride_tok % epl || p.v_stride_tok % epl || p.k_stride_tok < (int64_t)p.Hkv * D ||
                   p.v_stride_tok < (int64_t)p.Hkv * D || (((uintptr_t)p.k | (uintptr_t)p.v) & 15)))
     return fail(MI355_EINVAL, "%s: key / value rows must be 16-byte aligned and a token's heads packed", what);
+  const int64_t eb = dtype == MI355_F32 ? 4 : 2, out_bytes = (int64_t)T * p.Hq * D * eb;
+  if (T > 0 && (overlaps(p.q_out, out_bytes, p.q, p.q_stride_tok * eb, p.Hq * D * eb, T) ||
+                (p.slots && (overlaps(p.q_out, out_bytes, p.k, p.k_stride_tok * eb, p.Hkv * D * eb, T) ||
+                             overlaps(p.q_out, out_bytes, p.v, p.v_stride_tok * eb, p.Hkv * D * eb, T)))))
+    return fail(MI355_EINVAL, "%s: the output overlaps the rows it is made from", what);
   if (rotary_dim == 0) p.cos = p.sin = nullptr;
   p.R = rotary_dim;
   p.heads = p.slots ? p.Hq + 2 * p.Hkv : p.Hq;
   p.T = T;
-  if (ceil_div64((int64_t)T * p.heads, 256 / (D / 8)) > INT32_MAX) return fail(MI355_EINVAL, "%s: too many rows (T=%d)", what, T);
+  if (!kv4_grid_ok(ceil_div64((int64_t)T * p.heads, 256 / (D / 8)), 256)) return fail(MI355_EINVAL, "%s: too many rows (T=%d)", what, T);
   switch (dtype) {
     case MI355_F32: return launch_append<F32>(p, D, interleaved != 0, s);
     case MI355_BF16: return launch_append<BF16>(p, D, interleaved != 0, s);
@@ -411,7 +421,7 @@ extern "C" int mi355_rope_angles(float* cos_out, float* sin_out, const int64_t* 
   if (!cos_out || !sin_out || !positions || !inv_freq) return fail(MI355_EINVAL, "rope_angles: null pointer");
   if (T < 0 || half_dim <= 0) return fail(MI355_EINVAL, "rope_angles: bad shape (T=%d half_dim=%d)", T, half_dim);
   const int64_t total = (int64_t)T * half_dim;
-  if (ceil_div64(total, 256) > INT32_MAX) return fail(MI355_EINVAL, "rope_angles: too many rows (T=%d)", T);
+  if (!kv4_grid_ok(ceil_div64(total, 256), 256)) return fail(MI355_EINVAL, "rope_angles: too many rows (T=%d)", T);
   hipLaunchKernelGGL(rope_angles_kernel, dim3((unsigned)ceil_div64(total, 256)), dim3(256), 0,
                      static_cast<hipStream_t>(stream), cos_out, sin_out, positions, inv_freq, factor, total, half_dim);
   return check_launch("rope_angles_kernel");
@@ -481,7 +491,7 @@ extern "C" int mi355_kv4_read_slots(void* k_out, void* v_out, const void* k_cach
   p.num_slots = (int64_t)num_blocks * block_size;
   p.Hkv = Hkv;
   p.bs_shift = ilog2_exact(block_size);
-  if (ceil_div64((int64_t)T * 2 * Hkv, 256 / (D / 8)) > INT32_MAX) return fail(MI355_EINVAL, "kv4_read_slots: too many rows (T=%d)", T);
+  if (!kv4_grid_ok(ceil_div64((int64_t)T * 2 * Hkv, 256 / (D / 8)), 256)) return fail(MI355_EINVAL, "kv4_read_slots: too many rows (T=%d)", T);
   hipStream_t s = static_cast<hipStream_t>(stream);
   switch (dtype) {
     case MI355_F32: return launch_read<F32>(p, D, s);
