@@ -649,6 +649,49 @@ def test_captured_and_replayed(ops, device, decode):
     assert torch.equal(other, _step(ops, fresh[0]))
 
 
+@pytest.mark.parametrize('decode', [True, False])
+def test_two_streams_at_once(ops, device, decode):
+    """Split launches of two sizes in flight together: each stream has partial sums of its own."""
+    rng = np.random.default_rng(31)
+    steps = [_sequence_state(ops, rng, torch.bfloat16, lens, new, 8, 4, 64, 16, decode)[0]
+             for lens, new in (([6000, 300], [1, 1] if decode else [3, 40]), ([4000, 5000, 17], [1, 1, 1] if decode else [20, 9, 17]))]
+    want = [_step(ops, s) for s in steps]
+    streams = [torch.cuda.Stream() for _ in steps]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for side, s, outs in zip(streams, steps, got):
+            with torch.cuda.stream(side):
+                outs.append(_step(ops, s))
+    torch.cuda.synchronize()
+    for outs, w in zip(got, want):
+        assert all(torch.equal(o, w) for o in outs)
+
+
+def test_blocks_far_into_a_large_pool(ops, device):
+    """Records beyond 2^32 bytes: the same step over a pool of 6 GiB per tensor and over a small one."""
+    rng = np.random.default_rng(32)
+    Hkv, D, BS = 4, 128, 16
+    lens, new = [500, 40], [70, 40]
+    s = _sequence_state(ops, rng, torch.bfloat16, lens, new, 8, Hkv, D, BS, False)[0]
+    far = dict(s)
+    shape = ops.kv4_cache_shape((6 << 30) // (Hkv * 17 * D // 2), Hkv, BS, D)
+    move = shape[0] - s['kc'].shape[0]
+    for name in ('kc', 'vc'):
+        far[name] = torch.empty(shape, dtype=torch.uint8, device=device)
+        far[name][move:] = s[name]
+    far['tables'], far['slots'] = s['tables'] + move, s['slots'] + move * BS
+    assert move * Hkv * 17 * D // 2 > 1 << 32
+    assert torch.equal(_step(ops, far), _step(ops, s))
+    assert torch.equal(far['kc'][move:], s['kc']) and torch.equal(far['vc'][move:], s['vc'])
+    ctx = torch.tensor(lens, dtype=torch.int32, device=device)
+    q = s['q'][:2].contiguous()
+    assert torch.equal(ops.paged_decode_kv4(q, far['kc'], far['vc'], far['tables'], ctx, 500),
+                       ops.paged_decode_kv4(q, s['kc'], s['vc'], s['tables'], ctx, 500))
+    for a, b in zip(ops.kv4_read_slots(far['kc'], far['vc'], far['slots']), ops.kv4_read_slots(s['kc'], s['vc'], s['slots'])):
+        assert torch.equal(a, b)
+
+
 # ------------------------------------------------------------------ the engine over a 4-bit cache
 @pytest.mark.parametrize('rotary', [None, dict(dim=32, interleaved=True, scaling={'kind': 'yarn', 'factor': 4, 'original': 64})])
 def test_engine_layer_steps(ops, device, rotary):
