@@ -459,6 +459,12 @@ WIDE = [
     (8, 8, 128, 16, [512, 100, 512, 512, 512], [0, 0, 0, 0, 0]),
     (4, 2, 256, 16, [200, 100], [700, 0]),
     (8, 8, 32, 16, [512, 510, 512, 512, 333, 512], [1300, 0, 1290, 1300, 1000, 1777]),
+    (8, 8, 64, 16, [400] * 15 + [33], [0] * 16),
+    (8, 8, 32, 16, [512] * 8, [300] * 8),
+    (8, 8, 64, 32, [512, 511] * 4, [300] * 8),
+    (8, 8, 32, 16, [2048] * 8, [0] * 8),
+    (8, 8, 256, 16, [256, 250, 256] * 3, [0] * 9),
+    (8, 8, 128, 16, [256, 250, 256] * 3, [0] * 9),
 ]
 
 
@@ -521,6 +527,36 @@ def test_chunk_queries_before_the_first_position_see_nothing(ops, device, ctx):
         pick = [j - 14 for j in got]
         _near(out[got], want[pick], bound[pick])
         assert bool((out[20 + rows:] == 7.0).all())
+
+
+@pytest.mark.parametrize('Hq,Hkv,D,n,seqs,pos0', [
+    (8, 8, 64, 90, 2, 0), (8, 8, 64, 512, 8, 300), (8, 8, 64, 400, 16, 0), (8, 8, 64, 2048, 8, 0), (32, 8, 128, 300, 1, 40),
+    (32, 8, 128, 256, 3, 1600), (8, 8, 128, 250, 9, 0), (32, 8, 128, 300, 4, 0), (8, 8, 256, 250, 9, 0), (8, 2, 256, 60, 1, 9),
+    (8, 8, 32, 512, 8, 300), (8, 8, 32, 400, 16, 0), (8, 8, 32, 2048, 8, 0), (4, 2, 32, 50, 1, 5)])
+def test_chunk_nan_pattern_in_every_form(ops, device, Hq, Hkv, D, n, seqs, pos0):
+    """NaN value blocks within a chunk, one behind it and a NaN key: the queries that see them and no others, in the dims
+    of their blocks, whichever way the kernel cuts the rows up."""
+    rng = np.random.default_rng(n + D)
+    G, total, BS = Hq // Hkv, n + pos0, 16
+    blocks = -(-total // BS) + 1
+    tables = rng.permutation(seqs * blocks).reshape(seqs, blocks).astype(np.int32)
+    shape = ops.kv4_cache_shape(seqs * blocks, Hkv, BS, D)
+    kc = rng.integers(0, 256, shape).astype(np.uint8)
+    vc = rng.integers(0, 256, shape).astype(np.uint8)
+    kc[..., 8 * D:], vc[..., 8 * D:] = 127, 127
+    expect = np.zeros((seqs, n, Hq, D), dtype=bool)
+    for at, head, b in ((pos0 + n // 2, Hkv - 1, 0), (pos0 + n // 2 + 1, 0, D // 32 - 1), (pos0 + n - 1, 1, D // 32 // 2), (total, 0, 0)):
+        vc[tables[-1, at // BS], head, 0, orc.scale_place(D, at % 16, b, True)] = 255
+        if at < total:
+            expect[-1, at - pos0:, head * G:(head + 1) * G, 32 * b:32 * b + 32] = True
+    at = pos0 + n // 3
+    kc[tables[0, at // BS], Hkv // 2, 0, orc.scale_place(D, at % 16, 0, False)] = 255
+    expect[0, at - pos0:, Hkv // 2 * G:(Hkv // 2 + 1) * G] = True
+    q = torch.from_numpy(rng.standard_normal((seqs * n, Hq, D))).cuda().to(torch.bfloat16)
+    meta = torch.tensor([[i * n for i in range(seqs)], [n] * seqs, [pos0] * seqs], dtype=torch.int32, device=device)
+    out = ops.paged_prefill_kv4(q, torch.from_numpy(kc).cuda(), torch.from_numpy(vc).cuda(), torch.from_numpy(tables).cuda(),
+                                meta[0], meta[1], meta[2], n, total)
+    np.testing.assert_array_equal(torch.isnan(out).cpu().numpy().reshape(expect.shape), expect)
 
 
 def test_outputs_that_overlap_their_rows_are_refused(ops, device):

@@ -1,17 +1,19 @@
 // Attention of several new query tokens per sequence over the 4-bit KV cache (their K / V rows are in
 // it already): query j of a segment attends to positions 0 .. pos0 + j.
 //
-// The query rows of a (segment, kv head) are its (token, query head of the group) pairs.  A workgroup
-// of four waves owns 4 x MC tiles of 16 of them (a tile is the 16 columns of a score tile) and walks the
-// context in stages of SUB steps of 32 tokens.  Per stage each wave converts a quarter of the K and V
-// codes to bf16 (exact) and leaves them in LDS as the operands of the matrix instruction; every wave
-// reads them all back, once per MC tiles.  Conversion is what the format costs beside attention in
-// bf16: 130 vector instructions per 32 tokens of 128 dims, as many as two tiles' softmax, so it is done
-// once per workgroup and not once per wave.  Codes travel from memory one stage ahead in registers,
-// operands one stage ahead in LDS (two buffers, one barrier per stage).
-// A stage is a chain -- scores, softmax, values, barrier -- that eight waves of a CU overlap and four do not.
-// Where there are few workgroups each gets a second team of four waves for the same rows; the teams take
-// the stages in turn and are joined through LDS.
+// The query rows of a (segment, kv head) are its (token, query head of the group) pairs; they are the
+// columns of a score tile S^T = K Q^T, whose weights go back into the matrix unit in the registers they
+// were born in (see kv4.h).  Conversion of codes to bf16 (exact) is what the format costs beside attention
+// in bf16 -- 130 vector instructions per 32 tokens of 128 dims, as many as the softmax of 64 columns -- and
+// the two kernels differ in who does it:
+//   kv4_prefill_kernel  many rows.  A workgroup of four waves owns four tiles of 16 or 32 columns and walks
+//       the context in stages of SUB steps of 32 tokens.  Per stage each wave converts a quarter of the K
+//       and V codes and leaves them in LDS as the operands of the matrix instruction; every wave reads them
+//       all back.  Codes travel from memory one stage ahead in registers, operands one stage ahead in LDS
+//       (two buffers, one barrier per stage).  LDS is its bound: 20 KiB per step of 32 columns, 160 of the
+//       roughly 270 cycles that a CU takes for it at 128 dims.
+//   kv4_rows_kernel     few rows.  A workgroup owns 32 or 64 columns, its waves take the steps in turn and
+//       convert their own in registers: no barrier, a quarter of the walk, more conversion per row.
 #include <algorithm>
 #include <cmath>
 
@@ -64,78 +66,113 @@ __device__ __forceinline__ void lds_barrier() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-template <class Tag, int D, int MC, int TEAMS>
-__global__ void __launch_bounds__(256 * TEAMS, 2) kv4_prefill_kernel(const Kv4PrefillParams p) {
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+// How a wave lays out its tile of COLS query rows (a lane's column is lane % COLS): with 16 columns the 16x16x32 matrix
+// instruction, scores and values of 16 rows at a time; with 32 the 32x32x16 one.
+//   scores   32 tokens of a step in rows; a lane holds TOK of them.  With 32 columns row R is token (R & 7) + 8 (R >> 4) of
+//            tile (R >> 3) & 1, which makes the lane's tokens the ones that one conversion of a value block yields.
+//   values   32 dims of a block in rows: two tiles of even and odd dims, or one tile with the odd dims behind the even ones
+template <int COLS>
+struct Layout;
+template <>
+struct Layout<16> {
+  static constexpr int kTok = 8, kQ = 1, kHalf = 1;   // tokens per lane; contraction steps of a value product; chunks of 8 dims per block
+  typedef f32x4 scores_t[2];
+  typedef f32x4 sums_t[2];
+  static __device__ __forceinline__ int token(int g, int e) { return (e >> 2) * kKv4Tile + 4 * g + (e & 3); }
+  // where the frag of tile t, token c, dims (g, s) goes (units of operands of 64 lanes, and the lane)
+  static __device__ __forceinline__ int k_slot(int lane, int t, int KS) { return t * KS * 64 + lane; }
+  static constexpr int kStepS = 64;   // from s to s + 1
+  static __device__ __forceinline__ int v_even(int lane) { return lane; }
+  static __device__ __forceinline__ int v_odd(int lane) { return 64 + lane; }
+  static __device__ __forceinline__ int q_dim(int D, int g, int f) { return g * (D / 4) + 8 * f; }
+  static __device__ __forceinline__ float score(const scores_t& S, int e) { return S[e >> 2][e & 3]; }
+  static __device__ __forceinline__ int chunk(int g, int) { return 8 * g; }
+  static __device__ __forceinline__ float even(const sums_t& a, int, int i) { return a[0][i]; }
+  static __device__ __forceinline__ float odd(const sums_t& a, int, int i) { return a[1][i]; }
+};
+template <>
+struct Layout<32> {
+  static constexpr int kTok = 16, kQ = 2, kHalf = 2;
+  typedef f32x16 scores_t[1];
+  typedef f32x16 sums_t[1];
+  static __device__ __forceinline__ int token(int g, int e) { return ((e >> 2) & 1) * kKv4Tile + (e >> 3) * 8 + 4 * g + (e & 3); }
+  static __device__ __forceinline__ int k_slot(int lane, int t, int) {
+    const int g = lane >> 4, c = lane & 15;
+    return (g >> 1) * 64 + (g & 1) * 32 + (c >> 3) * 16 + t * 8 + (c & 7);
+  }
+  static constexpr int kStepS = 128;
+  static __device__ __forceinline__ int v_even(int lane) { return (lane >> 5) * 64 + ((lane >> 4) & 1) * 32 + (lane & 15); }
+  static __device__ __forceinline__ int v_odd(int lane) { return v_even(lane) + 16; }
+  static __device__ __forceinline__ int q_dim(int D, int g, int f) { return (2 * (f & 1) + g) * (D / 4) + 8 * (f >> 1); }
+  static __device__ __forceinline__ float score(const scores_t& S, int e) { return S[0][e]; }
+  static __device__ __forceinline__ int chunk(int g, int h) { return 16 * h + 8 * g; }
+  static __device__ __forceinline__ float even(const sums_t& a, int h, int i) { return a[0][4 * h + i]; }
+  static __device__ __forceinline__ float odd(const sums_t& a, int h, int i) { return a[0][8 + 4 * h + i]; }
+};
+__device__ __forceinline__ f32x16 mfma32_bf16(bf16x8_t a, bf16x8_t b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+template <class Tag, int D, int COLS>
+__global__ void __launch_bounds__(256, 2) kv4_prefill_kernel(const Kv4PrefillParams p) {
   typedef Stage<D> St;
+  typedef Layout<COLS> Lay;
   constexpr int NP = Kv4Pieces<Tag>::n, KS = D / 32, EB = Tag::kBytes, SUB = St::SUB, NB = St::NB, KT = St::KT, KF = St::KF;
   constexpr int KA = KS < 4 ? KS : 4, VA = KS < 2 ? KS : 2;   // operands read ahead of their use
-  struct Shared {   // one team's
-    bf16x8_t k[2][SUB][2][KS][64], v[2][SUB][KS][2][64];
-    uint32_t nan[2][SUB][KS];   // tokens of a step whose V block was NaN (masked stages only)
-  };
-  constexpr int kRow = D + 4;   // a column's sums, maximum and sum of weights on their way from team 1 to team 0
-  constexpr int kShared = TEAMS * (int)sizeof(Shared), kJoin = TEAMS > 1 ? kWaves * MC * 16 * kRow * 4 : 0;
-  __shared__ __attribute__((aligned(16))) char s_mem[kShared > kJoin ? kShared : kJoin];
-  const int lane = threadIdx.x & 63, wg_wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int team = TEAMS > 1 ? wg_wave / kWaves : 0, wave = TEAMS > 1 ? wg_wave % kWaves : wg_wave;
-  Shared& sh = reinterpret_cast<Shared*>(s_mem)[team];
-  const int g = lane >> 4, col = lane & 15;
+  constexpr int TOK = Lay::kTok, NQ = Lay::kQ, QF = KS * NQ;
+  __shared__ bf16x8_t s_k[2][SUB][2 * KS * 64], s_v[2][SUB][KS][2 * 64];
+  __shared__ uint32_t s_nan[2][SUB][KS];   // tokens of a step whose V block was NaN (masked stages only)
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane / COLS, col = lane % COLS;
   int idx = blockIdx.x;
-  const int sp = idx % p.nsplit;
-  idx /= p.nsplit;
   const int h = idx % p.Hkv;   // (kv heads on neighbouring XCDs: the row tiles of one head share an L2 where Hkv is a multiple of 8)
   idx /= p.Hkv;
   const int seg = idx % p.nseg;
   const int rt = p.row_tiles - 1 - idx / p.nseg;   // the longest contexts first
   const int q0 = p.seg_q0[seg], pos0 = p.seg_pos0[seg], len = segment_rows(p, q0, p.seg_len[seg]);
-  const int rows = len * p.G, wg_row0 = rt * kWaves * MC * 16;
+  const int rows = len * p.G, wg_row0 = rt * kWaves * COLS;
   if (wg_row0 >= rows) return;
-  const int row0 = wg_row0 + wave * MC * 16;
+  const int row0 = wg_row0 + wave * COLS;
 
-  int lim[MC];       // last position the column attends to; -1: none
-  int64_t orow[MC];  // its row of out (and of q), -1: none
-  bf16x8_t qf[MC][KS][NP];
-#pragma unroll
-  for (int mc = 0; mc < MC; ++mc) {
-    const int r = row0 + mc * 16 + col, rr = min(r, rows - 1);
+  int lim;        // last position the column attends to; -1: none
+  int64_t orow;   // its row of out (and of q), -1: none
+  bf16x8_t qf[QF][NP];
+  {
+    const int r = row0 + col, rr = min(r, rows - 1);
     const int tok = rr / p.G, hq = h * p.G + rr % p.G;
-    lim[mc] = min(pos0 + tok, p.max_ctx - 1);
-    orow[mc] = r < rows ? (int64_t)(q0 + tok) * p.Hq + hq : -1;
-    const char* src = p.q + ((int64_t)(q0 + tok) * p.q_stride + (int64_t)hq * D + g * (D / 4)) * EB;
+    lim = min(pos0 + tok, p.max_ctx - 1);
+    orow = r < rows ? (int64_t)(q0 + tok) * p.Hq + hq : -1;
+    const char* src = p.q + ((int64_t)(q0 + tok) * p.q_stride + (int64_t)hq * D) * EB;
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
+    for (int f = 0; f < QF; ++f) {
       float x[8];
-      load8<Tag>(src + s * 8 * EB, x);
+      load8<Tag>(src + Lay::q_dim(D, g, f) * EB, x);
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] = p.flip ? -x[e] : x[e];
-      bf16_pieces<NP>(x, qf[mc][s]);
+      bf16_pieces<NP>(x, qf[f]);
     }
   }
   auto limit = [&](int r) { return min(pos0 + min(r, rows - 1) / p.G, p.max_ctx - 1); };
   const int wave_first = limit(row0);
-  const int wg_first = limit(wg_row0), wg_end = limit(wg_row0 + kWaves * MC * 16 - 1);
-  const int lo = sp * p.tps, wg_last = min(wg_end, lo + p.tps - 1);   // this workgroup's tokens: lo .. wg_last
-  const int wave_last = row0 < rows ? min(limit(row0 + MC * 16 - 1), wg_last) : -1;
-  if (lo > wg_last && sp > 0) return;                                 // (the rows' own limits tell which splits are empty)
+  const int wg_first = limit(wg_row0), wg_last = limit(wg_row0 + kWaves * COLS - 1);
+  const int wave_last = row0 < rows ? limit(row0 + COLS - 1) : -1;
 
-  f32x4 acc[MC][KS][2], sum[MC];
-  float m[MC], m2[MC];   // running maximum of the raw scores, and times the scale
+  typename Lay::sums_t acc[KS];
+  float m = kKv4Floor, m2 = kKv4Floor;   // running maximum of the raw scores, and times the scale
+  float sum = 0.f;                       // of the lane's weights
 #pragma unroll
-  for (int mc = 0; mc < MC; ++mc) {
-    m[mc] = m2[mc] = kKv4Floor;
-    sum[mc] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < KS; ++s)
 #pragma unroll
-    for (int s = 0; s < KS; ++s) acc[mc][s][0] = acc[mc][s][1] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
-  bf16x8_t ones;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) ones[e] = (__bf16)1.f;
+    for (auto& a : acc[s]) a = 0.f;
 
   // ---- this wave's part of a stage
   const int32_t* table = p.bt + (int64_t)seg * p.max_blocks;
   const int last_tile = max(wg_last, 0) / kKv4Tile;
   const int vstep = St::step(wave), vblk = St::v_block(wave), kstep = vstep, ktile = St::k_tile(wave),
             kfirst = St::k_first(wave);
+  const int k_slot = Lay::k_slot(lane, St::k_tile(wave), KS), v_even = Lay::v_even(lane), v_odd = Lay::v_odd(lane);
   uint32_t o_k, o_ks, o_v, o_vs, turn;   // the lane's places in a record
   {
     Kv4Lane<D> at(lane);
@@ -201,197 +238,452 @@ __global__ void __launch_bounds__(256 * TEAMS, 2) kv4_prefill_kernel(const Kv4Pr
       }
       if (lane == 0) {
 #pragma unroll
-        for (int b = 0; b < NB; ++b) sh.nan[buf][vstep][vblk + b] = nan[b];
+        for (int b = 0; b < NB; ++b) s_nan[buf][vstep][vblk + b] = nan[b];
       }
     }
 #pragma unroll
     for (int i = 0; i < KT; ++i) {
       const float sc = u2f(__builtin_amdgcn_alignbit(rks[i], rks[i], turn));
+      const int slot = KT == 2 ? Lay::k_slot(lane, i, KS) : k_slot;
 #pragma unroll
-      for (int f = 0; f < KF; ++f) sh.k[buf][kstep][KT == 2 ? i : ktile][kfirst + f][lane] = kv4_k_frag(rk[i][f], sc);
+      for (int f = 0; f < KF; ++f) s_k[buf][kstep][slot + (kfirst + f) * Lay::kStepS] = kv4_k_frag(rk[i][f], sc);
     }
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       bf16x8_t ev, od;
       kv4_v_frags(rv[0][b], rv[1][b], rvs[0][b], rvs[1][b], ev, od);
-      sh.v[buf][vstep][vblk + b][0][lane] = ev;
-      sh.v[buf][vstep][vblk + b][1][lane] = od;
+      s_v[buf][vstep][vblk + b][v_even] = ev;
+      s_v[buf][vstep][vblk + b][v_odd] = od;
     }
   };
 
-  if (wg_last >= lo) {
-    constexpr int kStride = TEAMS * St::kTokens;   // the teams take stages in turn
-    const int first = lo + team * St::kTokens;
-    place(first);
+  if (wg_last >= 0) {
+    place(0);
     fetch();
-    place(first + kStride);
-    convert(first, 0);
+    place(St::kTokens);
+    convert(0, 0);
     fetch();
-    place(first + 2 * kStride);
+    place(2 * St::kTokens);
     int buf = 0;
-    for (int t0 = first; t0 - team * St::kTokens <= wg_last; t0 += kStride, buf ^= 1) {
+    for (int t0 = 0; t0 <= wg_last; t0 += St::kTokens, buf ^= 1) {
       lds_barrier();
-      convert(t0 + kStride, buf ^ 1);   // (behind the last stage: the last tile again, read by nobody)
+      convert(t0 + St::kTokens, buf ^ 1);   // (behind the last stage: the last tile again, read by nobody)
       fetch();
-      place(min(t0 + 3 * kStride, wg_last));
+      place(min(t0 + 3 * St::kTokens, wg_last));
       const bool wg_masked = t0 + St::kTokens - 1 > wg_first;
 #pragma unroll
       for (int sub = 0; sub < SUB; ++sub) {
         const int ts = t0 + sub * kKv4Step;
         if (ts > wave_last) break;
         const bool masked = ts + kKv4Step - 1 > wave_first;
-        f32x4 S[MC][2];
+        typename Lay::scores_t S;
+#pragma unroll
+        for (auto& c : S) c = 0.f;
         bf16x8_t kf[2][KA];   // K operands, read 2 KA ahead
 #pragma unroll
-        for (int f = 0; f < 2 * KA; ++f) kf[f / KA][f % KA] = sh.k[buf][sub][f / KS][f % KS][lane];
+        for (int f = 0; f < 2 * KA; ++f) kf[f / KA][f % KA] = s_k[buf][sub][f * 64 + lane];
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int f = 0; f < 2 * KS; ++f) {
+          const bf16x8_t a = kf[f / KA % 2][f % KA];
+          if (f + 2 * KA < 2 * KS) kf[f / KA % 2][f % KA] = s_k[buf][sub][(f + 2 * KA) * 64 + lane];
 #pragma unroll
-          for (int mc = 0; mc < MC; ++mc) S[mc][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int s = 0; s < KS; ++s) {
-            const int f = i * KS + s;
-            const bf16x8_t a = kf[f / KA % 2][f % KA];
-            if (f + 2 * KA < 2 * KS) kf[f / KA % 2][f % KA] = sh.k[buf][sub][(f + 2 * KA) / KS][(f + 2 * KA) % KS][lane];
-#pragma unroll
-            for (int mc = 0; mc < MC; ++mc)
-#pragma unroll
-              for (int n = 0; n < NP; ++n) S[mc][i] = mfma_bf16(a, qf[mc][s][n], S[mc][i]);
+          for (int n = 0; n < NP; ++n) {
+            if constexpr (COLS == 16) S[f / KS] = mfma_bf16(a, qf[f % KS][n], S[f / KS]);
+            else S[0] = mfma32_bf16(a, qf[f][n], S[0]);
           }
         }
         bf16x8_t vf[VA][2];   // V operands of the first blocks, on their way during the softmax
 #pragma unroll
         for (int s = 0; s < VA; ++s) {
-          vf[s][0] = sh.v[buf][sub][s][0][lane];
-          vf[s][1] = sh.v[buf][sub][s][1][lane];
+          vf[s][0] = s_v[buf][sub][s][lane];
+          vf[s][1] = s_v[buf][sub][s][64 + lane];
         }
         __builtin_amdgcn_sched_barrier(0);
         if (wg_masked) {
+          const int seen = lim + 1 - ts;   // tokens of the step the column sees
+          const uint32_t sees = seen >= 32 ? ~0u : (seen <= 0 ? 0u : (1u << seen) - 1u);
 #pragma unroll
           for (int s = 0; s < KS; ++s) {
-            const uint32_t nan = __builtin_amdgcn_readfirstlane(sh.nan[buf][sub][s]);
-            if (nan) {
+            const uint32_t nan = __builtin_amdgcn_readfirstlane(s_nan[buf][sub][s]);
+            if (nan & sees) {
 #pragma unroll
-              for (int mc = 0; mc < MC; ++mc) {
-                const int seen = lim[mc] + 1 - ts;   // tokens of the step the column sees
-                const uint32_t sees = seen >= 32 ? ~0u : (seen <= 0 ? 0u : (1u << seen) - 1u);
-                if (nan & sees) {
-#pragma unroll
-                  for (int e = 0; e < 4; ++e) acc[mc][s][0][e] = acc[mc][s][1][e] = __builtin_nanf("");
-                }
-              }
+              for (auto& a : acc[s]) a = __builtin_nanf("");
             }
           }
         }
-        bf16x8_t pf[MC][NP];
+        float x[TOK];
 #pragma unroll
-        for (int mc = 0; mc < MC; ++mc) {
-          float x[8];
+        for (int e = 0; e < TOK; ++e) x[e] = Lay::score(S, e);
+        if (masked) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = S[mc][e >> 2][e & 3];
-          if (masked) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (ts + (e >> 2) * kKv4Tile + 4 * g + (e & 3) > lim[mc]) x[e] = -INFINITY;
-          }
-          float top = fmaxf(fmaxf(x[0], x[1]), x[2]);
-          top = fmaxf(fmaxf(top, x[3]), x[4]);
-          top = fmaxf(fmaxf(top, x[5]), fmaxf(x[6], x[7]));
-          if (__ballot(top > m[mc] + p.raise)) {
-            top = fmaxf(top, __shfl_xor(top, 16));
-            top = fmaxf(top, __shfl_xor(top, 32));
-            const float mn = fmaxf(m[mc], top), f = fast_exp2((m[mc] - mn) * p.scale2);
-            m[mc] = mn;
-            m2[mc] = fmaxf(mn * p.scale2, kKv4Floor);
-            sum[mc] *= f;
-#pragma unroll
-            for (int s = 0; s < KS; ++s) {
-              acc[mc][s][0] *= f;
-              acc[mc][s][1] *= f;
-            }
-          }
-#pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = fast_exp2(__builtin_fmaf(x[e], p.scale2, -m2[mc]));
-          bf16_pieces<NP>(x, pf[mc]);
-#pragma unroll
-          for (int n = 0; n < NP; ++n) sum[mc] = mfma_bf16(ones, pf[mc][n], sum[mc]);   // every row: the column's sum of weights
+          for (int e = 0; e < TOK; ++e)
+            if (ts + Lay::token(g, e) > lim) x[e] = -INFINITY;
         }
+        float top = x[0];
+#pragma unroll
+        for (int e = 1; e + 1 < TOK; e += 2) top = fmaxf(fmaxf(top, x[e]), x[e + 1]);
+        top = fmaxf(top, x[TOK - 1]);
+        if (__ballot(top > m + p.raise)) {
+          if constexpr (COLS == 16) top = fmaxf(top, __shfl_xor(top, 16));
+          top = fmaxf(top, __shfl_xor(top, 32));
+          const float mn = fmaxf(m, top), f = fast_exp2((m - mn) * p.scale2);
+          m = mn;
+          m2 = fmaxf(mn * p.scale2, kKv4Floor);
+          sum *= f;
+#pragma unroll
+          for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (auto& a : acc[s]) a *= f;
+        }
+        bf16x8_t pf[NQ][NP];
+#pragma unroll
+        for (int e = 0; e < TOK; ++e) {
+          x[e] = fast_exp2(__builtin_fmaf(x[e], p.scale2, -m2));
+          sum += x[e];
+        }
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) bf16_pieces<NP>(*reinterpret_cast<const float(*)[8]>(&x[8 * n]), pf[n]);
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
-          const bf16x8_t ev = vf[s % VA][0], od = vf[s % VA][1];
+          const bf16x8_t a0 = vf[s % VA][0], a1 = vf[s % VA][1];
           if (s + VA < KS) {
-            vf[s % VA][0] = sh.v[buf][sub][s + VA][0][lane];
-            vf[s % VA][1] = sh.v[buf][sub][s + VA][1][lane];
+            vf[s % VA][0] = s_v[buf][sub][s + VA][lane];
+            vf[s % VA][1] = s_v[buf][sub][s + VA][64 + lane];
           }
 #pragma unroll
-          for (int mc = 0; mc < MC; ++mc)
-#pragma unroll
-            for (int n = 0; n < NP; ++n) {
-              acc[mc][s][0] = mfma_bf16(ev, pf[mc][n], acc[mc][s][0]);
-              acc[mc][s][1] = mfma_bf16(od, pf[mc][n], acc[mc][s][1]);
+          for (int n = 0; n < NP; ++n) {
+            if constexpr (COLS == 16) {
+              acc[s][0] = mfma_bf16(a0, pf[0][n], acc[s][0]);
+              acc[s][1] = mfma_bf16(a1, pf[0][n], acc[s][1]);
+            } else {
+              acc[s][0] = mfma32_bf16(a0, pf[0][n], acc[s][0]);
+              acc[s][0] = mfma32_bf16(a1, pf[1][n], acc[s][0]);
             }
+          }
         }
       }
     }
   }
 
-  if constexpr (TEAMS > 1) {
-    float* const join = reinterpret_cast<float*>(s_mem) + (wave * MC * 16 + col) * kRow;
-    __syncthreads();   // (nobody reads operands any more)
-    if (team == 1) {
+  if constexpr (COLS == 16) sum += __shfl_xor(sum, 16);
+  sum += __shfl_xor(sum, 32);
+  if (orow < 0) return;
+  const float inv = lim >= 0 ? 1.f / sum : 0.f;   // a query before position 0 sees nothing: zeros
 #pragma unroll
-      for (int mc = 0; mc < MC; ++mc) {
-        float* const row = join + mc * 16 * kRow;
+  for (int s = 0; s < KS; ++s)
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          *reinterpret_cast<f32x4*>(row + 32 * s + 8 * g) = acc[mc][s][0];
-          *reinterpret_cast<f32x4*>(row + 32 * s + 8 * g + 4) = acc[mc][s][1];
-        }
-        if (g == 0) row[D] = m2[mc], row[D + 1] = sum[mc][0];
+    for (int c = 0; c < Lay::kHalf; ++c) {
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[2 * i] = lim >= 0 ? Lay::even(acc[s], c, i) * inv : 0.f;
+        x[2 * i + 1] = lim >= 0 ? Lay::odd(acc[s], c, i) * inv : 0.f;
       }
+      store8<Tag>(p.out + (orow * D + 32 * s + Lay::chunk(g, c)) * EB, x);
     }
-    __syncthreads();
-    if (team == 1) return;
+}
+
+// A workgroup of CT tiles of 32 query rows; its four waves take the steps of the context in turn, so that a walk is a quarter
+// as long.  A wave converts its own steps in registers, as decode does, in the lanes where the matrix instruction wants them:
+//   K  lane (g, R) holds token (R & 7) + 8 (R >> 4) of tile (R >> 3) & 1, dims of groups g and 2 + g
+//   V  lane (g, half, c) holds dims 2 c, 2 c + 1 of a block of its half of the blocks, tokens of groups g and 2 + g; the even
+//      dims of two blocks are the 32 rows of one product, the odd dims of another (head_dim 32: both of the only block)
+// The queries wait in LDS, where the waves' sums meet at the end.
+template <class Tag, int D, int CT>
+__global__ void __launch_bounds__(256, 2) kv4_rows_kernel(const Kv4PrefillParams p) {
+  constexpr int NP = Kv4Pieces<Tag>::n, KS = D / 32, EB = Tag::kBytes, QF = 2 * KS, W = kWaves;
+  constexpr int QD = QF < 4 ? QF : NP == 1 && D < 256 && CT == 1 ? 4 : 2;   // query operands read ahead
+  constexpr int VB = KS > 1 ? KS / 2 : 1;            // value blocks per lane
+  constexpr int NT = KS > 1 ? 2 * VB : 1;            // 32-row tiles of the output
+  constexpr int kPart = D < 128 ? D : 128, kParts = D / kPart;   // dims of an epilogue pass
+  constexpr int kRow = kPart + 4, ROWS = CT * 32;
+  constexpr int kQ = CT * QF * NP * 64 * 16, kJoin = W * 32 * kRow * 4;
+  __shared__ __attribute__((aligned(16))) char s_mem[kQ > kJoin ? kQ : kJoin];
+  bf16x8_t* const s_q = reinterpret_cast<bf16x8_t*>(s_mem);   // [CT][QF][NP][64]
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 5, col = lane & 31, half = col >> 4, c = lane & 15;
+  int idx = blockIdx.x;
+  const int sp = idx % p.nsplit;
+  idx /= p.nsplit;
+  const int h = idx % p.Hkv;
+  idx /= p.Hkv;
+  const int seg = idx % p.nseg;
+  const int rt = p.row_tiles - 1 - idx / p.nseg;
+  const int q0 = p.seg_q0[seg], pos0 = p.seg_pos0[seg], len = segment_rows(p, q0, p.seg_len[seg]);
+  const int rows = len * p.G, row0 = rt * ROWS;
+  if (row0 >= rows) return;
+  auto limit = [&](int r) { return min(pos0 + min(r, rows - 1) / p.G, p.max_ctx - 1); };
+  const int wg_first = limit(row0), wg_end = limit(row0 + ROWS - 1);
+  const int lo = sp * p.tps, wg_last = min(wg_end, lo + p.tps - 1);
+  if (lo > wg_last && sp > 0) return;
+
+  // queries -> LDS, as the operands the waves read
+  int lim[CT];   // last position the column attends to; negative: none
 #pragma unroll
-    for (int mc = 0; mc < MC; ++mc) {
-      const float* const row = join + mc * 16 * kRow;
-      const float M = fmaxf(m2[mc], row[D]), fa = fast_exp2(m2[mc] - M), fb = fast_exp2(row[D] - M);
-      m2[mc] = M;
-      sum[mc][0] = __builtin_fmaf(row[D + 1], fb, sum[mc][0] * fa);
+  for (int ct = 0; ct < CT; ++ct) {
+    lim[ct] = limit(row0 + ct * 32 + col);
+    const int r = min(row0 + ct * 32 + col, rows - 1), tok = r / p.G, hq = h * p.G + r % p.G;
+    const char* src = p.q + ((int64_t)(q0 + tok) * p.q_stride + (int64_t)hq * D) * EB;
+    for (int f = wave; f < QF; f += W) {
+      float x[8];
+      load8<Tag>(src + ((2 * (f & 1) + g) * (D / 4) + 8 * (f >> 1)) * EB, x);
 #pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        const f32x4 e = *reinterpret_cast<const f32x4*>(row + 32 * s + 8 * g), o = *reinterpret_cast<const f32x4*>(row + 32 * s + 8 * g + 4);
+      for (int e = 0; e < 8; ++e) x[e] = p.flip ? -x[e] : x[e];
+      bf16x8_t y[NP];
+      bf16_pieces<NP>(x, y);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          acc[mc][s][0][i] = __builtin_fmaf(e[i], fb, acc[mc][s][0][i] * fa);
-          acc[mc][s][1][i] = __builtin_fmaf(o[i], fb, acc[mc][s][1][i] * fa);
-        }
-      }
+      for (int n = 0; n < NP; ++n) s_q[((ct * QF + f) * NP + n) * 64 + lane] = y[n];
     }
   }
+
+  f32x16 acc[CT][NT];
+  float m[CT], m2[CT], sum[CT];   // running maximum of the raw scores, and times the scale; sum of the lane's weights
 #pragma unroll
-  for (int mc = 0; mc < MC; ++mc) {
-    if (orow[mc] < 0) continue;
-    if (p.nsplit > 1) {
-      float* rec = p.ws + (orow[mc] * p.nsplit + sp) * (D + 4);
+  for (int ct = 0; ct < CT; ++ct) {
+    m[ct] = m2[ct] = kKv4Floor;
+    sum[ct] = 0.f;
 #pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        const f32x4 e = acc[mc][s][0], o = acc[mc][s][1];
-        *reinterpret_cast<f32x4*>(rec + 32 * s + 8 * g) = f32x4{e[0], o[0], e[1], o[1]};
-        *reinterpret_cast<f32x4*>(rec + 32 * s + 8 * g + 4) = f32x4{e[2], o[2], e[3], o[3]};
+    for (int j = 0; j < NT; ++j) acc[ct][j] = 0.f;
+  }
+
+  const int32_t* table = p.bt + (int64_t)seg * p.max_blocks;
+  const int last_tile = max(wg_last, 0) / kKv4Tile;
+  const char* const kbase = p.cache.k + (int64_t)h * p.cache.s_head;
+  const char* const vbase = p.cache.v + (int64_t)h * p.cache.s_head;
+  Kv4Place n0{}, n1{};
+  auto place = [&](int t0) {
+    const int tile = (int)((uint32_t)t0 / kKv4Tile);
+    n0 = kv4_place(p.cache, table, min(tile, last_tile));
+    n1 = kv4_place(p.cache, table, min(tile + 1, last_tile));
+  };
+  // K: lane (g, R) holds token (R & 7) + 8 (R >> 4) of tile (R >> 3) & 1, dims of groups g and 2 + g
+  constexpr int KW = D / 32, SW = D == 256 ? 2 : 1;
+  const int ktok = (col & 7) + 8 * half;
+  const bool ktile = (col >> 3) & 1;
+  const uint32_t o_k = ktok * (D / 2) + g * (D / 8);
+  const int sbyte = ktok * (D / 32) + (D == 256 ? 2 * g : D == 128 ? g : 0);   // of group g, s = 0
+  const uint32_t o_ks = 8 * D + (D == 256 ? ktok * 8 : (sbyte & ~3)), turn = 9 + 8 * (sbyte & 3);
+  uint32_t o_v = ((g * 16 + c) * KS + (KS > 1 ? half * VB : 0)) * 4, o_vs = 8 * D + (g * KS + (KS > 1 ? half * VB : 0)) * 4;
+  uint32_t rk[2][KW], rks[SW], rv[2][2][VB], rvs[2][2][VB];
+  auto fetch_k = [&](int64_t r0, int64_t r1) {
+    const gptr rec = (gptr)kbase + (ktile ? r1 : r0);
+    load_words<false>(rec + o_k, rk[0]);
+    load_words<false>(rec + o_k + D / 4, rk[1]);
+    load_words<false>(rec + o_ks, rks);
+  };
+  auto fetch_v = [&](int64_t r0, int64_t r1) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      gptr rec = scalar_base(vbase + (t ? r1 : r0));
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        load_words<false>(rec + lane_offset(o_v) + q * 64 * D / 16, rv[t][q]);
+        load_words<false>(rec + lane_offset(o_vs) + q * 2 * KS * 4, rvs[t][q]);
       }
-      if (g == 0) *reinterpret_cast<f32x4*>(rec + D) = f32x4{m2[mc], sum[mc][0], 0.f, 0.f};
-      continue;
     }
-    const float inv = lim[mc] >= 0 ? 1.f / sum[mc][0] : 0.f;   // a query before position 0 sees nothing: zeros
+  };
+  auto k_scale = [&](int f) {
+    const int pt = f & 1, s = f >> 1;
+    if constexpr (D == 256) return u2f(__builtin_amdgcn_alignbit(rks[pt], rks[pt], turn + 8 * (s >> 2)));
+    return u2f(__builtin_amdgcn_alignbit(rks[0], rks[0], turn + pt * (D == 128 ? 16 : D == 64 ? 8 : 0)));
+  };
+  __syncthreads();
+
+  constexpr int kStride = W * kKv4Step;
+  int t0 = lo + wave * kKv4Step;
+  if (t0 <= wg_last) {
+    place(t0);
+    const int64_t r0 = kv4_record(p.cache, n0, kv4_tile_bytes(D)), r1 = kv4_record(p.cache, n1, kv4_tile_bytes(D));
+    fetch_k(r0, r1);
+    fetch_v(r0, r1);
+    place(min(t0 + kStride, wg_last));
+  }
+  for (; t0 <= wg_last; t0 += kStride) {
+    const int64_t r0 = kv4_record(p.cache, n0, kv4_tile_bytes(D)), r1 = kv4_record(p.cache, n1, kv4_tile_bytes(D));
+    const bool masked = t0 + kKv4Step - 1 > wg_first;
+    if (masked) {
+      uint32_t nan[VB];
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      const f32x4 e = acc[mc][s][0], o = acc[mc][s][1];
-      float x[8] = {e[0], o[0], e[1], o[1], e[2], o[2], e[3], o[3]};
+      for (int b = 0; b < VB; ++b) nan[b] = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = lim[mc] >= 0 ? x[i] * inv : 0.f;
-      store8<Tag>(p.out + (orow[mc] * D + 32 * s + 8 * g) * EB, x);
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const int live = wg_last + 1 - (t0 + t * kKv4Tile + 4 * (g + 2 * q));
+          const uint32_t keep = live >= 4 ? ~0u : (live <= 0 ? 0u : (1u << (8 * live)) - 1u);
+#pragma unroll
+          for (int b = 0; b < VB; ++b) {
+            const uint32_t vs = (rvs[t][q][b] & keep) | (0x7f7f7f7fu & ~keep);
+            uint32_t bad = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const bool is_nan = ((vs >> (8 * j)) & 0xffu) == 255u;
+              bad |= is_nan ? 0xffu << (8 * j) : 0u;
+              nan[b] |= is_nan ? 1u << (t * 16 + 4 * (g + 2 * q) + j) : 0u;
+            }
+            rv[t][q][b] &= keep & ~bad;
+            rvs[t][q][b] = (vs & ~bad) | (0x7f7f7f7fu & bad);
+          }
+        }
+#pragma unroll
+      for (int b = 0; b < VB; ++b) {
+        nan[b] |= __shfl_xor(nan[b], 32);   // all tokens; by halves of the lanes the two blocks
+        const uint32_t mine = nan[b], other = __shfl_xor(mine, 16);
+        if (__ballot(mine | other)) {
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct) {
+            const int seen = lim[ct] + 1 - t0;   // tokens of the step the column sees
+            const uint32_t sees = seen >= 32 ? ~0u : (seen <= 0 ? 0u : (1u << seen) - 1u);
+            const bool low = ((half ? other : mine) & sees) != 0, high = ((half ? mine : other) & sees) != 0;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {   // (rows 16 .. 31, the second half's blocks, are elements 8 .. 15)
+              const bool hit = KS > 1 && e >= 8 ? high : low;
+              acc[ct][NT > 1 ? 2 * b : 0][e] = hit ? __builtin_nanf("") : acc[ct][NT > 1 ? 2 * b : 0][e];
+              if constexpr (NT > 1) acc[ct][2 * b + 1][e] = hit ? __builtin_nanf("") : acc[ct][2 * b + 1][e];
+            }
+          }
+        }
+      }
+    }
+    f32x16 S[CT];
+    bf16x8_t qr[QD][CT][NP];
+    auto read_q = [&](int f) {
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+        for (int n = 0; n < NP; ++n) qr[f % QD][ct][n] = s_q[((ct * QF + f) * NP + n) * 64 + lane];
+    };
+#pragma unroll
+    for (int f = 0; f < QD; ++f) read_q(f);
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) S[ct] = 0.f;
+#pragma unroll
+    for (int f = 0; f < QF; ++f) {
+      const bf16x8_t a = kv4_k_frag(rk[f & 1][f >> 1], k_scale(f));
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+        for (int n = 0; n < NP; ++n) S[ct] = mfma32_bf16(a, qr[f % QD][ct][n], S[ct]);
+      if (f + QD < QF) read_q(f + QD);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    fetch_k(r0, r1);
+    place(min(t0 + 2 * kStride, wg_last));
+    bf16x8_t pf[CT][2][NP];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      if (masked) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (t0 + Layout<32>::token(g, e) > lim[ct]) S[ct][e] = -INFINITY;
+      }
+      float top = S[ct][0];
+#pragma unroll
+      for (int e = 1; e + 1 < 16; e += 2) top = fmaxf(fmaxf(top, S[ct][e]), S[ct][e + 1]);
+      top = fmaxf(top, S[ct][15]);
+      if (__ballot(top > m[ct] + p.raise)) {
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const float mn = fmaxf(m[ct], top), f = fast_exp2((m[ct] - mn) * p.scale2);
+        m[ct] = mn;
+        m2[ct] = fmaxf(mn * p.scale2, kKv4Floor);
+        sum[ct] *= f;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[ct][j] *= f;
+      }
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          x[e] = fast_exp2(__builtin_fmaf(S[ct][8 * n + e], p.scale2, -m2[ct]));
+          sum[ct] += x[e];
+        }
+        bf16_pieces<NP>(x, pf[ct][n]);
+      }
+    }
+#pragma unroll
+    for (int b = 0; b < VB; ++b)
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        bf16x8_t ev, od;
+        kv4_v_frags(rv[0][q][b], rv[1][q][b], rvs[0][q][b], rvs[1][q][b], ev, od);
+        if constexpr (KS == 1) ev = half ? od : ev;
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+          for (int n = 0; n < NP; ++n) {
+            acc[ct][NT > 1 ? 2 * b : 0] = mfma32_bf16(ev, pf[ct][q][n], acc[ct][NT > 1 ? 2 * b : 0]);
+            if constexpr (NT > 1) acc[ct][2 * b + 1] = mfma32_bf16(od, pf[ct][q][n], acc[ct][2 * b + 1]);
+          }
+      }
+    fetch_v(r0, r1);
+  }
+
+  // join the waves
+  float* const s_o = reinterpret_cast<float*>(s_mem) + wave * 32 * kRow;
+  constexpr int P = kPart / 8;
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    const float total = sum[ct] + __shfl_xor(sum[ct], 32);
+#pragma unroll
+    for (int part = 0; part < kParts; ++part) {
+      __syncthreads();
+      float* const row = s_o + col * kRow;
+#pragma unroll
+      for (int j = 0; j < VB; ++j)
+#pragma unroll
+        for (int hf = 0; hf < (KS > 1 ? 2 : 1); ++hf) {
+          const int blk = j + hf * VB;
+          if (blk * 32 / kPart != part) continue;
+#pragma unroll
+          for (int bl = 0; bl < 2; ++bl) {
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              if constexpr (KS > 1) {
+                x[2 * i] = acc[ct][2 * j][(2 * hf + bl) * 4 + i];
+                x[2 * i + 1] = acc[ct][2 * j + 1][(2 * hf + bl) * 4 + i];
+              } else {
+                x[2 * i] = acc[ct][0][bl * 4 + i];
+                x[2 * i + 1] = acc[ct][0][8 + bl * 4 + i];
+              }
+            }
+            store8<F32>(reinterpret_cast<char*>(row + (blk * 32) % kPart + 16 * bl + 8 * g), x);
+          }
+        }
+      if (g == 0) *reinterpret_cast<f32x4*>(row + kPart) = f32x4{m2[ct], total, 0.f, 0.f};
+      __syncthreads();
+      for (int item = threadIdx.x; item < 32 * P; item += 256) {
+        const int cc = item / P, d = item % P * 8, r = row0 + ct * 32 + cc;
+        if (r >= rows) continue;
+        const float* rec = reinterpret_cast<const float*>(s_mem) + cc * kRow;
+        float M = kKv4Floor, L = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < W; ++w) M = fmaxf(M, rec[w * 32 * kRow + kPart]);
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+          const float f = fast_exp2(rec[w * 32 * kRow + kPart] - M);
+          L = __builtin_fmaf(rec[w * 32 * kRow + kPart + 1], f, L);
+          float y[8];
+          load8<F32>(reinterpret_cast<const char*>(rec + w * 32 * kRow + d), y);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) o[e] = __builtin_fmaf(y[e], f, o[e]);
+        }
+        const int tok = r / p.G, hq = h * p.G + r % p.G;
+        const int64_t orow = (int64_t)(q0 + tok) * p.Hq + hq;
+        if (p.nsplit > 1) {
+          float* out = p.ws + (orow * p.nsplit + sp) * (D + 4);
+          store8<F32>(reinterpret_cast<char*>(out + part * kPart + d), o);
+          if (d == 0 && part == 0) *reinterpret_cast<f32x4*>(out + D) = f32x4{M, L, 0.f, 0.f};
+        } else {
+          const bool any = limit(r) >= 0;
+          const float inv = any ? 1.f / L : 0.f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) o[e] = any ? o[e] * inv : 0.f;
+          store8<Tag>(p.out + (orow * D + part * kPart + d) * EB, o);
+        }
+      }
     }
   }
 }
@@ -419,7 +711,9 @@ void launch_merge(const Kv4PrefillParams& p, hipStream_t s) {
 }
 
 struct Kv4PrefillPlan {
-  int MC, teams, row_tiles, nsplit, tps;
+  bool dealt;            // kv4_rows_kernel, else kv4_prefill_kernel
+  int tiles, row_tiles;  // column tiles per wave; workgroups along a segment's rows
+  int nsplit, tps;       // splits of the context, tokens of one
   size_t ws_bytes;
 };
 
@@ -434,42 +728,47 @@ int make_plan(const char* what, int nseg, int total_rows, int max_q_len, int Hq,
   max_q_len = std::min(max_q_len, total_rows);
   const int64_t rows = (int64_t)max_q_len * (Hq / Hkv), heads = (int64_t)std::max(nseg, 1) * Hkv;
   if (rows > INT32_MAX) return fail(MI355_EINVAL, "%s: max_q_len %d", what, max_q_len);
-  // Two tiles of 16 rows per wave use every converted operand twice, one tile makes twice the workgroups.  Two teams per
-  // workgroup halve the stages of its walk and fill a chip that has too few workgroups, but take twice its LDS: they pay while
-  // all workgroups fit at once, one per CU, or (deep contexts, up to 64 dims) two.  us, as chosen / the other way:
-  //   two tiles: 8 prompts of 4096, 8 heads of 64 172 / 197; 8 of 1024, 8 of 128 37 / 42; 4 of 300, 32/8 of 128 32 / 37
-  //   one tile: 16 uneven chunks to 1024, 8 of 64 43 / 47; 12 uneven fp16 prompts to 1500 49 / 54; 5 of 512, 8 of 128 17 / 22
-  //   two teams: a prompt of 2000, 8 heads of 64 22 / 29; one of 500, 32/8 of 128 14.4 / 16.3; 2 of 128 behind 2000, 32/8 of
-  //   256 44 / 78; 8 of 512 behind 2000, 8 of 64 38 / 46; two tiles: 4 of 256 behind 3000, 32/8 of 128 67 / 88
-  //   one team: 12 uneven prompts to 400, 8 of 64 10.7 / 12.2; 8 of 4096, 8 of 64 172 / 228; 16 of 100 7.5 / 7.9
-  // Two tiles' registers at head_dim 256 (fp32: 128) would leave one wave per SIMD.
-  const bool narrow = D == 256 || (dtype == MI355_F32 && D == 128);
+  // kv4_rows_kernel has shorter walks and no barriers, but converts every code once per 32 (two tiles: 64) rows, where
+  // kv4_prefill_kernel does per 64 (128): the former while its workgroups fit the chip about at once -- three of one tile per
+  // CU, two beyond 64 dims; two of two tiles -- the latter beyond.  us, as chosen / the next best:
+  //   dealt, one tile   8 chunks to 45 behind 900, 8 heads of 64 10.5 / 13.9; a prompt of 2000, 8 of 64 15.3 / 21; one of 500,
+  //                     32/8 of 128 11.4 / 14.8; 2 of 128 behind 2000, 32/8 of 256 33 / 76; 5 of 512 behind 2000, 8 of 64, fp32
+  //                     50 / 57; 2 of 200 .. 300 behind 500 .. 1500, 32/8 of 128, fp16 45 / 52
+  //   dealt, two tiles  8 of 512 behind 2000, 8 of 64 34 / 40; 4 of 256 behind 3000, 32/8 of 128 65 / 75; a prompt of 2000,
+  //                     32/8 of 128 51 / 56
+  //   shared, one tile  16 uneven chunks to 1024, 8 of 64 42 / 44; 12 uneven fp16 prompts to 1500, 8 of 64 47.9 / 48.9; 3 of
+  //                     256, 32/8 of 128 12.2 / 13.8; 16 of 500, fp16, 8 of 256 54 / 75
+  //   shared, two tiles 8 of 4096, 8 of 64 158 / 200; 4 of 2048 behind 2048, 32/8 of 128 404 / 440; 8 of 1024, 8 of 128 36 / 38
+  // Registers set limits: two tiles spill at head_dim 256 and fp32's 128, and fp16's 128 where they are dealt.
+  const bool narrow = D == 256 || (dtype == MI355_F32 && D == 128), single = narrow || (dtype == MI355_F16 && D == 128);
   const int64_t all_rows = (int64_t)total_rows * (Hq / Hkv);
-  auto workgroups = [&](int mc) {   // of uneven segments: no more than the rows there are
-    const int64_t per = kWaves * 16 * mc;
+  auto workgroups = [&](int64_t per) {   // of uneven segments: no more than the rows there are
     return std::min(heads * ceil_div64(rows, per), Hkv * (ceil_div64(all_rows, per) + nseg));
   };
-  const int64_t wgs1 = workgroups(1), wgs2 = workgroups(2);
-  const bool deep = max_ctx >= 1536;
-  pl->MC = !narrow && (D <= 64 ? wgs2 >= 1024 : wgs2 > 256 || (wgs1 > 256 && deep)) ? 2 : 1;
-  pl->teams = 1;
-  if (max_ctx >= 256 && wgs1 <= 256) pl->teams = 2;
-  if (deep && (D <= 64 ? wgs1 <= 512 : pl->MC == 2 && wgs2 <= 256)) pl->teams = 2;
-  pl->row_tiles = (int)ceil_div64(rows, kWaves * pl->MC * 16);
-  const int stage = kKv4Step * (D == 256 ? 1 : D == 32 ? 4 : 2);
+  const int64_t wgs = workgroups(32);
+  pl->dealt = true;
+  pl->tiles = 1;
+  if (wgs > (single && max_ctx >= 768 ? 1024 : D <= 64 ? 768 : 512)) {
+    pl->tiles = 2;
+    if (single || max_ctx < 512 || workgroups(64) >= (D <= 64 ? 513 : 1024)) {
+      pl->dealt = false;
+      pl->tiles = !narrow && workgroups(128) > (D <= 64 ? 1023 : 256) ? 2 : 1;
+    }
+  }
+  pl->row_tiles = (int)ceil_div64(rows, (pl->dealt ? 32 : 64) * pl->tiles);
+  // Fewer workgroups than CUs: the context is split until there is one each, no split shorter than 256 tokens (16 tokens
+  // behind 30000, 32/8 heads of 128: 170 -> 23 us; 4 chunks to 64 behind 1500, 8/2 heads of 256: 23.9 -> 19.9), if that takes
+  // 1100 tokens off a walk: the merge costs a launch (4.4 us of the host's time) and the rows' partial sums (2 chunks of 64
+  // behind 2000, 32/8 heads of 128: 19.1 in one, 17.9 in two, 24.7 in eight).
+  const int stage = kWaves * kKv4Step;
   const int64_t stages = ceil_div64(max_ctx, stage);
-  // Still fewer than one workgroup per CU: the context is split until there is one, no split shorter than 256 tokens (16
-  // tokens behind 30000, 32/8 heads of 128: 348 -> 27 us; 8 chunks to 64 behind 2000, 8 heads of 64: 23.2 -> 15.4), if that
-  // takes 800 tokens off a walk.  The merge costs a launch (4.4 us of the host's time) and the rows' partial sums: 8 chunks
-  // to 45 behind 900 take 13.9 in one, 12.4 in four splits and 17 where the host is what they wait for; 128 tokens behind
-  // 1000, 32/8 heads of 128, 21.5 in one, 22.9 in two.
-  int64_t want = wgs1 <= 256 ? std::min<int64_t>(256 / std::max<int64_t>(wgs1, 1), ceil_div64(max_ctx, 256)) : 1;
-  if (max_ctx - max_ctx / want < 800) want = 1;
+  int64_t want = wgs <= 128 ? std::min<int64_t>(256 / std::max<int64_t>(wgs, 1), ceil_div64(max_ctx, 256)) : 1;
+  if (max_ctx - max_ctx / want < 1100) want = 1;
   const int64_t per = ceil_div64(stages, std::min(want, stages));
   pl->tps = (int)(per * stage);
   pl->nsplit = (int)ceil_div64(stages, per);
   pl->ws_bytes = pl->nsplit > 1 ? (size_t)total_rows * Hq * pl->nsplit * (D + 4) * sizeof(float) : 0;
-  if (!kv4_grid_ok(heads * pl->row_tiles * pl->nsplit, 256 * pl->teams) ||
+  if (!kv4_grid_ok(heads * pl->row_tiles * pl->nsplit, 256) ||
       (pl->nsplit > 1 && !kv4_grid_ok((int64_t)nseg * max_q_len * Hq, 256)))
     return fail(MI355_EINVAL, "%s: too many workgroups (nseg=%d max_q_len=%d Hq=%d)", what, nseg, max_q_len, Hq);
   return 0;
@@ -477,14 +776,16 @@ int make_plan(const char* what, int nseg, int total_rows, int max_q_len, int Hq,
 
 template <class Tag, int D>
 int launch(const Kv4PrefillParams& p, const Kv4PrefillPlan& pl, hipStream_t s) {
-  const dim3 grid((unsigned)((int64_t)p.row_tiles * p.nseg * p.Hkv * p.nsplit)), one(256), two(512);
-  if constexpr (D < 256 && !(Tag::kCode == MI355_F32 && D == 128)) {
-    if (pl.MC == 2 && pl.teams == 1) hipLaunchKernelGGL((kv4_prefill_kernel<Tag, D, 2, 1>), grid, one, 0, s, p);
-    if constexpr (D == 128)
-      if (pl.MC == 2 && pl.teams == 2) hipLaunchKernelGGL((kv4_prefill_kernel<Tag, D, 2, 2>), grid, two, 0, s, p);
+  const dim3 grid((unsigned)((int64_t)p.row_tiles * p.nseg * p.Hkv * p.nsplit)), block(256);
+  constexpr bool narrow = D == 256 || (Tag::kBytes == 4 && D == 128), single = narrow || (Tag::kCode == MI355_F16 && D == 128);
+  if (pl.tiles == 1) {
+    if (pl.dealt) hipLaunchKernelGGL((kv4_rows_kernel<Tag, D, 1>), grid, block, 0, s, p);
+    else hipLaunchKernelGGL((kv4_prefill_kernel<Tag, D, 16>), grid, block, 0, s, p);
+  } else if (pl.dealt) {
+    if constexpr (!single) hipLaunchKernelGGL((kv4_rows_kernel<Tag, D, 2>), grid, block, 0, s, p);
+  } else {
+    if constexpr (!narrow) hipLaunchKernelGGL((kv4_prefill_kernel<Tag, D, 32>), grid, block, 0, s, p);
   }
-  if (pl.MC == 1 && pl.teams == 1) hipLaunchKernelGGL((kv4_prefill_kernel<Tag, D, 1, 1>), grid, one, 0, s, p);
-  if (pl.MC == 1 && pl.teams == 2) hipLaunchKernelGGL((kv4_prefill_kernel<Tag, D, 1, 2>), grid, two, 0, s, p);
   if (int rc = check_launch("kv4_prefill_kernel")) return rc;
   if (p.nsplit > 1) {
     if (p.nsplit <= kKv4WalkedSplits) launch_merge<Tag, D, kv4_split_lanes<D>(true)>(p, s);
