@@ -2,6 +2,8 @@
 
 Every function walks dims, tokens or bytes by their place in the format; none shares code or layout
 tricks with the kernels."""
+import functools
+
 import numpy as np
 
 MAGNITUDES = np.array([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0])
@@ -80,6 +82,7 @@ def write_row(record, row, code, byte, value_form):
         record[scale_place(D, row, b, value_form)] = byte[b]
 
 
+@functools.lru_cache(None)
 def _places(D, value_form):
     at = np.array([[code_place(D, r, d, value_form)[0] for d in range(D)] for r in range(16)])
     shift = np.array([[code_place(D, r, d, value_form)[1] for d in range(D)] for r in range(16)])
