@@ -67,6 +67,7 @@ def require_device(*tensors: torch.Tensor) -> torch.device:
 
 
 _raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None)
+_current_device = getattr(torch._C, '_cuda_getDevice', torch.cuda.current_device)   # (a tensor on it exists: nothing is left to initialise)
 
 
 def _stream(dev: torch.device) -> int:
@@ -91,7 +92,7 @@ _NO_SWITCH = _NoSwitch()
 def _on(dev: torch.device):
     """Context in which `dev` is the current HIP device; free when it already is (the usual
     case: torch's device guard costs several microseconds per call)."""
-    if dev.index is None or torch.cuda.current_device() == dev.index:
+    if dev.index is None or _current_device() == dev.index:
         return _NO_SWITCH
     return torch.cuda.device(dev)
 
@@ -768,6 +769,7 @@ def paged_prefill(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
 
 KV4_HEAD_DIMS = (32, 64, 128, 256)
 KV4_TILE = 16          # tokens per record; a block holds a whole number of them
+_KV4_RECORDS = {17 * d // 2: d for d in KV4_HEAD_DIMS}
 
 
 def kv4_cache_shape(num_blocks: int, kv_heads: int, block_size: int, head_dim: int) -> Tuple[int, int, int, int]:
@@ -785,7 +787,8 @@ def _kv4_geometry(k_cache: torch.Tensor, v_cache: torch.Tensor):
     shape, strides = k_cache.shape, k_cache.stride()
     if k_cache.dtype != torch.uint8 or v_cache.dtype != torch.uint8:
         raise TypeError("4-bit caches are uint8 tensors")
-    if len(shape) != 4 or shape != v_cache.shape or (shape[3] * 2) % 17 or shape[3] * 2 // 17 not in KV4_HEAD_DIMS:
+    head_dim = _KV4_RECORDS.get(shape[-1]) if len(shape) == 4 and shape == v_cache.shape else None
+    if head_dim is None:
         raise ValueError(f"4-bit caches must share the shape kv4_cache_shape gives, got {tuple(shape)} and "
                          f"{tuple(v_cache.shape)}")
     blocks, heads, tiles, record = shape
@@ -794,7 +797,14 @@ def _kv4_geometry(k_cache: torch.Tensor, v_cache: torch.Tensor):
         strides = tuple(_stride(k_cache, d) for d in range(4))
         if strides != tuple(_stride(v_cache, d) for d in range(4)) or strides[3] != 1 or strides[2] != record:
             raise ValueError("4-bit caches must share strides, with the tiles of a head contiguous")
-    return blocks, heads, tiles * KV4_TILE, record * 2 // 17, strides[0], strides[1]
+    return blocks, heads, tiles * KV4_TILE, head_dim, strides[0], strides[1]
+
+
+def _rows_like(t: torch.Tensor, out: Optional[torch.Tensor], dev: torch.device) -> torch.Tensor:
+    """`out`, checked, or a contiguous tensor of t's shape and dtype (the quickest allocation torch has where t itself is one)."""
+    if out is not None:
+        return _checked_out(out, t.shape, t.dtype, dev)
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=dev)
 
 
 def _packed_rows(t: torch.Tensor) -> int:
@@ -858,7 +868,7 @@ def rope_angles(positions: torch.Tensor, inv_freq: torch.Tensor, factor: float =
     positions, inv_freq = positions.contiguous(), inv_freq.contiguous()
     T, half = positions.shape[0], inv_freq.shape[0]
     cos = torch.empty((T, half), dtype=torch.float32, device=dev)
-    sin = torch.empty((T, half), dtype=torch.float32, device=dev)
+    sin = torch.empty_like(cos)
     with _on(dev):
         rc = lib.mi355_rope_angles(cos.data_ptr(), sin.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(),
                                    float(factor), T, half, _stream(dev))
@@ -888,7 +898,7 @@ def rope_rotate(x: torch.Tensor, cos: Optional[torch.Tensor], sin: Optional[torc
     stride = _packed_rows(x)
     T, H, D = x.shape
     R = _angle_rows(cos, sin, T)
-    out = torch.empty((T, H, D), dtype=x.dtype, device=dev) if out is None else _checked_out(out, (T, H, D), x.dtype, dev)
+    out = _rows_like(x, out, dev)
     with _on(dev):
         rc = lib.mi355_rope_rotate(out.data_ptr(), x.data_ptr(), stride, cos.data_ptr() if R else None,
                                    sin.data_ptr() if R else None, R, int(interleaved), T, H, D, dtype_code(x),
@@ -918,7 +928,7 @@ def rope_kv4_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: Optio
         raise TypeError("slots must be int64 [T]")
     slots = slots.contiguous()
     R = _angle_rows(cos, sin, T)
-    out = torch.empty((T, Hq, D), dtype=dtype, device=dev) if out is None else _checked_out(out, (T, Hq, D), dtype, dev)
+    out = _rows_like(q, out, dev)
     with _on(dev):
         rc = lib.mi355_rope_kv4_write(
             out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), q_stride, k_stride, v_stride,
@@ -941,7 +951,7 @@ def kv4_read_slots(k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Te
     slots = slots.contiguous()
     T = slots.shape[0]
     k = torch.empty((T, Hkv, D), dtype=dtype, device=dev)
-    v = torch.empty((T, Hkv, D), dtype=dtype, device=dev)
+    v = torch.empty_like(k)
     code = dtype_code(k)
     with _on(dev):
         rc = lib.mi355_kv4_read_slots(k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
@@ -972,7 +982,7 @@ def paged_decode_kv4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         raise ValueError("block_tables must be [B, max_blocks] and context_lens [B]")
     block_tables, context_lens = block_tables.contiguous(), context_lens.contiguous()
     code = dtype_code(q)
-    out = torch.empty((B, Hq, D), dtype=q.dtype, device=dev) if out is None else _checked_out(out, (B, Hq, D), q.dtype, dev)
+    out = _rows_like(q, out, dev)
     if scale is None:
         scale = 1.0 / math.sqrt(D)
     width = block_tables.shape[1]
@@ -1015,7 +1025,7 @@ def paged_prefill_kv4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     block_tables = block_tables.contiguous()
     seg_q_start, seg_len, seg_pos0 = seg_q_start.contiguous(), seg_len.contiguous(), seg_pos0.contiguous()
     code = dtype_code(q)
-    out = torch.empty((T, Hq, D), dtype=q.dtype, device=dev) if out is None else _checked_out(out, (T, Hq, D), q.dtype, dev)
+    out = _rows_like(q, out, dev)
     if T == 0:
         return out
     if scale is None:
