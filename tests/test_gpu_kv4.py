@@ -813,3 +813,26 @@ def test_engine_rotary_settings_equal_the_table_where_they_mean_the_same(device)
         with torch.no_grad():
             logits.append(model(torch.arange(1, n + 1, device=device), pos, pos, [n], [True], block_tables=[list(range(9))]))
     torch.testing.assert_close(logits[0], logits[1], atol=1e-3, rtol=1e-3)
+
+
+def test_engine_prefix_caching_over_a_4_bit_cache(device):
+    """Requests that share full prompt blocks read the 4-bit blocks of the first; tokens as without sharing (float32
+    activations: weights carry 24 bits, so the way a prompt is cut moves logits by rounding only)."""
+    import mini_vllm as mv
+    rng = np.random.default_rng(3)
+    prefix, tails = rng.integers(1, 300, 70).tolist(), [rng.integers(1, 300, n).tolist() for n in (9, 30, 1)]
+    results = []
+    for caching in (True, False):
+        torch.manual_seed(7)
+        eng = mv.MiniVLLM(vocab_size=300, hidden_size=128, num_layers=2, num_heads=4, intermediate_size=256, num_kv_blocks=40,
+                          block_size=16, max_num_seqs=4, max_num_batched_tokens=48, device='cuda', dtype=torch.float32,
+                          kv_cache_dtype='mxfp4', enable_prefix_caching=caching)
+        out = []
+        for tail in tails + tails[:1]:
+            eng.add_request(prefix + tail, max_new_tokens=10, temperature=0.0)
+            got = []
+            while eng.scheduler.has_unfinished:
+                got += [tok for _, tok in eng.step()]
+            out.append(got)
+        results.append(out)
+    assert results[0] == results[1] and results[0][0] == results[0][3]
