@@ -460,6 +460,8 @@ WIDE = [
     (4, 2, 256, 16, [200, 100], [700, 0]),
     (8, 8, 32, 16, [512, 510, 512, 512, 333, 512], [1300, 0, 1290, 1300, 1000, 1777]),
     (8, 8, 64, 16, [400] * 15 + [33], [0] * 16),
+    (8, 2, 128, 16, [40, 90, 1], [900, 0, 1100]),
+    (4, 4, 32, 32, [130, 3], [0, 1000]),
     (8, 8, 32, 16, [512] * 8, [300] * 8),
     (8, 8, 64, 32, [512, 511] * 4, [300] * 8),
     (8, 8, 32, 16, [2048] * 8, [0] * 8),
@@ -531,7 +533,7 @@ def test_chunk_queries_before_the_first_position_see_nothing(ops, device, ctx):
 
 @pytest.mark.parametrize('Hq,Hkv,D,n,seqs,pos0', [
     (8, 8, 64, 90, 2, 0), (8, 8, 64, 512, 8, 300), (8, 8, 64, 400, 16, 0), (8, 8, 64, 2048, 8, 0), (32, 8, 128, 300, 1, 40),
-    (32, 8, 128, 256, 3, 1600), (8, 8, 128, 250, 9, 0), (32, 8, 128, 300, 4, 0), (8, 8, 256, 250, 9, 0), (8, 2, 256, 60, 1, 9),
+    (32, 8, 128, 256, 3, 1600), (8, 2, 128, 60, 2, 1000), (8, 8, 128, 250, 9, 0), (32, 8, 128, 300, 4, 0), (8, 8, 256, 250, 9, 0), (8, 2, 256, 60, 1, 9),
     (8, 8, 32, 512, 8, 300), (8, 8, 32, 400, 16, 0), (8, 8, 32, 2048, 8, 0), (4, 2, 32, 50, 1, 5)])
 def test_chunk_nan_pattern_in_every_form(ops, device, Hq, Hkv, D, n, seqs, pos0):
     """NaN value blocks within a chunk, one behind it and a NaN key: the queries that see them and no others, in the dims

@@ -12,8 +12,8 @@
 //       all back.  Codes travel from memory one stage ahead in registers, operands one stage ahead in LDS
 //       (two buffers, one barrier per stage).  LDS is its bound: 20 KiB per step of 32 columns, 160 of the
 //       roughly 270 cycles that a CU takes for it at 128 dims.
-//   kv4_rows_kernel     few rows.  A workgroup owns 32 or 64 columns, its waves take the steps in turn and
-//       convert their own in registers: no barrier, a quarter of the walk, more conversion per row.
+//   kv4_rows_kernel     few rows.  A workgroup owns 32 or 64 columns, its four or eight waves take the steps in turn
+//       and convert their own in registers: no barrier, short walks, more conversion per row.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -385,15 +385,15 @@ __global__ void __launch_bounds__(256, 2) kv4_prefill_kernel(const Kv4PrefillPar
     }
 }
 
-// A workgroup of CT tiles of 32 query rows; its four waves take the steps of the context in turn, so that a walk is a quarter
+// A workgroup of CT tiles of 32 query rows; its W waves take the steps of the context in turn, so that a walk is 1 / W
 // as long.  A wave converts its own steps in registers, as decode does, in the lanes where the matrix instruction wants them:
 //   K  lane (g, R) holds token (R & 7) + 8 (R >> 4) of tile (R >> 3) & 1, dims of groups g and 2 + g
 //   V  lane (g, half, c) holds dims 2 c, 2 c + 1 of a block of its half of the blocks, tokens of groups g and 2 + g; the even
 //      dims of two blocks are the 32 rows of one product, the odd dims of another (head_dim 32: both of the only block)
 // The queries wait in LDS, where the waves' sums meet at the end.
-template <class Tag, int D, int CT>
-__global__ void __launch_bounds__(256, 2) kv4_rows_kernel(const Kv4PrefillParams p) {
-  constexpr int NP = Kv4Pieces<Tag>::n, KS = D / 32, EB = Tag::kBytes, QF = 2 * KS, W = kWaves;
+template <class Tag, int D, int CT, int W>
+__global__ void __launch_bounds__(W * 64, 2) kv4_rows_kernel(const Kv4PrefillParams p) {
+  constexpr int NP = Kv4Pieces<Tag>::n, KS = D / 32, EB = Tag::kBytes, QF = 2 * KS;
   constexpr int QD = QF < 4 ? QF : NP == 1 && D < 256 && CT == 1 ? 4 : 2;   // query operands read ahead
   constexpr int VB = KS > 1 ? KS / 2 : 1;            // value blocks per lane
   constexpr int NT = KS > 1 ? 2 * VB : 1;            // 32-row tiles of the output
@@ -671,7 +671,7 @@ __global__ void __launch_bounds__(256, 2) kv4_rows_kernel(const Kv4PrefillParams
         }
       if (g == 0) *reinterpret_cast<f32x4*>(row + kPart) = f32x4{m2[ct], total, 0.f, 0.f};
       __syncthreads();
-      for (int item = threadIdx.x; item < 32 * P; item += 256) {
+      for (int item = threadIdx.x; item < 32 * P; item += W * 64) {
         const int cc = item / P, d = item % P * 8, r = row0 + ct * 32 + cc;
         if (r >= rows) continue;
         const float* rec = reinterpret_cast<const float*>(s_mem) + cc * kRow;
@@ -729,7 +729,7 @@ void launch_merge(const Kv4PrefillParams& p, hipStream_t s) {
 
 struct Kv4PrefillPlan {
   bool dealt;            // kv4_rows_kernel, else kv4_prefill_kernel
-  int tiles, row_tiles;  // column tiles per wave; workgroups along a segment's rows
+  int tiles, waves, row_tiles;  // column tiles per wave, waves per workgroup; workgroups along a segment's rows
   int nsplit, tps;       // splits of the context, tokens of one
   size_t ws_bytes;
 };
@@ -774,10 +774,14 @@ int make_plan(const char* what, int nseg, int total_rows, int max_q_len, int Hq,
   }
   pl->row_tiles = (int)ceil_div64(rows, (pl->dealt ? 32 : 64) * pl->tiles);
   // Fewer workgroups than CUs: the context is split until there is one each, no split shorter than 256 tokens (16 tokens
-  // behind 30000, 32/8 heads of 128: 170 -> 23 us; 4 chunks to 64 behind 1500, 8/2 heads of 256: 23.9 -> 19.9), if that takes
+  // behind 30000, 32/8 heads of 128: 137 -> 24 us; 4 chunks to 64 behind 1500, 8/2 heads of 256: 22.0 -> 19.9), if that takes
   // 1100 tokens off a walk: the merge costs a launch (4.4 us of the host's time) and the rows' partial sums (2 chunks of 64
-  // behind 2000, 32/8 heads of 128: 19.1 in one, 17.9 in two, 24.7 in eight).
-  const int stage = kWaves * kKv4Step;
+  // behind 2000, 32/8 heads of 128: 17.1 in one, 18.6 in two, 25.2 in four).
+  // One workgroup per CU or fewer: eight waves each, if the walk is long enough to pay for the larger join (2 of 512 behind
+  // 2000, 8 heads of 64, fp32 25.5 -> 21.7 us; 4 of 100 .. 200 behind 1500 .. 3000, 8 of 128 26.3 -> 22.2; 4 to 64 behind 600,
+  // 8 of 64 8.6 and 8.8; 4 of 250, 8 of 64 6.8 and 7.3).
+  pl->waves = pl->dealt && wgs <= 256 && max_ctx >= 768 ? 8 : kWaves;
+  const int stage = pl->waves * kKv4Step;
   const int64_t stages = ceil_div64(max_ctx, stage);
   int64_t want = wgs <= 128 ? std::min<int64_t>(256 / std::max<int64_t>(wgs, 1), ceil_div64(max_ctx, 256)) : 1;
   if (max_ctx - max_ctx / want < 1100) want = 1;
@@ -785,7 +789,7 @@ int make_plan(const char* what, int nseg, int total_rows, int max_q_len, int Hq,
   pl->tps = (int)(per * stage);
   pl->nsplit = (int)ceil_div64(stages, per);
   pl->ws_bytes = pl->nsplit > 1 ? (size_t)total_rows * Hq * pl->nsplit * (D + 4) * sizeof(float) : 0;
-  if (!kv4_grid_ok(heads * pl->row_tiles * pl->nsplit, 256) ||
+  if (!kv4_grid_ok(heads * pl->row_tiles * pl->nsplit, 64 * pl->waves) ||
       (pl->nsplit > 1 && !kv4_grid_ok((int64_t)nseg * max_q_len * Hq, 256)))
     return fail(MI355_EINVAL, "%s: too many workgroups (nseg=%d max_q_len=%d Hq=%d)", what, nseg, max_q_len, Hq);
   return 0;
@@ -796,10 +800,11 @@ int launch(const Kv4PrefillParams& p, const Kv4PrefillPlan& pl, hipStream_t s) {
   const dim3 grid((unsigned)((int64_t)p.row_tiles * p.nseg * p.Hkv * p.nsplit)), block(256);
   constexpr bool narrow = D == 256 || (Tag::kBytes == 4 && D == 128), single = narrow || (Tag::kCode == MI355_F16 && D == 128);
   if (pl.tiles == 1) {
-    if (pl.dealt) hipLaunchKernelGGL((kv4_rows_kernel<Tag, D, 1>), grid, block, 0, s, p);
+    if (pl.dealt && pl.waves == 8) hipLaunchKernelGGL((kv4_rows_kernel<Tag, D, 1, 8>), grid, dim3(512), 0, s, p);
+    else if (pl.dealt) hipLaunchKernelGGL((kv4_rows_kernel<Tag, D, 1, kWaves>), grid, block, 0, s, p);
     else hipLaunchKernelGGL((kv4_prefill_kernel<Tag, D, 16>), grid, block, 0, s, p);
   } else if (pl.dealt) {
-    if constexpr (!single) hipLaunchKernelGGL((kv4_rows_kernel<Tag, D, 2>), grid, block, 0, s, p);
+    if constexpr (!single) hipLaunchKernelGGL((kv4_rows_kernel<Tag, D, 2, kWaves>), grid, block, 0, s, p);
   } else {
     if constexpr (!narrow) hipLaunchKernelGGL((kv4_prefill_kernel<Tag, D, 32>), grid, block, 0, s, p);
   }
