@@ -339,6 +339,39 @@ def test_decode_long_context_split_and_bounds(ops, device, dtype):
     assert torch.equal(again, out)
 
 
+@pytest.mark.parametrize('dtype', ALL)
+@pytest.mark.parametrize('B,Hq,Hkv,D,longest', [(256, 8, 8, 64, 520), (256, 32, 8, 64, 257), (128, 8, 8, 128, 530), (257, 8, 8, 32, 1030),
+                                                (90, 16, 8, 32, 3000), (8, 8, 4, 128, 20000)])
+def test_decode_of_many_sequences(ops, device, dtype, B, Hq, Hkv, D, longest):
+    """Enough work for several kv heads per wave: six sequences against the oracle, a NaN block in one of them."""
+    rng = np.random.default_rng(B + D)
+    BS, G = 16, Hq // Hkv
+    lens = rng.integers(1, longest + 1, B)
+    lens[[0, B - 1]] = [longest, 1]
+    need = -(-lens // BS)
+    order = rng.permutation(int(need.sum()) + 3)
+    tables = np.zeros((B, int(need.max())), dtype=np.int32)
+    for i, at in enumerate(np.cumsum(need) - need):
+        tables[i, :need[i]] = order[at:at + need[i]]
+    shape = ops.kv4_cache_shape(len(order), Hkv, BS, D)
+    kc, vc = (rng.integers(0, 256, shape, dtype=np.uint8) for _ in range(2))
+    for c in (kc, vc):
+        c[..., 8 * D:] = rng.integers(124, 128, shape[:-1] + (D // 2,), dtype=np.uint8)
+    at = int(lens[0]) // 2
+    vc[tables[0, at // BS], 1, 0, orc.scale_place(D, at % 16, 0, True)] = 255
+    q, qv = _cast(rng.standard_normal((B, Hq, D)), dtype)
+    out = ops.paged_decode_kv4(q, *(torch.from_numpy(a).cuda() for a in (kc, vc, tables)),
+                               torch.tensor(lens, dtype=torch.int32, device=device), longest)
+    nan = torch.isnan(out).cpu().numpy()
+    assert nan[0, G:2 * G, :32].all() and nan.sum() == G * 32
+    pick = [1, 2, B // 3, B // 2, B - 2, B - 1]
+    want, size, big = _attend_all([qv[i:i + 1] for i in pick], kc, vc, tables[pick], [int(lens[i]) for i in pick], D ** -0.5,
+                                  [[int(lens[i]) - 1] for i in pick])
+    _near(out[pick], want, _attention_bound(size, big, want, D, longest, dtype))
+    want, size, big = _attend_all([qv[:1, :G]], kc[:, :1], vc[:, :1], tables[:1], [int(lens[0])], D ** -0.5, [[int(lens[0]) - 1]])
+    _near(out[:1, :G], want, _attention_bound(size, big, want, D, longest, dtype))
+
+
 def test_decode_scale_out_and_strided_caches(ops, device):
     """A layer's caches as a slice of one pool with heads of another order, a scale of either sign, out=."""
     rng = np.random.default_rng(8)

@@ -280,12 +280,18 @@ int make_plan(const char* what, int B, int Hq, int Hkv, int D, int max_ctx, int 
   pl->gc = std::min(G, 16);
   pl->qchunks = (G + 15) / 16;
   // kv heads per wave: more of them share a step's softmax and read longer runs of a block, but make fewer, longer
-  // workgroups.  `units` counts (kv head, 128 tokens) pieces of the whole call.  256 x 2048: 61 / 56 / 53.7 with 1 / 2 / 4
-  // heads; 16 x 4000: 14.7 / 14.4 / 14.5; 32 x 1000: 9.0 / 11.3.  The accumulators of NH heads take NH D / 2 registers:
-  // NH D <= 256 leaves room for two waves per SIMD.
-  const int64_t rounds128 = ((int64_t)max_ctx + 127) / 128, units = (int64_t)std::max(B, 1) * Hkv * pl->qchunks * rounds128;
+  // workgroups.  Where there is one (sequence, kv head) per CU or more, as many as leave a workgroup per CU: 256 x 2048
+  // 61 / 56 / 53.7 with 1 / 2 / 4 heads, 64 x 2048 19.0 / 18.2 / 21.0, 64 x 4096 at head_dim 32 30.4 / 20.9 / 23.3, 32 x 4000 at
+  // head_dim 128 27.9 / 29.8.  Below that the context is split all the same, and long ones (in `units` of a kv head's 128
+  // tokens) make up for the longer steps: 8 x 30000 33.3 / 30.7 / 31.9, 16 x 4000 14.8 / 15.7 / 15.7, 16 x 16000 at head_dim
+  // 32, fp32, 34.6 / 25.7 / 23.8, 4 to 65536, 32/8 heads of 128, fp16, 46.1 / 45.1.  The accumulators of NH heads take
+  // NH D / 2 registers: NH D <= 256 leaves room for two waves per SIMD.
+  const int64_t heads = (int64_t)std::max(B, 1) * Hkv * pl->qchunks, units = heads * (((int64_t)max_ctx + 127) / 128);
+  auto more = [&](int nh) {   // whether 2 nh heads are better than nh
+    return heads < 256 ? units >= (int64_t)128 * D * nh : heads / (2 * nh) >= 256 && units >= (int64_t)4096 * nh;
+  };
   pl->NH = 1;
-  while (pl->NH * 2 <= 256 / D && pl->NH * 2 * pl->gc <= 16 && Hkv % (pl->NH * 2) == 0 && units >= 4096 * pl->NH) pl->NH *= 2;
+  while (pl->NH * 2 <= 256 / D && pl->NH * 2 * pl->gc <= 16 && Hkv % (pl->NH * 2) == 0 && more(pl->NH)) pl->NH *= 2;
   pl->hgroups = Hkv / pl->NH;
   const int64_t groups = (int64_t)std::max(B, 1) * pl->hgroups * pl->qchunks;
   // More workgroups than the chip's 256 CUs: four waves each.  Fewer: eight waves each as long as that leaves a wave few
