@@ -123,7 +123,7 @@ REFUSED = (
     [('mi355_rope_kv4_write', WRITE, c, r) for c, r in CACHE + [
         (dict(q_out=None), -1), (dict(q=None), -1), (dict(k=None), -1), (dict(v=None), -1), (dict(slots=None), -1),
         (dict(ks=504), -1), (dict(vs=1540), -1), (dict(k=P + 2), -1), (dict(Hq=0), -1), (dict(R=24), -1), (dict(cos=None), -1),
-        (dict(T=-3), -1), (dict(T=LONG), -1), (dict(q_out=P), -1), (dict(k=OUT + 2048), -1), (dict(v=OUT - 3 * 3072 - 512), -1)]] +
+        (dict(T=-3), -1), (dict(T=LONG), -1), (dict(q_out=P), -1), (dict(k=OUT + 2048), -1), (dict(v=OUT - 3 * 2 * 1536 - 512), -1)]] +
     [('mi355_kv4_read_slots', READ, c, r) for c, r in CACHE + [
         (dict(ko=None), -1), (dict(vo=P + 8), -1), (dict(slots=None), -1), (dict(T=-1), -1), (dict(T=LONG), -1)]] +
     [('mi355_paged_decode_kv4', DECODE, c, r) for c, r in CACHE + [
