@@ -24,17 +24,12 @@ _DTYPES = {'bf16': torch.bfloat16, 'fp16': torch.float16, 'fp32': torch.float32}
 _MAGNITUDES = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
 
 
-_module = None
-
-
 def _ops():
-    """The framework's operators, imported once, as a program that uses them would."""
-    global _module
-    if _module is None:
-        sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), 'vllm-from-scratch_amd'))
-        from mi355_paged import ops
-        _module = ops
-    return _module
+    pkg = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), 'vllm-from-scratch_amd')
+    if pkg not in sys.path:
+        sys.path.insert(0, pkg)
+    from mi355_paged import ops
+    return ops
 
 
 # ---------------------------------------------------------------------------------------------- cases
