@@ -631,6 +631,53 @@ def test_chunk_nan_reaches_only_the_queries_that_see_it(ops, device):
     _near(torch.where(torch.isnan(out), torch.zeros_like(out), out), np.where(expect, 0.0, want), np.where(expect, 1.0, bound))
 
 
+# ------------------------------------------------------------------ slots nobody wrote
+def _unwritten(rng_seed, lens, Hkv, D, BS):
+    """A cache as _cache makes it, and which of its bytes belong to rows nobody wrote."""
+    kc, vc, tables = _cache(np.random.default_rng(rng_seed), lens, Hkv, D, BS, fill=255)
+    k0, v0, _ = _cache(np.random.default_rng(rng_seed), lens, Hkv, D, BS, fill=0)
+    return kc, vc, tables, kc != k0, vc != v0
+
+
+@pytest.mark.parametrize('dtype', ALL)
+@pytest.mark.parametrize('Hq,Hkv,D,BS,lens,pos0', [
+    (32, 8, 128, 16, [300, 290, 300, 300], [0, 0, 11, 0]), (8, 8, 64, 16, [2047, 2040] * 4, [0] * 8),
+    (8, 8, 32, 16, [2047, 2041] * 4, [0] * 8), (8, 8, 256, 16, [250, 249, 251] * 3, [0] * 9), (8, 8, 64, 16, [400] * 15 + [33], [0] * 16),
+    (8, 8, 64, 32, [512, 511] * 4, [301] * 8), (32, 8, 128, 16, [256, 250, 256], [1601, 1607, 0]), (4, 2, 32, 48, [7, 1], [90, 3]),
+    (4, 2, 64, 16, [5, 40], [7000, 2500])], ids=lambda v: str(v)[:40])
+def test_chunks_do_not_depend_on_unwritten_slots(ops, device, dtype, Hq, Hkv, D, BS, lens, pos0):
+    """Contexts that end inside a tile, behind it every kind of scale byte: 0, the two that no append writes and whose
+    values pass the largest bf16 (253, 254), NaN."""
+    total = [n + p for n, p in zip(lens, pos0)]
+    kc, vc, tables, free_k, free_v = _unwritten(sum(lens) + D, total, Hkv, D, BS)
+    tables = torch.from_numpy(np.minimum(tables, len(kc) - 1)).cuda()
+    q, _ = _cast(np.random.default_rng(1).standard_normal((sum(lens), Hq, D)), dtype)
+    meta = torch.tensor([np.cumsum([0] + lens)[:-1].tolist(), lens, pos0], dtype=torch.int32, device=device)
+    want = None
+    for fill in (0, 253, 254, 255):
+        kc[free_k], vc[free_v] = fill, fill
+        out = ops.paged_prefill_kv4(q, torch.from_numpy(kc).cuda(), torch.from_numpy(vc).cuda(), tables, meta[0], meta[1], meta[2],
+                                    max(lens), max(total))
+        want = out if want is None else want
+        assert torch.isfinite(out).all() and torch.equal(out, want), fill
+
+
+@pytest.mark.parametrize('dtype', ALL)
+@pytest.mark.parametrize('Hq,Hkv,D,BS,lens', [(8, 8, 64, 16, [1, 15, 18, 333]), (32, 8, 128, 16, [257, 50]), (4, 4, 32, 32, [5, 700, 41]),
+                                              (8, 4, 256, 16, [20, 77]), (4, 2, 64, 48, [9001, 130])], ids=lambda v: str(v)[:40])
+def test_decode_does_not_depend_on_unwritten_slots(ops, device, dtype, Hq, Hkv, D, BS, lens):
+    kc, vc, tables, free_k, free_v = _unwritten(sum(lens) + D, lens, Hkv, D, BS)
+    tables = torch.from_numpy(np.minimum(tables, len(kc) - 1)).cuda()
+    q, _ = _cast(np.random.default_rng(1).standard_normal((len(lens), Hq, D)), dtype)
+    want = None
+    for fill in (0, 253, 254, 255):
+        kc[free_k], vc[free_v] = fill, fill
+        out = ops.paged_decode_kv4(q, torch.from_numpy(kc).cuda(), torch.from_numpy(vc).cuda(), tables,
+                                   torch.tensor(lens, dtype=torch.int32, device=device), max(lens))
+        want = out if want is None else want
+        assert torch.isfinite(out).all() and torch.equal(out, want), fill
+
+
 # ------------------------------------------------------------------ streams, graphs, all of them together
 def _step(ops, s):
     """One layer's work on new rows: angles, rotation + append, attention."""

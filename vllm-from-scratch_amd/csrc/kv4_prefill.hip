@@ -221,7 +221,8 @@ __global__ void __launch_bounds__(256, 2) kv4_prefill_kernel(const Kv4PrefillPar
       for (int b = 0; b < NB; ++b) nan[b] = 0;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int live = wg_last + 1 - (t0 + vstep * kKv4Step + i * kKv4Tile + 4 * g);   // of this lane's four tokens
+        // (of this lane's four tokens: those of the record's order, whatever the number of columns)
+        const int live = wg_last + 1 - (t0 + vstep * kKv4Step + i * kKv4Tile + 4 * (lane >> 4));
         const uint32_t keep = live >= 4 ? ~0u : (live <= 0 ? 0u : (1u << (8 * live)) - 1u);
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
