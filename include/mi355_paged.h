@@ -504,8 +504,8 @@ int mi355_kv4_read_slots(void* k_out, void* v_out, const void* k_cache, const vo
  * mi355_paged_decode over the 4-bit cache: same arguments and meaning (out, q [B, Hq, D], tables,
  * context_lens clamped to min(max_context, max_blocks * block_size), 0 gives zeros, ids clamped into
  * the pool) but for the cache's strides.  Scores, softmax and sums are fp32; the cached values and
- * the queries enter the products exactly, the softmax weights with 8 / 16 / 24 bits for bf16 / fp16 /
- * fp32 queries.
+ * the queries enter the products exactly, the softmax weights with 16 bits for bf16 and fp16 queries
+ * and with 24 for fp32 ones.
  */
 int mi355_paged_decode_kv4(void* out, const void* q, int64_t q_stride_seq, const void* k_cache,
                            const void* v_cache, const int32_t* block_tables, const int32_t* context_lens,

@@ -678,6 +678,82 @@ def test_decode_does_not_depend_on_unwritten_slots(ops, device, dtype, Hq, Hkv, 
         assert torch.isfinite(out).all() and torch.equal(out, want), fill
 
 
+# ------------------------------------------------------------------ the weights' bits
+def _close_bound(size, big, want, D, n, dtype):
+    """_attention_bound with the 16 bits that a weight has at least: two pieces leave out 2^-16 of it, and as much may be
+    missing from the sum of weights."""
+    return (2 * (3 * D + 8) * U * big + 2.0 ** -22 + 2 * (n + 8) * U + 2.0 ** -15) * size + \
+        (HALF[dtype] + 2 * (n + 8) * U) * np.abs(want) + 1e-30
+
+
+@pytest.mark.parametrize('dtype', ALL)
+@pytest.mark.parametrize('Hq,Hkv,D,lens', [(8, 8, 64, [37, 700]), (32, 8, 128, [300]), (4, 4, 32, [90, 1025]), (8, 4, 256, [50]), (4, 2, 64, [5000])],
+                         ids=lambda v: str(v))
+def test_decode_rounds_the_result_not_the_weights(ops, device, dtype, Hq, Hkv, D, lens):
+    rng = np.random.default_rng(D + sum(lens))
+    kc, vc, tables = _cache(rng, lens, Hkv, D, 16)
+    B = len(lens)
+    q, qv = _cast(rng.standard_normal((B, Hq, D)), dtype)
+    want, size, big = _attend_all([qv[i:i + 1] for i in range(B)], kc, vc, tables, lens, D ** -0.5, [[n - 1] for n in lens])
+    out = ops.paged_decode_kv4(q, torch.from_numpy(kc).cuda(), torch.from_numpy(vc).cuda(), torch.from_numpy(tables).cuda(),
+                               torch.tensor(lens, dtype=torch.int32, device=device), max(lens))
+    _near(out, want, _close_bound(size, big, want, D, max(lens), dtype))
+
+
+@pytest.mark.parametrize('dtype', ALL)
+@pytest.mark.parametrize('Hq,Hkv,D,lens,pos0', [
+    (8, 8, 64, [3, 45], [0, 700]), (32, 8, 128, [300, 290, 300, 300], [0, 0, 11, 0]), (8, 8, 64, [2047, 2040] * 4, [0] * 8),
+    (8, 8, 64, [512, 500, 512, 512, 480, 512], [1300, 0, 1290, 1300, 1000, 1777]), (8, 8, 256, [250, 249, 251] * 3, [0] * 9),
+    (4, 4, 32, [130, 3], [0, 1000]), (8, 8, 128, [256, 250, 256] * 3, [0] * 9)], ids=lambda v: str(v)[:40])
+def test_chunks_round_the_result_not_the_weights(ops, device, dtype, Hq, Hkv, D, lens, pos0):
+    rng = np.random.default_rng(D + sum(lens))
+    total = [n + p for n, p in zip(lens, pos0)]
+    kc, vc, tables = _cache(rng, total, Hkv, D, 16)
+    start = [int(x) for x in np.cumsum([0] + lens)[:-1]]
+    q, qv = _cast(rng.standard_normal((sum(lens), Hq, D)), dtype)
+    meta = torch.tensor([start, lens, pos0], dtype=torch.int32, device=device)
+    out = ops.paged_prefill_kv4(q, *(torch.from_numpy(a).cuda() for a in (kc, vc, tables)), meta[0], meta[1], meta[2],
+                                max(lens), max(total))
+    pick = [sorted({0, n - 1} | set(rng.integers(0, n, min(n // 4, 12)).tolist())) for n in lens]
+    want, size, big = _attend_all([qv[[s + j for j in p]] for s, p in zip(start, pick)], kc, vc, tables, total, D ** -0.5,
+                                  [[p0 + j for j in p] for p0, p in zip(pos0, pick)])
+    rows = torch.tensor([s + j for s, p in zip(start, pick) for j in p]).cuda()
+    _near(out[rows], want, _close_bound(size, big, want, D, max(total), dtype))
+
+
+@pytest.mark.parametrize('dtype', ALL)
+@pytest.mark.parametrize('seqs,n,Hq,Hkv,D', [(2, 0, 8, 8, 64), (2, 0, 32, 8, 128), (1, 40, 8, 8, 64), (8, 1024, 8, 8, 64), (4, 512, 32, 8, 128),
+                                             (9, 250, 8, 8, 256)])
+def test_equal_value_rows_come_back(ops, device, dtype, seqs, n, Hq, Hkv, D):
+    """All value rows 1.5, scores of 2^-6 q0 up to one token's 2^6 q0, far behind the others: its weight has all its bits and
+    stands beside a maximum of an earlier token.  1.5 (1 +- 2^-12) rounds to 1.5 in 8 and in 11 bits; in fp32 the numerator
+    and the sum of weights are sums of n terms of one sign, each off by at most n u of itself, and their quotient by one
+    rounding more: 1.5 * 2 (n + 8) u = 1.9e-4 for n = 1024 (2^-15 of the weights and these stay below 2^-12)."""
+    rng = np.random.default_rng(n + D)
+    ctx = max(n, 600)
+    code = np.full((seqs, Hkv, -(-ctx // 16), 16, D), 3, dtype=np.uint8)                 # 1.5
+    byte = np.full(code.shape[:-1] + (D // 32,), 127, dtype=np.uint8)
+    vc = orc.pack(code, byte, True).reshape(-1, 1, 17 * D // 2)
+    code[...] = 0
+    code[..., 0] = 15                                                                    # -6
+    code[:, :, 0, :, 0], code[:, :, 18, 9, 0] = 0, 7                                     # the first tile 0, position 297: 6
+    kc = orc.pack(code, byte, False).reshape(-1, 1, 17 * D // 2)
+    blocks = -(-ctx // 16)
+    kc, vc = (torch.from_numpy(np.ascontiguousarray(a.reshape(seqs, Hkv, blocks, -1).transpose(0, 2, 1, 3)).reshape(seqs * blocks, Hkv, 1, -1)).cuda()
+              for a in (kc, vc))
+    tables = torch.arange(seqs * blocks, dtype=torch.int32, device=device).view(seqs, blocks)
+    rows = seqs * max(n, 1)
+    x = np.zeros((rows, Hq, D))
+    x[..., 0] = rng.uniform(0.2, 1.3, (rows, Hq))
+    q, _ = _cast(x, dtype)
+    if n == 0:
+        out = ops.paged_decode_kv4(q, kc, vc, tables, torch.full((seqs,), ctx, dtype=torch.int32, device=device), ctx, scale=math.log(2.0))
+    else:
+        meta = torch.tensor([[i * n for i in range(seqs)], [n] * seqs, [ctx - n] * seqs], dtype=torch.int32, device=device)
+        out = ops.paged_prefill_kv4(q, kc, vc, tables, meta[0], meta[1], meta[2], n, ctx, scale=math.log(2.0))
+    _near(out, np.full(x.shape, 1.5), 1.5 * 2 * (ctx + 8) * U if dtype == torch.float32 else 0.0)
+
+
 # ------------------------------------------------------------------ streams, graphs, all of them together
 def _step(ops, s):
     """One layer's work on new rows: angles, rotation + append, attention."""

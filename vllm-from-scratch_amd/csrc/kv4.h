@@ -150,14 +150,18 @@ __device__ __forceinline__ void bf16_pieces(const float (&x)[8], bf16x8_t (&out)
   }
 }
 
+// Pieces of a query (all of its bits) and of a softmax weight.  A weight takes two at least: in one piece the rows of bf16
+// queries move by as much as their own rounding does (1.7e-3 of a row from the exact one, 2.3e-3 in one piece); in two
+// they move by 2^-17.  The second piece costs 4 x 2048 rows behind 2048, 32/8 heads of 128, 540 us for 409, and decode,
+// which memory bounds, under 1 %.
 template <class Tag>
 struct Kv4Pieces;
 template <>
-struct Kv4Pieces<BF16> { static constexpr int n = 1; };
+struct Kv4Pieces<BF16> { static constexpr int n = 1, weights = 2; };
 template <>
-struct Kv4Pieces<F16> { static constexpr int n = 2; };
+struct Kv4Pieces<F16> { static constexpr int n = 2, weights = 2; };
 template <>
-struct Kv4Pieces<F32> { static constexpr int n = 3; };
+struct Kv4Pieces<F32> { static constexpr int n = 3, weights = 3; };
 
 // Eight consecutive elements of a row (16-byte aligned) as floats, and back with one rounding.
 template <class Tag>

@@ -34,7 +34,7 @@ struct Kv4DecodeParams {
 
 template <class Tag, int D, int NH, int W>
 __global__ void __launch_bounds__(W * 64) kv4_decode_kernel(const Kv4DecodeParams p) {
-  constexpr int NP = Kv4Pieces<Tag>::n, KS = D / 32, EB = Tag::kBytes;
+  constexpr int NP = Kv4Pieces<Tag>::n, NW = Kv4Pieces<Tag>::weights, KS = D / 32, EB = Tag::kBytes;
   __shared__ float s_o[W][16][D + 4];
   __shared__ float s_m[W][16], s_l[W][16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -177,10 +177,10 @@ __global__ void __launch_bounds__(W * 64) kv4_decode_kernel(const Kv4DecodeParam
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = fast_exp2(__builtin_fmaf(x[e], p.scale2, -m2));
-    bf16x8_t pf[NP];
-    bf16_pieces<NP>(x, pf);
+    bf16x8_t pf[NW];
+    bf16_pieces<NW>(x, pf);
 #pragma unroll
-    for (int n = 0; n < NP; ++n) sum = mfma_bf16(ones, pf[n], sum);   // every row: the column's sum of weights
+    for (int n = 0; n < NW; ++n) sum = mfma_bf16(ones, pf[n], sum);   // every row: the column's sum of weights
 #pragma unroll
     for (int j = 0; j < NH; ++j)
 #pragma unroll
@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(W * 64) kv4_decode_kernel(const Kv4DecodeParam
         bf16x8_t ev, od;
         kv4_v_frags(T[j][0].v[s], T[j][1].v[s], T[j][0].vs[s], T[j][1].vs[s], ev, od);
 #pragma unroll
-        for (int n = 0; n < NP; ++n) {
+        for (int n = 0; n < NW; ++n) {
           acc[j][s][0] = mfma_bf16(ev, pf[n], acc[j][s][0]);
           acc[j][s][1] = mfma_bf16(od, pf[n], acc[j][s][1]);
         }

@@ -120,7 +120,8 @@ template <class Tag, int D, int COLS>
 __global__ void __launch_bounds__(256, 2) kv4_prefill_kernel(const Kv4PrefillParams p) {
   typedef Stage<D> St;
   typedef Layout<COLS> Lay;
-  constexpr int NP = Kv4Pieces<Tag>::n, KS = D / 32, EB = Tag::kBytes, SUB = St::SUB, NB = St::NB, KT = St::KT, KF = St::KF;
+  constexpr int NP = Kv4Pieces<Tag>::n, NW = Kv4Pieces<Tag>::weights, KS = D / 32, EB = Tag::kBytes;
+  constexpr int SUB = St::SUB, NB = St::NB, KT = St::KT, KF = St::KF;
   constexpr int KA = KS < 4 ? KS : 4, VA = KS < 2 ? KS : 2;   // operands read ahead of their use
   constexpr int TOK = Lay::kTok, NQ = Lay::kQ, QF = KS * NQ;
   __shared__ bf16x8_t s_k[2][SUB][2 * KS * 64], s_v[2][SUB][KS][2 * 64];
@@ -338,14 +339,14 @@ __global__ void __launch_bounds__(256, 2) kv4_prefill_kernel(const Kv4PrefillPar
 #pragma unroll
             for (auto& a : acc[s]) a *= f;
         }
-        bf16x8_t pf[NQ][NP];
+        bf16x8_t pf[NQ][NW];
 #pragma unroll
         for (int e = 0; e < TOK; ++e) {
           x[e] = fast_exp2(__builtin_fmaf(x[e], p.scale2, -m2));
           sum += x[e];
         }
 #pragma unroll
-        for (int n = 0; n < NQ; ++n) bf16_pieces<NP>(*reinterpret_cast<const float(*)[8]>(&x[8 * n]), pf[n]);
+        for (int n = 0; n < NQ; ++n) bf16_pieces<NW>(*reinterpret_cast<const float(*)[8]>(&x[8 * n]), pf[n]);
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
           const bf16x8_t a0 = vf[s % VA][0], a1 = vf[s % VA][1];
@@ -354,7 +355,7 @@ __global__ void __launch_bounds__(256, 2) kv4_prefill_kernel(const Kv4PrefillPar
             vf[s % VA][1] = s_v[buf][sub][s + VA][64 + lane];
           }
 #pragma unroll
-          for (int n = 0; n < NP; ++n) {
+          for (int n = 0; n < NW; ++n) {
             if constexpr (COLS == 16) {
               acc[s][0] = mfma_bf16(a0, pf[0][n], acc[s][0]);
               acc[s][1] = mfma_bf16(a1, pf[0][n], acc[s][1]);
@@ -394,7 +395,7 @@ __global__ void __launch_bounds__(256, 2) kv4_prefill_kernel(const Kv4PrefillPar
 // The queries wait in LDS, where the waves' sums meet at the end.
 template <class Tag, int D, int CT, int W>
 __global__ void __launch_bounds__(W * 64, 2) kv4_rows_kernel(const Kv4PrefillParams p) {
-  constexpr int NP = Kv4Pieces<Tag>::n, KS = D / 32, EB = Tag::kBytes, QF = 2 * KS;
+  constexpr int NP = Kv4Pieces<Tag>::n, NW = Kv4Pieces<Tag>::weights, KS = D / 32, EB = Tag::kBytes, QF = 2 * KS;
   constexpr int QD = QF < 4 ? QF : NP == 1 && D < 256 && CT == 1 ? 4 : 2;   // query operands read ahead
   constexpr int VB = KS > 1 ? KS / 2 : 1;            // value blocks per lane
   constexpr int NT = KS > 1 ? 2 * VB : 1;            // 32-row tiles of the output
@@ -580,7 +581,7 @@ __global__ void __launch_bounds__(W * 64, 2) kv4_rows_kernel(const Kv4PrefillPar
     }
     fetch_k(w, r0, r1);
     place(min(t0 + (SETS + 1) * kStride, wg_last));
-    bf16x8_t pf[CT][2][NP];
+    bf16x8_t pf[CT][2][NW];
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
       if (masked) {
@@ -609,7 +610,7 @@ __global__ void __launch_bounds__(W * 64, 2) kv4_rows_kernel(const Kv4PrefillPar
           x[e] = fast_exp2(__builtin_fmaf(S[ct][8 * n + e], p.scale2, -m2[ct]));
           sum[ct] += x[e];
         }
-        bf16_pieces<NP>(x, pf[ct][n]);
+        bf16_pieces<NW>(x, pf[ct][n]);
       }
     }
 #pragma unroll
@@ -622,7 +623,7 @@ __global__ void __launch_bounds__(W * 64, 2) kv4_rows_kernel(const Kv4PrefillPar
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
-          for (int n = 0; n < NP; ++n) {
+          for (int n = 0; n < NW; ++n) {
             acc[ct][NT > 1 ? 2 * b : 0] = mfma32_bf16(ev, pf[ct][q][n], acc[ct][NT > 1 ? 2 * b : 0]);
             if constexpr (NT > 1) acc[ct][2 * b + 1] = mfma32_bf16(od, pf[ct][q][n], acc[ct][2 * b + 1]);
           }
