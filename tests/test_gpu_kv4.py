@@ -754,6 +754,79 @@ def test_equal_value_rows_come_back(ops, device, dtype, seqs, n, Hq, Hkv, D):
     _near(out, np.full(x.shape, 1.5), 1.5 * 2 * (ctx + 8) * U if dtype == torch.float32 else 0.0)
 
 
+# ------------------------------------------------------------------ extremes of scores and values
+FORMS = [   # sequences, query rows each (0: decode), Hq, Hkv, D, context: each way rows and contexts are cut up
+    (3, 0, 8, 8, 64, 600), (2, 0, 8, 2, 128, 9000), (70, 0, 8, 8, 64, 700), (1, 40, 8, 8, 64, 600), (1, 9, 8, 2, 128, 6000), (8, 512, 8, 8, 64, 812),
+    (8, 1024, 8, 8, 64, 1024), (4, 512, 32, 8, 128, 600), (9, 250, 8, 8, 256, 600)]
+
+
+def _attend_form(ops, form, dtype, key, value, scale):
+    """Output [sequences, rows, Hq, D] (float64) of queries of ones whose cached rows have the values key(t) in their dim 0
+    and value(t) in all dims; codes and scale bytes given as (code, byte) arrays over the positions."""
+    seqs, n, Hq, Hkv, D, ctx = form
+    blocks = -(-ctx // 16)
+    caches = []
+    for (code, byte), dims, last in ((key, 1, False), (value, D, True)):
+        c, b = np.zeros((blocks * 16, D), dtype=np.uint8), np.full((blocks * 16, D // 32), 127, dtype=np.uint8)
+        c[:ctx, :dims], b[:ctx] = code[:, None], byte[:, None]
+        rec = orc.pack(c.reshape(blocks, 16, D), b.reshape(blocks, 16, D // 32), last)
+        caches.append(torch.from_numpy(rec).cuda()[:, None, None].expand(-1, Hkv, 1, -1).contiguous())
+    order = torch.from_numpy(np.stack([np.arange(blocks)] * seqs).astype(np.int32)).cuda()
+    rows = seqs * max(n, 1)
+    q = torch.zeros((rows, Hq, D), dtype=dtype, device='cuda')
+    q[..., 0] = 1.0
+    if n == 0:
+        out = ops.paged_decode_kv4(q, *caches, order, torch.full((seqs,), ctx, dtype=torch.int32, device='cuda'), ctx, scale=scale)
+    else:
+        meta = torch.tensor([[i * n for i in range(seqs)], [n] * seqs, [ctx - n] * seqs], dtype=torch.int32, device='cuda')
+        out = ops.paged_prefill_kv4(q, *caches, order, meta[0], meta[1], meta[2], n, ctx, scale=scale)
+    return out.double().cpu().numpy().reshape(seqs, max(n, 1), Hq, D)
+
+
+@pytest.mark.parametrize('dtype', ALL)
+@pytest.mark.parametrize('form', FORMS, ids=str)
+@pytest.mark.parametrize('scale', [1e9, 3e11, -3e11])
+def test_scores_far_beyond_the_range_of_an_exponential(ops, device, dtype, form, scale):
+    """Scores of 10^9 and more, where a float's last bit is far more than one power of two: the two positions that share the
+    largest one share the weight, whatever step, wave or split they are in; nothing else has any."""
+    ctx = form[5]
+    n = max(form[1], 1)
+    key = np.full(ctx, 1 if scale > 0 else 9, dtype=np.uint8)              # 0.5 (-0.5 under a negative scale)
+    key[1], key[ctx - n - 2 if ctx > n + 3 else 2] = (7, 7) if scale > 0 else (15, 15)      # 6 (-6)
+    code = np.where(np.arange(ctx) % 2 == 0, 2, 4).astype(np.uint8)        # 1 and 2
+    value = np.array([1.0, 2.0])[np.arange(ctx) % 2]
+    out = _attend_form(ops, form, dtype, (key, np.full(ctx, 127, dtype=np.uint8)), (code, np.full(ctx, 127, dtype=np.uint8)), scale)
+    top = key == key[1]
+    for j in range(n):
+        seen = top & (np.arange(ctx) <= ctx - n + j)
+        want = value[seen].mean() if seen.any() else value[0]
+        np.testing.assert_array_equal(out[:, j], want)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('form', FORMS, ids=str)
+def test_values_at_the_top_of_the_format(ops, device, dtype, form):
+    """Values of 6 * 2^125 under a score of almost 2^8 times the weight of the maximum before it, so that the maximum may
+    stay: the weighted mean is 6 * 2^125 (1 - small) and its sums stay below the largest float."""
+    ctx, n = form[5], max(form[1], 1)
+    key = np.zeros(ctx, dtype=np.uint8)
+    key[1:], key[ctx - n - 1 if ctx > n + 2 else 300] = 15, 7               # 0 at position 0, -6 elsewhere, 6 once
+    at = int(np.argmax(key == 7))
+    code = np.where(np.arange(ctx) == at, 7, 0).astype(np.uint8)
+    scale = 1.3 * math.log(2.0)                                             # weights 1, 2^-7.8 and 2^7.8
+    out = _attend_form(ops, form, dtype, (key, np.full(ctx, 127, dtype=np.uint8)), (code, np.full(ctx, 252, dtype=np.uint8)), scale)
+    weight = 2.0 ** (1.3 * np.array([0, -6, 6]))
+    for j in range(n):
+        m = ctx - n + j + 1
+        w = np.full(m, weight[1])
+        w[0] = weight[0]
+        if at < m:
+            w[at] = weight[2]
+        want = 6 * 2.0 ** 125 * (w[at] / w.sum() if at < m else 0.0)
+        bound = want * (HALF[dtype] + 2.0 ** -15 + 2 * 8 * 200 * U + 2.0 ** -22 + 4 * (m + 8) * U)
+        assert (np.abs(out[:, j] - want) <= bound).all(), (j, want, out[0, j, 0, 0])
+
+
 # ------------------------------------------------------------------ streams, graphs, all of them together
 def _step(ops, s):
     """One layer's work on new rows: angles, rotation + append, attention."""

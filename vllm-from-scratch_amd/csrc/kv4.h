@@ -31,7 +31,9 @@ constexpr int kKv4MaxContext = 1 << 29;   // positions are ints, and a step look
 constexpr int kKv4Step = 32;          // tokens per contraction step: two records
 constexpr int kKv4MinExp = -120, kKv4MaxExp = 125;
 constexpr float kKv4Floor = -3e38f;   // a running maximum no score has raised yet
-constexpr float kKv4Raise = 8.f;      // powers of two a score may pass the running maximum by before it is raised
+// Powers of two a score may pass the running maximum by before it is raised.  Weights are made as much smaller, 2^-8 at the
+// maximum: they stay at 1 or below, and values up to the largest that the format holds below the largest float.
+constexpr float kKv4Raise = 8.f;
 
 static inline bool kv4_dtype_ok(int dtype) { return dtype == MI355_F32 || dtype == MI355_BF16 || dtype == MI355_F16; }
 // A launch has fewer than 2^32 threads.
@@ -266,7 +268,15 @@ __device__ __forceinline__ float kv4_k_scale(const Kv4TileRegs<D>& t, const Kv4L
   return u2f(__builtin_amdgcn_alignbit(t.ks, t.ks, turn));
 }
 
-// Joins a row's `n` split records of D + 4 floats (unnormalised sums, running maximum, sum of weights)
+// The softmax weight of a score against a running maximum.  (The difference first: it is exact near the maximum however
+// large the two are, which the difference of their products with the scale is not -- 2^31 would be off by 2^7.)
+__device__ __forceinline__ float kv4_weight(float score, float m, float scale2) {
+  return fast_exp2(__builtin_fmaf(score - m, scale2, -kKv4Raise));
+}
+// What sums that belong to maximum `from` are worth under maximum `to`.
+__device__ __forceinline__ float kv4_shift(float from, float to, float scale2) { return fast_exp2((from - to) * scale2); }
+
+// Joins a row's `n` split records of D + 4 floats (unnormalised sums, running maximum of the raw scores, sum of weights)
 // and stores the row.  A thread owns eight dims and every SL-th split, SL * D / 8 threads a row; with
 // SL > 1 the row is the whole workgroup's (256 threads) and its threads of the same dims meet in LDS.
 // The records of a row lie a memory latency apart when one thread walks them (32 splits of 128 dims:
@@ -276,13 +286,13 @@ constexpr int kKv4WalkedSplits = 8;
 template <int D>
 constexpr int kv4_split_lanes(bool walked) { return walked ? 1 : 256 / (D / 8); }
 template <class Tag, int D, int SL>
-__device__ inline void kv4_join_splits(char* out, const float* ws, int n) {
+__device__ inline void kv4_join_splits(char* out, const float* ws, int n, float scale2) {
   constexpr int P = D / 8;
   __shared__ float s_m[SL][P], s_l[SL][P], s_o[SL][P][9];   // (9: neighbouring threads on neighbouring banks)
   const int piece = threadIdx.x % P, sl = SL == 1 ? 0 : threadIdx.x / P;
   float M = kKv4Floor, L = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   auto join = [&](float ms, float ls, const float (&x)[8]) {
-    const float Mn = fmaxf(M, ms), fo = fast_exp2(M - Mn), fn = fast_exp2(ms - Mn);
+    const float Mn = fmaxf(M, ms), fo = kv4_shift(M, Mn, scale2), fn = kv4_shift(ms, Mn, scale2);
     M = Mn;
     L = __builtin_fmaf(ls, fn, L * fo);
 #pragma unroll

@@ -70,7 +70,7 @@ __global__ void __launch_bounds__(W * 64) kv4_decode_kernel(const Kv4DecodeParam
   for (int j = 0; j < NH; ++j)
 #pragma unroll
     for (int s = 0; s < KS; ++s) acc[j][s][0] = acc[j][s][1] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float m = kKv4Floor, m2 = kKv4Floor;   // running maximum of the raw scores, and times the scale
+  float m = kKv4Floor;   // running maximum of the raw scores
   bf16x8_t ones;
 #pragma unroll
   for (int e = 0; e < 8; ++e) ones[e] = (__bf16)1.f;
@@ -163,9 +163,8 @@ __global__ void __launch_bounds__(W * 64) kv4_decode_kernel(const Kv4DecodeParam
     if (__ballot(top > m + p.raise)) {
       top = fmaxf(top, __shfl_xor(top, 16));
       top = fmaxf(top, __shfl_xor(top, 32));
-      const float mn = fmaxf(m, top), f = fast_exp2((m - mn) * p.scale2);
+      const float mn = fmaxf(m, top), f = kv4_shift(m, mn, p.scale2);
       m = mn;
-      m2 = fmaxf(mn * p.scale2, kKv4Floor);
       sum *= f;
 #pragma unroll
       for (int j = 0; j < NH; ++j)
@@ -176,7 +175,7 @@ __global__ void __launch_bounds__(W * 64) kv4_decode_kernel(const Kv4DecodeParam
         }
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = fast_exp2(__builtin_fmaf(x[e], p.scale2, -m2));
+    for (int e = 0; e < 8; ++e) x[e] = kv4_weight(x[e], m, p.scale2);
     bf16x8_t pf[NW];
     bf16_pieces<NW>(x, pf);
 #pragma unroll
@@ -198,7 +197,7 @@ __global__ void __launch_bounds__(W * 64) kv4_decode_kernel(const Kv4DecodeParam
 
   // the lane's column: dims 32 s + 8 g .. + 8 (even and odd rows of the two accumulators alternate)
   if (g == 0) {
-    s_m[wave][col] = m2;
+    s_m[wave][col] = m;
     s_l[wave][col] = sum[0];
   }
 #pragma unroll
@@ -229,7 +228,7 @@ __global__ void __launch_bounds__(W * 64) kv4_decode_kernel(const Kv4DecodeParam
     float L = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int w = 0; w < W; ++w) {
-      const float f = fast_exp2(s_m[w][c] - M);
+      const float f = kv4_shift(s_m[w][c], M, p.scale2);
       L = __builtin_fmaf(s_l[w][c], f, L);
 #pragma unroll
       for (int e = 0; e < 8; ++e) o[e] = __builtin_fmaf(s_o[w][c][d + e], f, o[e]);
@@ -251,18 +250,19 @@ __global__ void __launch_bounds__(W * 64) kv4_decode_kernel(const Kv4DecodeParam
 
 template <class Tag, int D, int SL>
 __global__ void __launch_bounds__(256)
-kv4_merge_kernel(char* out, const float* ws, const int32_t* ctx_lens, int rows, int Hq, int max_ctx, int nsplit, int tps) {
+kv4_merge_kernel(char* out, const float* ws, const int32_t* ctx_lens, int rows, int Hq, int max_ctx, int nsplit, int tps,
+                 float scale2) {
   const int64_t row = (int64_t)blockIdx.x * (256 / (SL * D / 8)) + (SL == 1 ? threadIdx.x / (D / 8) : 0);
   if (row >= rows) return;
   const int ctx = min(ctx_lens[row / Hq], max_ctx);
   kv4_join_splits<Tag, D, SL>(out + row * D * Tag::kBytes, ws + row * nsplit * (D + 4),
-                              ctx <= 0 ? 0 : min(nsplit, (ctx + tps - 1) / tps));
+                              ctx <= 0 ? 0 : min(nsplit, (ctx + tps - 1) / tps), scale2);
 }
 template <class Tag, int D, int SL>
 void launch_merge(const Kv4DecodeParams& p, hipStream_t s) {
   const int rows = p.B * p.Hq;
   hipLaunchKernelGGL((kv4_merge_kernel<Tag, D, SL>), dim3((unsigned)ceil_div64(rows, 256 / (SL * D / 8))), dim3(256), 0, s,
-                     p.out, p.ws, p.ctx, rows, p.Hq, p.max_ctx, p.nsplit, p.tps);
+                     p.out, p.ws, p.ctx, rows, p.Hq, p.max_ctx, p.nsplit, p.tps, p.scale2);
 }
 
 struct Kv4Plan {

@@ -162,8 +162,8 @@ __global__ void __launch_bounds__(256, 2) kv4_prefill_kernel(const Kv4PrefillPar
   const int wave_last = row0 < rows ? limit(row0 + COLS - 1) : -1;
 
   typename Lay::sums_t acc[KS];
-  float m = kKv4Floor, m2 = kKv4Floor;   // running maximum of the raw scores, and times the scale
-  float sum = 0.f;                       // of the lane's weights
+  float m = kKv4Floor;   // running maximum of the raw scores
+  float sum = 0.f;       // of the lane's weights
 #pragma unroll
   for (int s = 0; s < KS; ++s)
 #pragma unroll
@@ -330,9 +330,8 @@ __global__ void __launch_bounds__(256, 2) kv4_prefill_kernel(const Kv4PrefillPar
         if (__ballot(top > m + p.raise)) {
           if constexpr (COLS == 16) top = fmaxf(top, __shfl_xor(top, 16));
           top = fmaxf(top, __shfl_xor(top, 32));
-          const float mn = fmaxf(m, top), f = fast_exp2((m - mn) * p.scale2);
+          const float mn = fmaxf(m, top), f = kv4_shift(m, mn, p.scale2);
           m = mn;
-          m2 = fmaxf(mn * p.scale2, kKv4Floor);
           sum *= f;
 #pragma unroll
           for (int s = 0; s < KS; ++s)
@@ -342,7 +341,7 @@ __global__ void __launch_bounds__(256, 2) kv4_prefill_kernel(const Kv4PrefillPar
         bf16x8_t pf[NQ][NW];
 #pragma unroll
         for (int e = 0; e < TOK; ++e) {
-          x[e] = fast_exp2(__builtin_fmaf(x[e], p.scale2, -m2));
+          x[e] = kv4_weight(x[e], m, p.scale2);
           sum += x[e];
         }
 #pragma unroll
@@ -441,10 +440,10 @@ __global__ void __launch_bounds__(W * 64, 2) kv4_rows_kernel(const Kv4PrefillPar
   }
 
   f32x16 acc[CT][NT];
-  float m[CT], m2[CT], sum[CT];   // running maximum of the raw scores, and times the scale; sum of the lane's weights
+  float m[CT], sum[CT];   // running maximum of the raw scores; sum of the lane's weights
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
-    m[ct] = m2[ct] = kKv4Floor;
+    m[ct] = kKv4Floor;
     sum[ct] = 0.f;
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[ct][j] = 0.f;
@@ -595,9 +594,8 @@ __global__ void __launch_bounds__(W * 64, 2) kv4_rows_kernel(const Kv4PrefillPar
       top = fmaxf(top, S[ct][15]);
       if (__ballot(top > m[ct] + p.raise)) {
         top = fmaxf(top, __shfl_xor(top, 32));
-        const float mn = fmaxf(m[ct], top), f = fast_exp2((m[ct] - mn) * p.scale2);
+        const float mn = fmaxf(m[ct], top), f = kv4_shift(m[ct], mn, p.scale2);
         m[ct] = mn;
-        m2[ct] = fmaxf(mn * p.scale2, kKv4Floor);
         sum[ct] *= f;
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[ct][j] *= f;
@@ -607,7 +605,7 @@ __global__ void __launch_bounds__(W * 64, 2) kv4_rows_kernel(const Kv4PrefillPar
         float x[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          x[e] = fast_exp2(__builtin_fmaf(S[ct][8 * n + e], p.scale2, -m2[ct]));
+          x[e] = kv4_weight(S[ct][8 * n + e], m[ct], p.scale2);
           sum[ct] += x[e];
         }
         bf16_pieces<NW>(x, pf[ct][n]);
@@ -671,7 +669,7 @@ __global__ void __launch_bounds__(W * 64, 2) kv4_rows_kernel(const Kv4PrefillPar
             store8<F32>(reinterpret_cast<char*>(row + (blk * 32) % kPart + 16 * bl + 8 * g), x);
           }
         }
-      if (g == 0) *reinterpret_cast<f32x4*>(row + kPart) = f32x4{m2[ct], total, 0.f, 0.f};
+      if (g == 0) *reinterpret_cast<f32x4*>(row + kPart) = f32x4{m[ct], total, 0.f, 0.f};
       __syncthreads();
       for (int item = threadIdx.x; item < 32 * P; item += W * 64) {
         const int cc = item / P, d = item % P * 8, r = row0 + ct * 32 + cc;
@@ -682,7 +680,7 @@ __global__ void __launch_bounds__(W * 64, 2) kv4_rows_kernel(const Kv4PrefillPar
         for (int w = 0; w < W; ++w) M = fmaxf(M, rec[w * 32 * kRow + kPart]);
 #pragma unroll
         for (int w = 0; w < W; ++w) {
-          const float f = fast_exp2(rec[w * 32 * kRow + kPart] - M);
+          const float f = kv4_shift(rec[w * 32 * kRow + kPart], M, p.scale2);
           L = __builtin_fmaf(rec[w * 32 * kRow + kPart + 1], f, L);
           float y[8];
           load8<F32>(reinterpret_cast<const char*>(rec + w * 32 * kRow + d), y);
@@ -720,7 +718,7 @@ __global__ void __launch_bounds__(256) kv4_prefill_merge_kernel(const Kv4Prefill
   const int lim = min(p.seg_pos0[seg] + tok, p.max_ctx - 1);
   const int64_t row = (int64_t)(q0 + tok) * p.Hq + hq;
   kv4_join_splits<Tag, D, SL>(p.out + row * D * Tag::kBytes, p.ws + row * p.nsplit * (D + 4),
-                              lim < 0 ? 0 : min(lim / p.tps + 1, p.nsplit));
+                              lim < 0 ? 0 : min(lim / p.tps + 1, p.nsplit), p.scale2);
 }
 template <class Tag, int D, int SL>
 void launch_merge(const Kv4PrefillParams& p, hipStream_t s) {
