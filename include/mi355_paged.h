@@ -450,7 +450,10 @@ int32_t mi355_paged_prefill_max_context(int32_t dtype, int32_t D, int32_t block_
  *               of token 4 g + j; scales [4 g][D / 32][4 j]
  *   stride_block, stride_head: BYTES between blocks / heads, multiples of 16, the same for K and V; a
  *   head's tiles are contiguous.  D in {32, 64, 128, 256}; block_size a multiple of 16.
- *   A slot (block * block_size + row) nobody wrote may hold anything: no result depends on it.
+ *   A slot (block * block_size + row) nobody wrote may hold anything: no result depends on it but those
+ *   of queries whose context contains it.  Scale bytes 253 and 254 are never written (their blocks hold
+ *   values beyond the largest float); attention may answer a value block that has one with infinities
+ *   or NaN, to the queries that see it.
  * ---------------------------------------------------------------------------------------------
  */
 

@@ -678,6 +678,32 @@ def test_decode_does_not_depend_on_unwritten_slots(ops, device, dtype, Hq, Hkv, 
         assert torch.isfinite(out).all() and torch.equal(out, want), fill
 
 
+@pytest.mark.parametrize('dtype', ALL)
+@pytest.mark.parametrize('byte', [253, 254])
+@pytest.mark.parametrize('seqs,n,Hq,Hkv,D,pos0', [
+    (1, 90, 8, 8, 64, 0), (8, 512, 8, 8, 64, 300), (16, 400, 8, 8, 64, 0), (8, 2048, 8, 8, 64, 0), (4, 300, 32, 8, 128, 0), (2, 60, 8, 2, 128, 1000),
+    (9, 250, 8, 8, 256, 0), (8, 512, 8, 8, 32, 300), (8, 2048, 8, 8, 32, 0), (1, 20, 8, 2, 64, 5000)], ids=str)
+def test_rows_beyond_the_format_reach_only_the_queries_that_see_them(ops, device, dtype, byte, seqs, n, Hq, Hkv, D, pos0):
+    """A slot in the middle of a chunk that nobody wrote: the queries before it are what they are without it."""
+    rng = np.random.default_rng(n + D)
+    blocks = -(-(n + pos0) // 16)
+    shape = ops.kv4_cache_shape(seqs * blocks, Hkv, 16, D)
+    kc, vc = (torch.from_numpy(rng.integers(0, 256, shape, dtype=np.uint8)).cuda() for _ in range(2))
+    kc[..., 8 * D:], vc[..., 8 * D:] = 126, 127
+    tables = torch.arange(seqs * blocks, dtype=torch.int32, device=device).view(seqs, blocks)
+    q = torch.from_numpy(rng.standard_normal((seqs * n, Hq, D))).cuda().to(dtype)
+    meta = torch.tensor([[i * n for i in range(seqs)], [n] * seqs, [pos0] * seqs], dtype=torch.int32, device=device)
+    args = (tables, meta[0], meta[1], meta[2], n, n + pos0)
+    want = ops.paged_prefill_kv4(q, kc, vc, *args)
+    at = [pos0 + n // 2, pos0 + n - 1]
+    for t in at:
+        for b in range(D // 32):
+            vc[tables[-1, t // 16].long(), :, 0, orc.scale_place(D, t % 16, b, True)] = byte
+    got = ops.paged_prefill_kv4(q, kc, vc, *args)
+    before = (seqs - 1) * n + n // 2
+    assert torch.isfinite(want).all() and torch.equal(got[:before], want[:before])
+
+
 # ------------------------------------------------------------------ the weights' bits
 def _close_bound(size, big, want, D, n, dtype):
     """_attention_bound with the 16 bits that a weight has at least: two pieces leave out 2^-16 of it, and as much may be

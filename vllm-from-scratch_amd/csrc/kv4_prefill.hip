@@ -216,7 +216,8 @@ __global__ void __launch_bounds__(256, 2) kv4_prefill_kernel(const Kv4PrefillPar
     if (t0 + St::kTokens - 1 > wg_first) {
       // Some column must not see some of these value rows; they enter its product with weight 0, and 0 * NaN is
       // NaN.  Rows behind the workgroup's last position count as 0; NaN blocks become 0 here and are put back,
-      // for the columns that see them, where the stage is used.
+      // for the columns that see them, where the stage is used.  (Scale bytes above the largest that the append
+      // writes count as NaN here: with them a value may be an infinity.)
       uint32_t nan[NB];
 #pragma unroll
       for (int b = 0; b < NB; ++b) nan[b] = 0;
@@ -230,7 +231,7 @@ __global__ void __launch_bounds__(256, 2) kv4_prefill_kernel(const Kv4PrefillPar
           uint32_t vs = (rvs[i][b] & keep) | (0x7f7f7f7fu & ~keep), bad = 0;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const bool is_nan = ((vs >> (8 * j)) & 0xffu) == 255u;
+            const bool is_nan = ((vs >> (8 * j)) & 0xffu) > kKv4MaxExp + 127u;
             const uint64_t all = __ballot(is_nan);   // lanes 0, 16, 32, 48 speak for tokens j, 4 + j, 8 + j, 12 + j
             nan[b] |= (uint32_t)((all & 1) | (all >> 16 & 1) << 4 | (all >> 32 & 1) << 8 | (all >> 48 & 1) << 12) << (16 * i + j);
             bad |= is_nan ? 0xffu << (8 * j) : 0u;
@@ -528,7 +529,7 @@ __global__ void __launch_bounds__(W * 64, 2) kv4_rows_kernel(const Kv4PrefillPar
             uint32_t bad = 0;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              const bool is_nan = ((vs >> (8 * j)) & 0xffu) == 255u;
+              const bool is_nan = ((vs >> (8 * j)) & 0xffu) > kKv4MaxExp + 127u;
               bad |= is_nan ? 0xffu << (8 * j) : 0u;
               nan[b] |= is_nan ? 1u << (t * 16 + 4 * (g + 2 * q) + j) : 0u;
             }
