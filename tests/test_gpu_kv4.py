@@ -985,6 +985,37 @@ def test_blocks_far_into_a_large_pool(ops, device):
         assert torch.equal(a, b)
 
 
+def test_blocks_of_more_than_2_to_the_31_bytes(ops, device):
+    """One block that holds a whole long sequence, 2.2 GB per tensor: rows at its end are written, read and attended to.
+    Keys of 0 everywhere else, whose 16 million weights are e^-70 of the last rows' at most."""
+    D, tiles, n = 256, 1_000_000, 40
+    ctx = tiles * 16 - 7
+    shape = ops.kv4_cache_shape(1, 1, tiles * 16, D)
+    assert shape[2] * shape[3] > 1 << 31
+    kc, vc = (torch.full(shape, 0, dtype=torch.uint8, device=device) for _ in range(2))
+    for c in (kc, vc):
+        c[..., 8 * D:] = 127
+    rng = np.random.default_rng(9)
+    x = torch.from_numpy(rng.choice([-1.0, 1.0], (n, 3, D))).cuda().to(torch.bfloat16)
+    q, k, v = x[:, :1].contiguous() * 0.5, x[:, :1].contiguous() * 3, x[:, 2:].contiguous()
+    slots = torch.arange(ctx - n, ctx, device=device)
+    out = ops.rope_kv4_write(q, k, v, None, None, slots, kc, vc)
+    assert torch.equal(out, q)
+    rk, rv = ops.kv4_read_slots(kc, vc, slots)
+    assert torch.equal(rk, k) and torch.equal(rv, v)
+    table, scale = torch.zeros(1, 1, dtype=torch.int32, device=device), 0.25                          # a row's own score is 96, the others' have a spread of 6
+    got = ops.paged_decode_kv4(q[-1:].contiguous(), kc, vc, table, torch.tensor([ctx], dtype=torch.int32, device=device), ctx, scale=scale)
+    meta = torch.tensor([[0], [n], [ctx - n]], dtype=torch.int32, device=device)
+    chunk = ops.paged_prefill_kv4(q, kc, vc, table, meta[0], meta[1], meta[2], n, ctx, scale=scale)
+    qd, kd, vd = (t.double()[:, 0] for t in (q, k, v))
+    score = qd @ kd.T * scale
+    score = score.masked_fill(torch.ones_like(score).triu(1).bool(), -math.inf)
+    want = (torch.softmax(score, -1) @ vd).cpu().numpy()
+    bound = 2.0 ** -8 * np.abs(want) + 2.0 ** -14 + 2.0 ** -22
+    _near(chunk[:, 0], want, bound)
+    _near(got[:, 0], want[-1:], bound[-1:])
+
+
 # ------------------------------------------------------------------ the engine over a 4-bit cache
 @pytest.mark.parametrize('rotary', [None, dict(dim=32, interleaved=True, scaling={'kind': 'yarn', 'factor': 4, 'original': 64})])
 def test_engine_layer_steps(ops, device, rotary):

@@ -75,7 +75,7 @@ __device__ __forceinline__ Kv4Place kv4_place(const Kv4Cache& c, const int32_t* 
 // Byte offset of its record within a head's part of the pool.
 __device__ __forceinline__ int64_t kv4_record(const Kv4Cache& c, Kv4Place at, int tile_bytes) {
   const int id = at.id < 0 ? 0 : (at.id >= c.num_blocks ? c.num_blocks - 1 : at.id);
-  return (int64_t)((uint64_t)(uint32_t)id * (uint64_t)c.s_blk) + (int64_t)(at.sub * tile_bytes);
+  return (int64_t)((uint64_t)(uint32_t)id * (uint64_t)c.s_blk) + (int64_t)at.sub * tile_bytes;   // (a block may pass 2^31 bytes)
 }
 
 // E8M0 byte j of a dword -> the scale operand of the conversion instructions, which read the exponent

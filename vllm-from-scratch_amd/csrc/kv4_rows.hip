@@ -131,7 +131,7 @@ __device__ __forceinline__ int64_t slot_record(const Kv4Cache& c, int64_t slot, 
   const int64_t blk = bs_shift >= 0 ? (slot >> bs_shift) : slot / (c.tpb * kKv4Tile);
   const int in = (int)(slot - blk * c.tpb * kKv4Tile);
   r = in % kKv4Tile;
-  return blk * c.s_blk + (int64_t)h * c.s_head + in / kKv4Tile * kv4_tile_bytes(D);
+  return blk * c.s_blk + (int64_t)h * c.s_head + (int64_t)(in / kKv4Tile) * kv4_tile_bytes(D);
 }
 // Whether two tokens' codes are neighbouring bytes of a value record, in order.
 __device__ __forceinline__ bool one_pair(int64_t a, int64_t b) { return a % 2 == 0 && b == a + 1; }
