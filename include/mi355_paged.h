@@ -459,8 +459,9 @@ int32_t mi355_paged_prefill_max_context(int32_t dtype, int32_t D, int32_t block_
 
 /*
  * cos_out[t][i] = factor * cos(positions[t] * inv_freq[i]), sin_out likewise; both [T, half_dim]
- * floats.  The product and its reduction are done in double (positions up to 2^53), so that far
- * positions keep their angle; the reference's tables end at position 8191
+ * floats.  The product is a double, and cos and sin are those of that double to 7e-12 and the rounding
+ * to float, up to 2^63 in magnitude (NaN beyond).  The product's own rounding, 2^-53 of the angle,
+ * stays below a float's up to angles of 2^28; the reference's tables end at position 8191
  * (RotaryEmbedding, 05_mini_vllm/mini_vllm.py:360-374).  One call serves every layer of a step.
  *   positions [T] int64, inv_freq [half_dim] double (device memory)
  */

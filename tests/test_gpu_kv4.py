@@ -62,6 +62,23 @@ def test_angles(ops, device, T, half):
         _near(got, want, U * np.abs(want) + factor * (2.0 ** -52 * np.abs(a) + 2e-11))
 
 
+@pytest.mark.parametrize('kind', [None, 'yarn'])
+def test_angles_of_far_positions(ops, device, kind):
+    """cos and sin of the rounded product itself, up to the last position: the first Taylor term left out, (pi/4)^13 / 13! =
+    7e-12, and the rounding to float."""
+    rng = np.random.default_rng(5)
+    pos = np.concatenate([rng.integers(1 << e, 1 << (e + 1), 40) for e in range(63)] + [np.array([0, (1 << 53) + 1, (1 << 63) - 1, -(1 << 63)])])
+    pos[::7] *= -1
+    freq, factor = ops.rope_frequencies(64, scaling=kind and {'kind': kind, 'factor': 8, 'original': 4096})
+    cos, sin = ops.rope_angles(torch.from_numpy(pos).cuda(), freq.cuda(), factor)
+    a = pos[:, None].astype(np.float64) * freq.numpy()
+    for got, f in ((cos, math.cos), (sin, math.sin)):
+        want = np.vectorize(f)(a) * factor
+        _near(got, want, U * np.abs(want) + factor * 7.1e-12)
+    cos, sin = ops.rope_angles(torch.tensor([1, (1 << 63) - 1], device=device), torch.tensor([1e300, 4.0, 1.0], dtype=torch.float64, device=device))
+    assert torch.isnan(cos).tolist() == torch.isnan(sin).tolist() == [[True, False, False], [True, True, False]]
+
+
 def test_angles_refusals(ops, device):
     pos, freq = torch.zeros(3, dtype=torch.int64, device=device), torch.ones(4, dtype=torch.float64, device=device)
     with pytest.raises(TypeError):

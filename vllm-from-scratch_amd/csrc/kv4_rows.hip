@@ -32,11 +32,23 @@ namespace {
 // ---------------------------------------------------------------------------
 // a = position * frequency is formed in double: at position 2^24 a float's last bit is a whole
 // radian.  Reduction to [-pi/4, pi/4] with pi/2 in two parts, then the Taylor polynomials: the first
-// term left out is below 1e-11, far under the float the result is rounded to.
+// term left out is below 7e-12, far under the float the result is rounded to.  The rounding of
+// a * 2 / pi moves the quotient by 2^-13 at 2^40 and by whole turns beyond 2^53, so far angles are
+// reduced a second time.  (Beyond 2^63, where no 64-bit position leads at a frequency of 1: NaN.)
 __device__ __forceinline__ void sincos_reduced(double a, double& s, double& c) {
-  const double n = __builtin_rint(a * 0.63661977236758134308);                 // 2 / pi
-  double r = __builtin_fma(-n, 1.57079632679489655800e+00, a);
-  r = __builtin_fma(-n, 6.12323399573676603587e-17, r);
+  constexpr double kTurns = 0.63661977236758134308;                            // 2 / pi
+  constexpr double kHi = 1.57079632679489655800e+00, kLo = 6.12323399573676603587e-17;
+  const double n = __builtin_rint(a * kTurns);
+  double r = __builtin_fma(-n, kHi, a);
+  r = __builtin_fma(-n, kLo, r);
+  long long quarter = (long long)n;
+  if (!(__builtin_fabs(a) < 0x1p40)) {
+    const double m = __builtin_rint(r * kTurns);
+    r = __builtin_fma(-m, kHi, r);
+    r = __builtin_fma(-m, kLo, r);
+    quarter += (long long)m;
+    if (!(__builtin_fabs(a) <= 0x1p63)) r = __builtin_nan("");
+  }
   const double z = r * r;
   double ps = -1.0 / 39916800.0;
   ps = __builtin_fma(ps, z, 1.0 / 362880.0);
@@ -51,7 +63,7 @@ __device__ __forceinline__ void sincos_reduced(double a, double& s, double& c) {
   pc = __builtin_fma(pc, z, 1.0 / 24.0);
   pc = __builtin_fma(pc, z, -0.5);
   const double cr = __builtin_fma(pc, z, 1.0);
-  const int q = (int)(long long)n & 3;   // |n| < 2^62 for every position below 2^62
+  const int q = (int)quarter & 3;
   const double sv = (q & 1) ? cr : sr, cv = (q & 1) ? sr : cr;
   s = (q & 2) ? -sv : sv;
   c = (q == 1 || q == 2) ? -cv : cv;
