@@ -797,6 +797,87 @@ def test_equal_value_rows_come_back(ops, device, dtype, seqs, n, Hq, Hkv, D):
     _near(out, np.full(x.shape, 1.5), 1.5 * 2 * (ctx + 8) * U if dtype == torch.float32 else 0.0)
 
 
+# ------------------------------------------------------------------ contexts split over workgroups
+def _border_caches(rng, seqs, ctx, Hkv, D, marked):
+    """Caches of sequences of ctx tokens in scattered blocks: random values; dim 0 of a key is 6 at the marked positions and
+    -6 elsewhere, all else 0.  Returns (K, V, tables, values [seqs, ctx, Hkv, D])."""
+    blocks = -(-ctx // 16)
+    tables = rng.permutation(seqs * blocks).reshape(seqs, blocks).astype(np.int32)
+    byte = np.full((seqs * blocks, Hkv, 16, D // 32), 127, dtype=np.uint8)
+    kcode = np.zeros((seqs * blocks, Hkv, 16, D), dtype=np.uint8)
+    flag = np.zeros(blocks * 16, dtype=bool)
+    flag[marked] = True
+    for i in range(seqs):
+        kcode[tables[i], :, :, 0] = np.where(flag, 7, 15).reshape(blocks, 1, 16)
+    vcode = rng.integers(0, 16, kcode.shape).astype(np.uint8)
+    values = orc.dequantise(vcode, byte)[tables].transpose(0, 1, 3, 2, 4).reshape(seqs, blocks * 16, Hkv, D)
+    return orc.pack(kcode, byte, False)[:, :, None], orc.pack(vcode, byte, True)[:, :, None], tables, values
+
+
+def _border_want(values, marked, limits, G):
+    """Mean of the marked value rows up to each limit, and of their magnitudes: [len(limits), Hkv * G, D]."""
+    seen = [[t for t in marked if t <= lim] for lim in limits]
+    return (np.repeat(np.stack([values[t].mean(0) for t in seen]), G, 1), np.repeat(np.stack([np.abs(values[t]).mean(0) for t in seen]), G, 1))
+
+
+@pytest.mark.parametrize('dtype', ALL)
+@pytest.mark.parametrize('B,Hq,Hkv,D,ctx,splits', [
+    (16, 4, 4, 256, 2000, 4), (2, 4, 2, 256, 5000, 20), (4, 8, 8, 32, 4000, 16), (16, 8, 8, 32, 2500, 4), (3, 8, 2, 128, 3000, 12), (12, 8, 8, 128, 2000, 6),
+    (2, 8, 8, 64, 6000, 24), (10, 16, 8, 64, 1500, 6)])
+def test_decode_splits_lose_and_double_no_token(ops, device, dtype, B, Hq, Hkv, D, ctx, splits):
+    """The tokens on either side of every border that a split may have, and a context's last, share all of the weight; one
+    missing or counted twice moves every output by its value's share.  Contexts that end in front of, on and behind borders."""
+    from mi355_paged import _lib
+    bytes_ = _lib.load().mi355_paged_decode_kv4_workspace_bytes(B, Hq, Hkv, D, ctx, ops.dtype_code(torch.empty(0, dtype=dtype)))
+    assert bytes_ == B * Hq * splits * (D + 4) * 4          # (the way of cutting up that this test is for)
+    rng = np.random.default_rng(ctx + D)
+    lens = [ctx] + [max(1, ctx - 127 * i - i % 3) for i in range(1, B - 1)] + [1]
+    lens[1:2] = [ctx - ctx % 128]
+    marked = sorted({t for t in range(ctx) if t % 128 in (0, 127)} | {n - 1 for n in lens})
+    kc, vc, tables, values = _border_caches(rng, B, ctx, Hkv, D, marked)
+    q = torch.zeros(B, Hq, D, dtype=dtype, device=device)
+    q[..., 0] = 1.0
+    args = [torch.from_numpy(a).cuda() for a in (kc, vc, tables)]
+    out = ops.paged_decode_kv4(q, *args, torch.tensor(lens, dtype=torch.int32, device=device), ctx, scale=8.0)
+    want, size = (np.concatenate(x) for x in zip(*[_border_want(values[i], marked, [lens[i] - 1], Hq // Hkv) for i in range(B)]))
+    _near(out, want, HALF[dtype] * np.abs(want) + (2.0 ** -15 + 2 * (ctx + 8) * U) * size)
+    # a NaN value block in a late split: its dims, its head's queries, the sequences that reach it
+    at, head, b = ctx - 200, Hkv - 1, D // 32 - 1
+    args[1][torch.from_numpy(tables[:, at // 16]).long().cuda(), head, 0, orc.scale_place(D, at % 16, b, True)] = 255
+    out = ops.paged_decode_kv4(q, *args, torch.tensor(lens, dtype=torch.int32, device=device), ctx, scale=8.0)
+    expect = np.zeros(want.shape, dtype=bool)
+    expect[np.array(lens) > at, head * (Hq // Hkv):, 32 * b:] = True
+    np.testing.assert_array_equal(torch.isnan(out).cpu().numpy(), expect)
+
+
+@pytest.mark.parametrize('dtype', ALL)
+@pytest.mark.parametrize('seqs,n,Hq,Hkv,D,ctx,splits', [
+    (1, 16, 32, 8, 128, 4000, 16), (4, 16, 8, 8, 128, 3000, 6), (2, 16, 8, 2, 256, 3000, 12), (8, 30, 8, 8, 256, 2500, 4), (1, 9, 8, 8, 32, 5000, 20),
+    (4, 20, 8, 8, 32, 2300, 5), (2, 5, 4, 2, 64, 7000, 28), (3, 40, 8, 4, 64, 2600, 6)])
+def test_chunk_splits_lose_and_double_no_token(ops, device, dtype, seqs, n, Hq, Hkv, D, ctx, splits):
+    from mi355_paged import _lib
+    bytes_ = _lib.load().mi355_paged_prefill_kv4_workspace_bytes(seqs, seqs * n, n, Hq, Hkv, D, ctx, ops.dtype_code(torch.empty(0, dtype=dtype)))
+    assert bytes_ == seqs * n * Hq * splits * (D + 4) * 4
+    rng = np.random.default_rng(ctx + D)
+    end = [ctx, ctx - ctx % 256 + n // 2, 256 + n // 3, n][:seqs] + [ctx - 300 * i for i in range(1, seqs - 3)]       # chunks across borders
+    marked = sorted({t for t in range(ctx) if t % 128 in (0, 127)} | {t for e in end for t in range(e - n, e)})
+    kc, vc, tables, values = _border_caches(rng, seqs, ctx, Hkv, D, marked)
+    q = torch.zeros(seqs * n, Hq, D, dtype=dtype, device=device)
+    q[..., 0] = 1.0
+    args = [torch.from_numpy(a).cuda() for a in (kc, vc, tables)]
+    meta = torch.tensor([[i * n for i in range(seqs)], [n] * seqs, [e - n for e in end]], dtype=torch.int32, device=device)
+    out = ops.paged_prefill_kv4(q, *args, meta[0], meta[1], meta[2], n, ctx, scale=8.0)
+    want, size = (np.concatenate(x) for x in zip(*[_border_want(values[i], marked, list(range(e - n, e)), Hq // Hkv) for i, e in enumerate(end)]))
+    _near(out, want, HALF[dtype] * np.abs(want) + (2.0 ** -15 + 2 * (ctx + 8) * U) * size)
+    # NaN value blocks in a late split: one that all queries of the first chunk see, one in the middle of the chunk
+    expect = np.zeros(want.shape, dtype=bool)
+    for at, head, b in ((ctx - 3 * n, 0, 0), (ctx - n // 2, Hkv - 1, D // 32 - 1)):
+        args[1][int(tables[0, at // 16]), head, 0, orc.scale_place(D, at % 16, b, True)] = 255
+        expect[max(0, at - (ctx - n)):n, head * (Hq // Hkv):(head + 1) * (Hq // Hkv), 32 * b:32 * b + 32] = True
+    out = ops.paged_prefill_kv4(q, *args, meta[0], meta[1], meta[2], n, ctx, scale=8.0)
+    np.testing.assert_array_equal(torch.isnan(out).cpu().numpy(), expect)
+
+
 # ------------------------------------------------------------------ extremes of scores and values
 FORMS = [   # sequences, query rows each (0: decode), Hq, Hkv, D, context: each way rows and contexts are cut up
     (3, 0, 8, 8, 64, 600), (2, 0, 8, 2, 128, 9000), (70, 0, 8, 8, 64, 700), (1, 40, 8, 8, 64, 600), (1, 9, 8, 2, 128, 6000), (8, 512, 8, 8, 64, 812),
