@@ -16,7 +16,6 @@
 //       and convert their own in registers: no barrier, short walks, more conversion per row.
 #include <algorithm>
 #include <cmath>
-#include <type_traits>
 
 #include "kv4.h"
 
@@ -468,31 +467,28 @@ __global__ void __launch_bounds__(W * 64, 2) kv4_rows_kernel(const Kv4PrefillPar
   const int sbyte = ktok * (D / 32) + (D == 256 ? 2 * g : D == 128 ? g : 0);   // of group g, s = 0
   const uint32_t o_ks = 8 * D + (D == 256 ? ktok * 8 : (sbyte & ~3)), turn = 9 + 8 * (sbyte & 3);
   uint32_t o_v = ((g * 16 + c) * KS + (KS > 1 ? half * VB : 0)) * 4, o_vs = 8 * D + (g * KS + (KS > 1 ? half * VB : 0)) * 4;
-  // Steps whose codes are under way in registers: one / two 10.5 / 9.9 us for 8 chunks behind 900, 12.4 / 11.5 for 64 tokens
-  // behind 8000, both 8 heads of 64; at 128 dims the second set's registers cost more (2 of 256 behind 3000: 42 / 44).
-  constexpr int SETS = D <= 64 && CT == 1 ? 2 : 1;
-  uint32_t rk[SETS][2][KW], rks[SETS][SW], rv[SETS][2][2][VB], rvs[SETS][2][2][VB];
-  auto fetch_k = [&](int w, int64_t r0, int64_t r1) {
+  uint32_t rk[2][KW], rks[SW], rv[2][2][VB], rvs[2][2][VB];
+  auto fetch_k = [&](int64_t r0, int64_t r1) {
     const gptr rec = (gptr)kbase + (ktile ? r1 : r0);
-    load_words<false>(rec + o_k, rk[w][0]);
-    load_words<false>(rec + o_k + D / 4, rk[w][1]);
-    load_words<false>(rec + o_ks, rks[w]);
+    load_words<false>(rec + o_k, rk[0]);
+    load_words<false>(rec + o_k + D / 4, rk[1]);
+    load_words<false>(rec + o_ks, rks);
   };
-  auto fetch_v = [&](int w, int64_t r0, int64_t r1) {
+  auto fetch_v = [&](int64_t r0, int64_t r1) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       gptr rec = scalar_base(vbase + (t ? r1 : r0));
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        load_words<false>(rec + lane_offset(o_v) + q * 64 * D / 16, rv[w][t][q]);
-        load_words<false>(rec + lane_offset(o_vs) + q * 2 * KS * 4, rvs[w][t][q]);
+        load_words<false>(rec + lane_offset(o_v) + q * 64 * D / 16, rv[t][q]);
+        load_words<false>(rec + lane_offset(o_vs) + q * 2 * KS * 4, rvs[t][q]);
       }
     }
   };
-  auto k_scale = [&](int w, int f) {
+  auto k_scale = [&](int f) {
     const int pt = f & 1, s = f >> 1;
-    if constexpr (D == 256) return u2f(__builtin_amdgcn_alignbit(rks[w][pt], rks[w][pt], turn + 8 * (s >> 2)));
-    return u2f(__builtin_amdgcn_alignbit(rks[w][0], rks[w][0], turn + pt * (D == 128 ? 16 : D == 64 ? 8 : 0)));
+    if constexpr (D == 256) return u2f(__builtin_amdgcn_alignbit(rks[pt], rks[pt], turn + 8 * (s >> 2)));
+    return u2f(__builtin_amdgcn_alignbit(rks[0], rks[0], turn + pt * (D == 128 ? 16 : D == 64 ? 8 : 0)));
   };
   __syncthreads();
 
@@ -500,17 +496,13 @@ __global__ void __launch_bounds__(W * 64, 2) kv4_rows_kernel(const Kv4PrefillPar
   int t0 = lo + wave * kKv4Step;
   if (t0 <= wg_last) {
     place(t0);
-#pragma unroll
-    for (int w = 0; w < SETS; ++w) {
-      const int64_t r0 = kv4_record(p.cache, n0, kv4_tile_bytes(D)), r1 = kv4_record(p.cache, n1, kv4_tile_bytes(D));
-      fetch_k(w, r0, r1);
-      fetch_v(w, r0, r1);
-      place(min(t0 + (w + 1) * kStride, wg_last));
-    }
+    const int64_t r0 = kv4_record(p.cache, n0, kv4_tile_bytes(D)), r1 = kv4_record(p.cache, n1, kv4_tile_bytes(D));
+    fetch_k(r0, r1);
+    fetch_v(r0, r1);
+    place(min(t0 + kStride, wg_last));
   }
-  // One step with the codes of set w, which is refilled for SETS steps ahead as soon as its codes are converted.
-  auto step = [&](auto which) {
-    constexpr int w = decltype(which)::value;
+  // One step; its registers are refilled for the next as soon as their codes are converted.
+  auto step = [&]() {
     const int64_t r0 = kv4_record(p.cache, n0, kv4_tile_bytes(D)), r1 = kv4_record(p.cache, n1, kv4_tile_bytes(D));
     const bool masked = t0 + kKv4Step - 1 > wg_first;
     if (masked) {
@@ -525,7 +517,7 @@ __global__ void __launch_bounds__(W * 64, 2) kv4_rows_kernel(const Kv4PrefillPar
           const uint32_t keep = live >= 4 ? ~0u : (live <= 0 ? 0u : (1u << (8 * live)) - 1u);
 #pragma unroll
           for (int b = 0; b < VB; ++b) {
-            const uint32_t vs = (rvs[w][t][q][b] & keep) | (0x7f7f7f7fu & ~keep);
+            const uint32_t vs = (rvs[t][q][b] & keep) | (0x7f7f7f7fu & ~keep);
             uint32_t bad = 0;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -533,8 +525,8 @@ __global__ void __launch_bounds__(W * 64, 2) kv4_rows_kernel(const Kv4PrefillPar
               bad |= is_nan ? 0xffu << (8 * j) : 0u;
               nan[b] |= is_nan ? 1u << (t * 16 + 4 * (g + 2 * q) + j) : 0u;
             }
-            rv[w][t][q][b] &= keep & ~bad;
-            rvs[w][t][q][b] = (vs & ~bad) | (0x7f7f7f7fu & bad);
+            rv[t][q][b] &= keep & ~bad;
+            rvs[t][q][b] = (vs & ~bad) | (0x7f7f7f7fu & bad);
           }
         }
 #pragma unroll
@@ -571,7 +563,7 @@ __global__ void __launch_bounds__(W * 64, 2) kv4_rows_kernel(const Kv4PrefillPar
     for (int ct = 0; ct < CT; ++ct) S[ct] = 0.f;
 #pragma unroll
     for (int f = 0; f < QF; ++f) {
-      const bf16x8_t a = kv4_k_frag(rk[w][f & 1][f >> 1], k_scale(w, f));
+      const bf16x8_t a = kv4_k_frag(rk[f & 1][f >> 1], k_scale(f));
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
@@ -579,8 +571,8 @@ __global__ void __launch_bounds__(W * 64, 2) kv4_rows_kernel(const Kv4PrefillPar
       if (f + QD < QF) read_q(f + QD);
       __builtin_amdgcn_sched_barrier(0);
     }
-    fetch_k(w, r0, r1);
-    place(min(t0 + (SETS + 1) * kStride, wg_last));
+    fetch_k(r0, r1);
+    place(min(t0 + 2 * kStride, wg_last));
     bf16x8_t pf[CT][2][NW];
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
@@ -617,7 +609,7 @@ __global__ void __launch_bounds__(W * 64, 2) kv4_rows_kernel(const Kv4PrefillPar
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
         bf16x8_t ev, od;
-        kv4_v_frags(rv[w][0][q][b], rv[w][1][q][b], rvs[w][0][q][b], rvs[w][1][q][b], ev, od);
+        kv4_v_frags(rv[0][q][b], rv[1][q][b], rvs[0][q][b], rvs[1][q][b], ev, od);
         if constexpr (KS == 1) ev = half ? od : ev;
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct)
@@ -627,16 +619,10 @@ __global__ void __launch_bounds__(W * 64, 2) kv4_rows_kernel(const Kv4PrefillPar
             if constexpr (NT > 1) acc[ct][2 * b + 1] = mfma32_bf16(od, pf[ct][q][n], acc[ct][2 * b + 1]);
           }
       }
-    fetch_v(w, r0, r1);
+    fetch_v(r0, r1);
     t0 += kStride;
   };
-  while (t0 <= wg_last) {
-    step(std::integral_constant<int, 0>());
-    if constexpr (SETS == 2) {
-      if (t0 > wg_last) break;
-      step(std::integral_constant<int, 1>());
-    }
-  }
+  while (t0 <= wg_last) step();
 
   // join the waves
   float* const s_o = reinterpret_cast<float*>(s_mem) + wave * 32 * kRow;
