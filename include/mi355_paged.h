@@ -471,7 +471,8 @@ int mi355_rope_angles(float* cos_out, float* sin_out, const int64_t* positions, 
 /*
  * Rotary embedding of the first rotary_dim dims of every head row, out of place; the other dims are
  * copied.  Pairs are (i, i + rotary_dim / 2), or (2 i, 2 i + 1) when `interleaved`:
- *   a' = a cos[t][i] - b sin[t][i],  b' = b cos[t][i] + a sin[t][i]      (one rounding per value)
+ *   a' = a cos[t][i] - b sin[t][i],  b' = b cos[t][i] + a sin[t][i]
+ * in fp32 (one product rounded, the other in the sum's rounding), then rounded to the type.
  *   out [T, H, D] contiguous; x [T, H, D], x_stride_tok elements between tokens, heads D apart;
  *   cos_rows / sin_rows [T, rotary_dim / 2] floats, one row per token (mi355_rope_angles);
  *   rotary_dim a multiple of 16 in [0, D] (0: cos_rows / sin_rows may be NULL); an out that
@@ -497,7 +498,7 @@ int mi355_rope_kv4_write(void* q_out, const void* q, const void* k, const void* 
 
 /*
  * The cached rows of T slots as values: k_out, v_out [T, Hkv, D] contiguous.  A slot outside the
- * cache gives zeros; bf16 and fp32 hold every cached value exactly.
+ * cache gives zeros; bf16 and fp32 hold every value that the append writes exactly.
  */
 int mi355_kv4_read_slots(void* k_out, void* v_out, const void* k_cache, const void* v_cache,
                          const int64_t* slots, int32_t T, int32_t Hkv, int32_t D, int32_t block_size,

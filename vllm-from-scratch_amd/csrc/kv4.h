@@ -85,7 +85,8 @@ __device__ __forceinline__ float kv4_scale(uint32_t w, int j) {
   return u2f(j == 3 ? w >> 1 : w << (23 - 8 * j));
 }
 
-// Byte J of `w` -> (low nibble, high nibble) as two bf16, times the scale: exact.
+// Byte J of `w` -> (low nibble, high nibble) as two bf16, times the scale: exact for every scale that the append writes
+// (bytes 253 and 254 lead beyond the largest bf16: infinities).
 template <int J>
 __device__ __forceinline__ uint32_t kv4_to_bf16(uint32_t w, float scale) {
   return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, J));

@@ -281,10 +281,10 @@ int make_plan(const char* what, int B, int Hq, int Hkv, int D, int max_ctx, int 
   pl->qchunks = (G + 15) / 16;
   // kv heads per wave: more of them share a step's softmax and read longer runs of a block, but make fewer, longer
   // workgroups.  Where there is one (sequence, kv head) per CU or more, as many as leave a workgroup per CU: 256 x 2048
-  // 61 / 56 / 53.7 with 1 / 2 / 4 heads, 64 x 2048 19.0 / 18.2 / 21.0, 64 x 4096 at head_dim 32 30.4 / 20.9 / 23.3, 32 x 4000 at
-  // head_dim 128 27.9 / 29.8.  Below that the context is split all the same, and long ones (in `units` of a kv head's 128
-  // tokens) make up for the longer steps: 8 x 30000 33.3 / 30.7 / 31.9, 16 x 4000 14.8 / 15.7 / 15.7, 16 x 16000 at head_dim
-  // 32, fp32, 34.6 / 25.7 / 23.8, 4 to 65536, 32/8 heads of 128, fp16, 46.1 / 45.1.  The accumulators of NH heads take
+  // 61.7 / 56.8 / 54.6 with 1 / 2 / 4 heads, 64 x 2048 20.2 / 18.4 / 21.8, 64 x 4096 at head_dim 32 30.2 / 21.1 / 23.6, 32 x 4000
+  // at head_dim 128 28.1 / 30.6.  Below that the context is split all the same, and long ones (in `units` of a kv head's 128
+  // tokens) make up for the longer steps: 8 x 30000 35.2 / 31.1 / 32.4, 16 x 4000 15.6 / 16.0 / 15.5, 16 x 16000 at head_dim
+  // 32, fp32, 34.9 / 26.3 / 23.8, 4 to 65536, 32/8 heads of 128, fp16, 47.4 / 45.5.  The accumulators of NH heads take
   // NH D / 2 registers: NH D <= 256 leaves room for two waves per SIMD.
   const int64_t heads = (int64_t)std::max(B, 1) * Hkv * pl->qchunks, units = heads * (((int64_t)max_ctx + 127) / 128);
   auto more = [&](int nh) {   // whether 2 nh heads are better than nh
@@ -295,9 +295,10 @@ int make_plan(const char* what, int B, int Hq, int Hkv, int D, int max_ctx, int 
   pl->hgroups = Hkv / pl->NH;
   const int64_t groups = (int64_t)std::max(B, 1) * pl->hgroups * pl->qchunks;
   // More workgroups than the chip's 256 CUs: four waves each.  Fewer: eight waves each as long as that leaves a wave few
-  // steps (1 x 500: 6.6, in two splits and their merge 8.5; 32 x 1000: 9.0 against 10.4 with four waves), else the context
-  // is split over workgroups, two per CU (1 x 8000: 9.5; 4 sequences to 65536, 32/8 heads of 128, fp16: 45 against 67 with
-  // one per CU; head_dim 256 takes one per CU: 16 x 2000, 4 heads of 256: 15.1 against 16.0), none shorter than 256 tokens.
+  // steps (1 x 500: 6.3, in two splits and their merge 7.6; 32 x 1000: 9.2 against 10.6 with four waves), else the context
+  // is split over workgroups, two per CU (1 x 8000: 9.2, whole 29.0; 8 x 30000 31.0 against 35.5 with one per CU, 16 x 4000
+  // 15.7 against 18.4; head_dim 256 takes one per CU: 16 x 2000, 4 heads of 256: 15.8 against 18.4), none shorter than 256
+  // tokens.
   int64_t want = 1;
   pl->W = 4;
   if (groups <= 256) {

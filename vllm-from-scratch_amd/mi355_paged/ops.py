@@ -829,7 +829,9 @@ def rope_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional[d
       {'kind': 'yarn', 'factor': s, 'original': n}   pairs that turn more than beta_fast (32) times over n
                                         positions keep their frequency, those below beta_slow (1) turns
                                         are divided by s, a linear ramp in between; cos and sin are
-                                        multiplied by 0.1 ln s + 1 (Peng et al. 2023)"""
+                                        multiplied by 0.1 ln s + 1 (Peng et al. 2023).  The ramp is linear in the
+                                        turns, as in the paper; a checkpoint made with a ramp that is linear in the
+                                        pair's index has other frequencies: give rope_angles those"""
     if rotary_dim <= 0 or rotary_dim % 2:
         raise ValueError(f"rotary_dim {rotary_dim} must be a positive even number")
     i = torch.arange(rotary_dim // 2, dtype=torch.float64)
@@ -942,7 +944,7 @@ def rope_kv4_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: Optio
 def kv4_read_slots(k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor,
                    dtype: torch.dtype = torch.bfloat16):
     """(k, v), each [T, kv_heads, head_dim]: the values cached at `slots` (int64 [T]); zeros for a slot
-    outside the cache.  bfloat16 and float32 hold every cached value exactly."""
+    outside the cache.  bfloat16 and float32 hold every value that rope_kv4_write caches exactly."""
     dev = require_device(k_cache, v_cache, slots)
     lib = _lib.load()
     NB, Hkv, BS, D, sb, sh = _kv4_geometry(k_cache, v_cache)
