@@ -153,6 +153,30 @@ __device__ __forceinline__ void bf16_pieces(const float (&x)[8], bf16x8_t (&out)
   }
 }
 
+// The same of eight softmax weights, with one instruction for what a rounding leaves of a weight instead of two: the dot
+// product of the rounded pair with (-1, 0) or (0, -1), added to the weight (exact, as the difference is).  The two pairs of
+// constants stay in registers: as an inline constant of this instruction -1 is not the pair that the compiler takes it for.
+template <int N>
+__device__ __forceinline__ void weight_pieces(const float (&x)[8], bf16x8_t (&out)[N]) {
+  typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+  uint32_t first = 0x0000bf80u, second = 0xbf800000u;
+  asm("" : "+s"(first), "+s"(second));
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    float a = x[e], b = x[e + 1];
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const bf16x2_t h = {(__bf16)a, (__bf16)b};
+      out[n][e] = h[0];
+      out[n][e + 1] = h[1];
+      if (n + 1 < N) {
+        a = __builtin_amdgcn_fdot2_f32_bf16(h, __builtin_bit_cast(bf16x2_t, first), a, false);
+        b = __builtin_amdgcn_fdot2_f32_bf16(h, __builtin_bit_cast(bf16x2_t, second), b, false);
+      }
+    }
+  }
+}
+
 // Pieces of a query (all of its bits) and of a softmax weight.  A weight takes two at least: in one piece the rows of bf16
 // queries move by as much as their own rounding does (1.7e-3 of a row from the exact one, 2.3e-3 in one piece); in two
 // they move by 2^-17.  The second piece costs 4 x 2048 rows behind 2048, 32/8 heads of 128, 540 us for 409, and decode,

@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(W * 64) kv4_decode_kernel(const Kv4DecodeParam
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = kv4_weight(x[e], m, p.scale2);
     bf16x8_t pf[NW];
-    bf16_pieces<NW>(x, pf);
+    weight_pieces<NW>(x, pf);
 #pragma unroll
     for (int n = 0; n < NW; ++n) sum = mfma_bf16(ones, pf[n], sum);   // every row: the column's sum of weights
 #pragma unroll

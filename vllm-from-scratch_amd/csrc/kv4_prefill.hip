@@ -345,7 +345,7 @@ __global__ void __launch_bounds__(256, 2) kv4_prefill_kernel(const Kv4PrefillPar
           sum += x[e];
         }
 #pragma unroll
-        for (int n = 0; n < NQ; ++n) bf16_pieces<NW>(*reinterpret_cast<const float(*)[8]>(&x[8 * n]), pf[n]);
+        for (int n = 0; n < NQ; ++n) weight_pieces<NW>(*reinterpret_cast<const float(*)[8]>(&x[8 * n]), pf[n]);
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
           const bf16x8_t a0 = vf[s % VA][0], a1 = vf[s % VA][1];
@@ -601,7 +601,7 @@ __global__ void __launch_bounds__(W * 64, 2) kv4_rows_kernel(const Kv4PrefillPar
           x[e] = kv4_weight(S[ct][8 * n + e], m[ct], p.scale2);
           sum[ct] += x[e];
         }
-        bf16_pieces<NW>(x, pf[ct][n]);
+        weight_pieces<NW>(x, pf[ct][n]);
       }
     }
 #pragma unroll
