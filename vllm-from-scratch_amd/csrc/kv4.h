@@ -179,8 +179,8 @@ __device__ __forceinline__ void weight_pieces(const float (&x)[8], bf16x8_t (&ou
 
 // Pieces of a query (all of its bits) and of a softmax weight.  A weight takes two at least: in one piece the rows of bf16
 // queries move by as much as their own rounding does (1.7e-3 of a row from the exact one, 2.3e-3 in one piece); in two
-// they move by 2^-17.  The second piece costs 4 x 2048 rows behind 2048, 32/8 heads of 128, 540 us for 409, and decode,
-// which memory bounds, under 1 %.
+// they move by 2^-17.  The second piece costs 4 x 2048 rows behind 2048, 32/8 heads of 128, 560 us for 417, 8 chunks behind
+// 900 10.3 for 9.7, and decode, which memory bounds, under 1 %.
 template <class Tag>
 struct Kv4Pieces;
 template <>

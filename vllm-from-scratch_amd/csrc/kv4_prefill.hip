@@ -4,7 +4,7 @@
 // The query rows of a (segment, kv head) are its (token, query head of the group) pairs; they are the
 // columns of a score tile S^T = K Q^T, whose weights go back into the matrix unit in the registers they
 // were born in (see kv4.h).  Conversion of codes to bf16 (exact up to the largest bf16) is what the format costs beside attention
-// in bf16 -- 130 vector instructions per 32 tokens of 128 dims, as many as the softmax of 64 columns -- and
+// in bf16 -- 130 vector instructions per 32 tokens of 128 dims, as many as the softmax of 32 columns -- and
 // the two kernels differ in who does it:
 //   kv4_prefill_kernel  many rows.  A workgroup of four waves owns four tiles of 16 or 32 columns and walks
 //       the context in stages of SUB steps of 32 tokens.  Per stage each wave converts a quarter of the K
@@ -735,14 +735,14 @@ int make_plan(const char* what, int nseg, int total_rows, int max_q_len, int Hq,
   // kv4_rows_kernel has shorter walks and no barriers, but converts every code once per 32 (two tiles: 64) rows, where
   // kv4_prefill_kernel does per 64 (128): the former while its workgroups fit the chip about at once -- three of one tile per
   // CU, two beyond 64 dims; two of two tiles -- the latter beyond.  us, as chosen / the next best:
-  //   dealt, one tile   8 chunks to 45 behind 900, 8 heads of 64 10.9 / 15.7; a prompt of 2000, 8 of 64 19 / 25; one of 500,
-  //                     32/8 of 128 12.2 / 16.1; 2 of 128 behind 2000, 32/8 of 256 35 / 86; 5 of 512 behind 2000, 8 of 64, fp32
-  //                     49 / 61; 2 of 200 .. 300 behind 500 .. 1500, 32/8 of 128, fp16 45 / 60
-  //   dealt, two tiles  8 of 512 behind 2000, 8 of 64 44.7 / 46.6; 4 of 256 behind 3000, 32/8 of 128 85 / 91; a prompt of 2000,
-  //                     32/8 of 128 63 / 69
-  //   shared, one tile  16 uneven chunks to 1024, 8 of 64 34 / 37; 12 uneven fp16 prompts to 1500, 8 of 64 49.1 / 52.6; 3 of
-  //                     256, 32/8 of 128 13.0 / 14.9; 16 of 500, fp16, 8 of 256 52 / 69
-  //   shared, two tiles 8 of 4096, 8 of 64 240 / 254; 4 of 2048 behind 2048, 32/8 of 128 563 / 593; 8 of 1024, 8 of 128 42.7 / 43.8
+  //   dealt, one tile   8 chunks to 45 behind 900, 8 heads of 64 10.3 / 15.4; a prompt of 2000, 8 of 64 18 / 25; one of 500,
+  //                     32/8 of 128 12.2 / 15.5; 2 of 128 behind 2000, 32/8 of 256 35 / 86; 5 of 512 behind 2000, 8 of 64, fp32
+  //                     47 / 58; 2 of 200 .. 300 behind 500 .. 1500, 32/8 of 128, fp16 46 / 60
+  //   dealt, two tiles  8 of 512 behind 2000, 8 of 64 43.0 / 43.3; 4 of 256 behind 3000, 32/8 of 128 82 / 89; a prompt of 2000,
+  //                     32/8 of 128 62 / 68
+  //   shared, one tile  16 uneven chunks to 1024, 8 of 64 34 / 33; 12 uneven fp16 prompts to 1500, 8 of 64 48.6 / 52.8; 3 of
+  //                     256, 32/8 of 128 13.1 / 15.0; 16 of 500, fp16, 8 of 256 53 / 69
+  //   shared, two tiles 8 of 4096, 8 of 64 234 / 250; 4 of 2048 behind 2048, 32/8 of 128 561 / 562; 8 of 1024, 8 of 128 43.0 / 42.6
   // Registers set limits: two tiles spill at head_dim 256 and fp32's 128, and fp16's 128 where they are dealt.
   const bool narrow = D == 256 || (dtype == MI355_F32 && D == 128), single = narrow || (dtype == MI355_F16 && D == 128);
   const int64_t all_rows = (int64_t)total_rows * (Hq / Hkv);
@@ -761,12 +761,12 @@ int make_plan(const char* what, int nseg, int total_rows, int max_q_len, int Hq,
   }
   pl->row_tiles = (int)ceil_div64(rows, (pl->dealt ? 32 : 64) * pl->tiles);
   // Fewer workgroups than CUs: the context is split until there is one each, no split shorter than 256 tokens (16 tokens
-  // behind 30000, 32/8 heads of 128: 172 -> 28 us; 4 chunks to 64 behind 1500, 8/2 heads of 256: 25.4 -> 21.3), if that takes
+  // behind 30000, 32/8 heads of 128: 169 -> 27 us; 4 chunks to 64 behind 1500, 8/2 heads of 256: 24.6 -> 21.0), if that takes
   // 1100 tokens off a walk: the merge costs a launch (4.4 us of the host's time where steps are not replayed) and the rows'
-  // partial sums (2 chunks of 64 behind 2000, 32/8 heads of 128, replayed: 19.4 in one, 19.9 in two, 27.0 in four).
+  // partial sums (2 chunks of 64 behind 2000, 32/8 heads of 128, replayed: 19.3 in one, 20.0 in two, 26.6 in four).
   // One workgroup per CU or fewer: eight waves each, if the walk is long enough to pay for the larger join (2 of 512 behind
-  // 2000, 8 heads of 64, fp32 24.1 -> 22.6 us; 4 of 100 .. 200 behind 1500 .. 3000, 8 of 128 29.3 -> 26.1; 4 to 64 behind 600,
-  // 8 of 64 9.7 and 9.6; 4 of 250, 8 of 64 7.3 and 7.8).
+  // 2000, 8 heads of 64, fp32 23.3 -> 21.4 us; 4 of 100 .. 200 behind 1500 .. 3000, 8 of 128 29.4 -> 25.8; 4 to 64 behind 600,
+  // 8 of 64 9.4 and 9.2; 4 of 250, 8 of 64 7.0 and 7.3).
   pl->waves = pl->dealt && wgs <= 256 && max_ctx >= 768 ? 8 : kWaves;
   const int stage = pl->waves * kKv4Step;
   const int64_t stages = ceil_div64(max_ctx, stage);
