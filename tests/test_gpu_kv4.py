@@ -951,6 +951,80 @@ def test_values_at_the_top_of_the_format(ops, device, dtype, form):
         assert (np.abs(out[:, j] - want) <= bound).all(), (j, want, out[0, j, 0, 0])
 
 
+# ------------------------------------------------------------------ every form, whatever the plan would take
+@pytest.mark.parametrize('dtype', ALL)
+@pytest.mark.parametrize('D', [32, 64, 128, 256])
+@pytest.mark.parametrize('form', [1, 2, 11, 12])
+@pytest.mark.parametrize('Hq,Hkv,BS,lens,pos0', [(4, 2, 16, [1, 37, 0, 70, 130], [0, 5, 3, 33, 0]), (3, 1, 48, [45, 2, 64], [0, 1300, 1]), (8, 8, 16, [3, 33], [61, 0])],
+                         ids=lambda v: str(v))
+def test_chunks_in_every_form(ops, device, dtype, D, form, Hq, Hkv, BS, lens, pos0):
+    """Ragged chunks in each form of the prompt kernels (two tiles only where registers hold them): results, rows outside, rows
+    nobody wrote, NaN blocks; few rows behind a long context in splits where the form has them."""
+    rng = np.random.default_rng(D + sum(lens))
+    total = [n + p for n, p in zip(lens, pos0)]
+    kc, vc, tables, free_k, free_v = _unwritten(D + sum(lens), total, Hkv, D, BS)
+    tables = np.minimum(tables, len(kc) - 1)
+    start = [2 + int(x) + i for i, x in enumerate(np.cumsum([0] + lens)[:-1])]
+    rows = start[-1] + lens[-1] + 1
+    q, qv = _cast(rng.standard_normal((rows, Hq, D)), dtype)
+    bt, meta = torch.from_numpy(tables).cuda(), torch.tensor([start, lens, pos0], dtype=torch.int32, device=device)
+    inside = np.concatenate([np.arange(s, s + n) for s, n in zip(start, lens)])
+    outside = np.setdiff1d(np.arange(rows), inside)
+
+    def run():
+        out = torch.full((rows, Hq, D), 7.0, dtype=dtype, device=device)
+        with ops.debug_knob('MI355_KV4_CHUNK_FORM', form):
+            ops.paged_prefill_kv4(q, torch.from_numpy(kc).cuda(), torch.from_numpy(vc).cuda(), bt, meta[0], meta[1], meta[2], max(lens), max(total), out=out)
+        assert bool((out[torch.from_numpy(outside).cuda()] == 7.0).all())
+        return out[torch.from_numpy(inside).cuda()]
+
+    want, size, big = _attend_all([qv[s:s + n] for s, n in zip(start, lens)], kc, vc, tables, total, D ** -0.5,
+                                  [[p + j for j in range(n)] for n, p in zip(lens, pos0)])
+    first = run()
+    _near(first, want, _close_bound(size, big, want, D, max(total), dtype))
+    for fill in (0, 253, 254):
+        kc[free_k], vc[free_v] = fill, fill
+        assert torch.equal(run(), first), fill
+    # a NaN value block in the middle of the second chunk and a NaN key at its last position
+    i, n, p = 1, lens[1], pos0[1]
+    at, b, G = p + n // 2, D // 32 - 1, Hq // Hkv
+    vc[tables[i, at // BS], 0, at % BS // 16, orc.scale_place(D, at % 16, b, True)] = 255
+    kc[tables[i, (p + n - 1) // BS], Hkv - 1, (p + n - 1) % BS // 16, orc.scale_place(D, (p + n - 1) % 16, 0, False)] = 255
+    expect = np.zeros(want.shape, dtype=bool)
+    row0 = sum(lens[:i])
+    expect[row0 + n // 2:row0 + n, :G, 32 * b:32 * b + 32] = True
+    expect[row0 + n - 1, (Hkv - 1) * G:] = True
+    np.testing.assert_array_equal(torch.isnan(run()).cpu().numpy(), expect)
+
+
+@pytest.mark.parametrize('dtype', ALL)
+@pytest.mark.parametrize('heads', [1, 2, 4, 8])
+@pytest.mark.parametrize('Hq,Hkv,D,BS,lens', [(8, 8, 32, 16, [1, 33, 0, 300]), (16, 8, 32, 16, [77, 5]), (8, 8, 64, 48, [1, 17, 200]), (16, 4, 64, 16, [50, 2500]),
+                                              (8, 8, 128, 16, [31, 129]), (12, 2, 128, 16, [90]), (4, 4, 256, 16, [40, 7])], ids=lambda v: str(v))
+def test_decode_with_every_number_of_heads_per_wave(ops, device, dtype, heads, Hq, Hkv, D, BS, lens):
+    rng = np.random.default_rng(D + sum(lens))
+    kc, vc, tables, free_k, free_v = _unwritten(D + sum(lens), lens, Hkv, D, BS)
+    tables = np.minimum(tables, len(kc) - 1)
+    q, qv = _cast(rng.standard_normal((len(lens), Hq, D)), dtype)
+    want, size, big = _attend_all([qv[i:i + 1] for i in range(len(lens))], kc, vc, tables, lens, D ** -0.5, [[n - 1] for n in lens])
+
+    def run():
+        with ops.debug_knob('MI355_KV4_DECODE_HEADS', heads):
+            return ops.paged_decode_kv4(q, torch.from_numpy(kc).cuda(), torch.from_numpy(vc).cuda(), torch.from_numpy(tables).cuda(),
+                                        torch.tensor(lens, dtype=torch.int32, device=device), max(lens))
+
+    first = run()
+    _near(first, want, _close_bound(size, big, want, D, max(lens), dtype))
+    for fill in (0, 253, 254):
+        kc[free_k], vc[free_v] = fill, fill
+        assert torch.equal(run(), first), fill
+    i, at, G = len(lens) - 1, lens[-1] // 2, Hq // Hkv
+    vc[tables[i, at // BS], Hkv - 1, at % BS // 16, orc.scale_place(D, at % 16, 0, True)] = 255
+    expect = np.zeros(want.shape, dtype=bool)
+    expect[i, (Hkv - 1) * G:, :32] = True
+    np.testing.assert_array_equal(torch.isnan(run()).cpu().numpy(), expect)
+
+
 # ------------------------------------------------------------------ streams, graphs, all of them together
 def _step(ops, s):
     """One layer's work on new rows: angles, rotation + append, attention."""

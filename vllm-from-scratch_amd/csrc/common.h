@@ -44,6 +44,8 @@ enum Knob {
   kKnobMlaWideSplitTokens,  // MI355_MLA_WIDE_SPLIT_TOKENS  fewest tokens per workgroup at which a launch with token splits takes the 128-head kernel (0: planned)
   kKnobMlaWideFusedMerge,   // MI355_MLA_WIDE_FUSED_MERGE   1: two token splits of the 128-head kernel are merged by the later workgroup of the pair (0: by the merge kernel)
   kKnobMlaWideSkewTokens,   // MI355_MLA_WIDE_SKEW_TOKENS   tokens split 0 of such a pair is given less than half (so that only one record is written); 0: even splits
+  kKnobKv4ChunkForm,        // MI355_KV4_CHUNK_FORM         0: planned; prompt chunks over the 4-bit cache in 1 / 2 column tiles shared, 11 / 12 dealt (where registers hold two)
+  kKnobKv4DecodeHeads,      // MI355_KV4_DECODE_HEADS       0: planned; kv heads per wave of decode over the 4-bit cache (where a wave holds them)
   kKnobCount
 };
 int knob(Knob k);

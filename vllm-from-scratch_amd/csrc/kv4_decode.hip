@@ -292,6 +292,7 @@ int make_plan(const char* what, int B, int Hq, int Hkv, int D, int max_ctx, int 
   };
   pl->NH = 1;
   while (pl->NH * 2 <= 256 / D && pl->NH * 2 * pl->gc <= 16 && Hkv % (pl->NH * 2) == 0 && more(pl->NH)) pl->NH *= 2;
+  if (const int nh = knob(kKnobKv4DecodeHeads); nh > 0 && (nh & (nh - 1)) == 0 && nh <= 256 / D && nh * pl->gc <= 16 && Hkv % nh == 0) pl->NH = nh;
   pl->hgroups = Hkv / pl->NH;
   const int64_t groups = (int64_t)std::max(B, 1) * pl->hgroups * pl->qchunks;
   // More workgroups than the chip's 256 CUs: four waves each.  Fewer: eight waves each as long as that leaves a wave few

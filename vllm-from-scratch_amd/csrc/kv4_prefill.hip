@@ -759,6 +759,10 @@ int make_plan(const char* what, int nseg, int total_rows, int max_q_len, int Hq,
       pl->tiles = !narrow && workgroups(128) > (D <= 64 ? 1023 : 256) ? 2 : 1;
     }
   }
+  if (const int form = knob(kKnobKv4ChunkForm); form == 1 || form == 2 || form == 11 || form == 12) {
+    pl->dealt = form > 10;
+    pl->tiles = form % 10 == 2 && !(pl->dealt ? single : narrow) ? 2 : 1;
+  }
   pl->row_tiles = (int)ceil_div64(rows, (pl->dealt ? 32 : 64) * pl->tiles);
   // Fewer workgroups than CUs: the context is split until there is one each, no split shorter than 256 tokens (16 tokens
   // behind 30000, 32/8 heads of 128: 169 -> 27 us; 4 chunks to 64 behind 1500, 8/2 heads of 256: 24.6 -> 21.0), if that takes
@@ -767,10 +771,10 @@ int make_plan(const char* what, int nseg, int total_rows, int max_q_len, int Hq,
   // One workgroup per CU or fewer: eight waves each, if the walk is long enough to pay for the larger join (2 of 512 behind
   // 2000, 8 heads of 64, fp32 23.3 -> 21.4 us; 4 of 100 .. 200 behind 1500 .. 3000, 8 of 128 29.4 -> 25.8; 4 to 64 behind 600,
   // 8 of 64 9.4 and 9.2; 4 of 250, 8 of 64 7.0 and 7.3).
-  pl->waves = pl->dealt && wgs <= 256 && max_ctx >= 768 ? 8 : kWaves;
+  pl->waves = pl->dealt && pl->tiles == 1 && wgs <= 256 && max_ctx >= 768 ? 8 : kWaves;
   const int stage = pl->waves * kKv4Step;
   const int64_t stages = ceil_div64(max_ctx, stage);
-  int64_t want = wgs <= 128 ? std::min<int64_t>(256 / std::max<int64_t>(wgs, 1), ceil_div64(max_ctx, 256)) : 1;
+  int64_t want = pl->dealt && wgs <= 128 ? std::min<int64_t>(256 / std::max<int64_t>(wgs, 1), ceil_div64(max_ctx, 256)) : 1;
   if (max_ctx - max_ctx / want < 1100) want = 1;
   const int64_t per = ceil_div64(stages, std::min(want, stages));
   pl->tps = (int)(per * stage);
