@@ -581,6 +581,25 @@ def test_chunk_queries_before_the_first_position_see_nothing(ops, device, ctx):
         assert bool((out[20 + rows:] == 7.0).all())
 
 
+@pytest.mark.parametrize('longest', [40, 1 << 31, (1 << 32) + 7, 1 << 62])
+@pytest.mark.parametrize('bound', [300, (1 << 31) + 5, 1 << 62])
+def test_loose_host_bounds(ops, device, longest, bound):
+    """Bounds far beyond what the tensors hold say nothing: no rows and no positions are lost."""
+    rng = np.random.default_rng(6)
+    Hq, Hkv, D, BS = 4, 2, 64, 16
+    kc, vc, tables = _cache(rng, [300, 90], Hkv, D, BS)
+    args = [torch.from_numpy(a).cuda() for a in (kc, vc, tables)]
+    q, _ = _cast(rng.standard_normal((60, Hq, D)), torch.bfloat16)
+    meta = torch.tensor([[0, 40], [40, 20], [260, 70]], dtype=torch.int32, device=device)
+    want = ops.paged_prefill_kv4(q, *args, meta[0], meta[1], meta[2], 40, 300)
+    out = torch.full_like(want, 7.0)
+    ops.paged_prefill_kv4(q, *args, meta[0], meta[1], meta[2], longest, bound, out=out)
+    torch.testing.assert_close(out, want, atol=2.0 ** -6, rtol=2.0 ** -7)       # (another bound may cut the context up in another way)
+    ctx = torch.tensor([300, 90], dtype=torch.int32, device=device)
+    torch.testing.assert_close(ops.paged_decode_kv4(q[:2].contiguous(), *args, ctx, bound), ops.paged_decode_kv4(q[:2].contiguous(), *args, ctx, 300),
+                               atol=2.0 ** -6, rtol=2.0 ** -7)
+
+
 @pytest.mark.parametrize('Hq,Hkv,D,n,seqs,pos0', [
     (8, 8, 64, 90, 2, 0), (8, 8, 64, 512, 8, 300), (8, 8, 64, 400, 16, 0), (8, 8, 64, 2048, 8, 0), (32, 8, 128, 300, 1, 40),
     (32, 8, 128, 256, 3, 1600), (8, 2, 128, 60, 2, 1000), (8, 8, 128, 250, 9, 0), (32, 8, 128, 300, 4, 0), (8, 8, 256, 250, 9, 0), (8, 2, 256, 60, 1, 9),

@@ -174,6 +174,13 @@ def test_ops_refuse_host_tensors():
         ops.rope_angles(torch.zeros(1, dtype=torch.int64), torch.zeros(4, dtype=torch.float64))
 
 
+def test_blocks_beyond_the_entry_points_integers_are_refused():
+    big = torch.empty((1, 1, (1 << 28) + 1, 17 * 32 // 2), dtype=torch.uint8, device='meta')     # (16 tokens to a 32-bit count)
+    with pytest.raises(ValueError, match='per block'):
+        ops._kv4_geometry(big, big)
+    assert ops._kv4_geometry(big[:, :, :1000], big[:, :, :1000])[2] == 16000
+
+
 # ------------------------------------------------------------------ the engine's arguments
 @pytest.mark.parametrize('kw', [dict(kv_cache_dtype='mxfp4'), dict(rotary={}), dict(kv_cache_dtype='mxfp4', device='cuda', reference_compat=True),
                                 dict(kv_cache_dtype='fp4', device='cuda')])

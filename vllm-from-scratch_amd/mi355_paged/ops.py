@@ -769,6 +769,7 @@ def paged_prefill(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
 
 KV4_HEAD_DIMS = (32, 64, 128, 256)
 KV4_TILE = 16          # tokens per record; a block holds a whole number of them
+_INT32_MAX = 2 ** 31 - 1   # (what the C entry points take: larger numbers would lose their upper bits on the way)
 _KV4_RECORDS = {17 * d // 2: d for d in KV4_HEAD_DIMS}
 
 
@@ -792,6 +793,8 @@ def _kv4_geometry(k_cache: torch.Tensor, v_cache: torch.Tensor):
         raise ValueError(f"4-bit caches must share the shape kv4_cache_shape gives, got {tuple(shape)} and "
                          f"{tuple(v_cache.shape)}")
     blocks, heads, tiles, record = shape
+    if tiles * KV4_TILE > _INT32_MAX:
+        raise ValueError(f"4-bit caches hold fewer than 2^31 tokens per block, not {tiles * KV4_TILE}")
     if strides != v_cache.stride() or strides[3] != 1 or strides[2] != record or blocks == 1 or heads == 1:
         # (a dim of size 1 may carry any stride)
         strides = tuple(_stride(k_cache, d) for d in range(4))
@@ -988,7 +991,7 @@ def paged_decode_kv4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     if scale is None:
         scale = 1.0 / math.sqrt(D)
     width = block_tables.shape[1]
-    max_context = min(int(max_context), width * BS)
+    max_context = min(int(max_context), width * BS, _INT32_MAX)
     with _on(dev):
         stream = _stream(dev)
         need = lib.mi355_paged_decode_kv4_workspace_bytes(B, Hq, Hkv, D, max_context, code)
@@ -1033,15 +1036,15 @@ def paged_prefill_kv4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     if scale is None:
         scale = 1.0 / math.sqrt(D)
     width = block_tables.shape[1]
-    max_context = min(int(max_context), width * BS)
+    max_context, max_q_len = min(int(max_context), width * BS, _INT32_MAX), min(int(max_q_len), T)
     with _on(dev):
         stream = _stream(dev)
-        need = lib.mi355_paged_prefill_kv4_workspace_bytes(nseg, T, int(max_q_len), Hq, Hkv, D, max_context, code)
+        need = lib.mi355_paged_prefill_kv4_workspace_bytes(nseg, T, max_q_len, Hq, Hkv, D, max_context, code)
         ws, ws_bytes = _workspace(dev, need, stream)
         rc = lib.mi355_paged_prefill_kv4(
             out.data_ptr(), q.data_ptr(), q_stride, k_cache.data_ptr(), v_cache.data_ptr(),
             block_tables.data_ptr(), seg_q_start.data_ptr(), seg_len.data_ptr(), seg_pos0.data_ptr(), nseg,
-            T, int(max_q_len), Hq, Hkv, D, BS, width, NB, max_context, sb, sh, float(scale), code,
+            T, max_q_len, Hq, Hkv, D, BS, width, NB, max_context, sb, sh, float(scale), code,
             ws.data_ptr() if ws is not None else None, ws_bytes, stream)
     if rc:
         _lib.check(rc, 'mi355_paged_prefill_kv4')
