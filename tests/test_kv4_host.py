@@ -218,3 +218,14 @@ def test_plan_keeps_prompts_on_the_cache():
     assert plan.causal_tokens == 0 and plan.append_tokens == 5 and plan.append_meta.tolist() == [[0], [5], [0]]
     assert plan.paged_rows == 2 and plan.paged_context.tolist() == [8, 1] and not plan.pure_decode
     assert mini_vllm.build_attn_plan(**args).causal_tokens == 6
+
+
+@pytest.mark.parametrize('kw', [dict(), dict(reference_compat=True, block_tables=[[0]]), dict(table_rows=[0])])
+@pytest.mark.parametrize('prefill', [True, False])
+def test_model_over_a_4_bit_cache_needs_block_tables(kw, prefill):
+    """Without them a decode token would attend to slot 0 alone (the reference's decode branch), without an error."""
+    import mini_vllm
+    model = mini_vllm.MiniTransformer(50, 128, 1, 4, 64, 4, 16, kv_cache_dtype='mxfp4')
+    one = torch.zeros(1, dtype=torch.int64)
+    with pytest.raises(ValueError, match='block tables'):
+        model(one, one, one, [1], [prefill], **kw)

@@ -1025,6 +1025,9 @@ class MiniTransformer(nn.Module):
         block ids per request) enables attention over the true paged context, positions_host
         is an optional host copy of `positions` that saves a device read-back; device_tables +
         table_rows (what MiniVLLM passes) replace block_tables by rows of a persistent device copy."""
+        if self.kv4 and (reference_compat or (block_tables is None and (device_tables is None or table_rows is None))):
+            raise ValueError("a 4-bit cache is read through block tables: pass block_tables (or device_tables and table_rows), "
+                             "without reference_compat")
         home = self.embedding.weight.device
         token_ids, positions, slot_mapping = (t.to(home) for t in (token_ids, positions, slot_mapping))
         if positions_host is None:
