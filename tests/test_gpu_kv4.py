@@ -1249,6 +1249,37 @@ def test_engine_layer_steps(ops, device, rotary):
         _near(got, a @ w.T, bound.reshape(len(pos), -1) @ np.abs(w).T + (H * D + 2) * U * (np.abs(a) @ np.abs(w).T))
 
 
+@pytest.mark.parametrize('kw', [dict(kv_cache_dtype='mxfp4'), dict(rotary=dict(dim=16))], ids=str)
+def test_a_plan_serves_calls_with_other_positions(device, kw):
+    """One plan object for two steps whose tensors are updated in place, and for a single layer afterwards: every call
+    rotates by its own positions."""
+    import mini_vllm as mv
+    results = []
+    for fresh in (True, False):
+        torch.manual_seed(3)
+        model = mv.MiniTransformer(100, 64, 2, 2, 64, 8, 16, **kw).to(device)
+        ids = torch.tensor([5, 9], device=device)
+        tables = torch.tensor([[1, 2], [4, 3]], dtype=torch.int32, device=device)
+        ctx = torch.ones(2, dtype=torch.int32, device=device)
+        mk = lambda: mv.AttnPlan(total_tokens=2, causal_index=None, cu_seqlens=None, causal_tokens=0, max_causal_len=0, paged_index=None,
+                                 paged_tables=tables, paged_context=ctx, paged_rows=2, max_context=32, pure_decode=True)
+        plan, outs = mk(), []
+        with torch.no_grad():
+            for step in range(3):
+                pos = torch.full((2,), step, dtype=torch.int64, device=device)
+                slots = tables[:, 0].long() * 16 + pos
+                ctx.fill_(step + 1)
+                outs.append(model.forward_planned(ids, pos, slots, mk() if fresh else plan))
+            x = torch.randn(2, 64, generator=torch.Generator(device).manual_seed(1), device=device)
+            pos = torch.full((2,), 3, dtype=torch.int64, device=device)
+            ctx.fill_(4)
+            outs.append(model.layers[0].attn(x, pos, (model.k_cache[0], model.v_cache[0]), tables[:, 0].long() * 16 + pos, [1, 1], [False] * 2,
+                                             mk() if fresh else plan))
+        results.append(outs)
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+
+
 def _generate(mv, graphs, dtype, **kw):
     torch.manual_seed(7)
     eng = mv.MiniVLLM(vocab_size=300, hidden_size=128, num_layers=2, num_heads=4, intermediate_size=256, num_kv_blocks=64,

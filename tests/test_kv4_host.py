@@ -229,3 +229,11 @@ def test_model_over_a_4_bit_cache_needs_block_tables(kw, prefill):
     one = torch.zeros(1, dtype=torch.int64)
     with pytest.raises(ValueError, match='block tables'):
         model(one, one, one, [1], [prefill], **kw)
+
+
+def test_layer_over_a_4_bit_cache_needs_a_plan():
+    import mini_vllm
+    model = mini_vllm.MiniTransformer(50, 128, 1, 4, 64, 4, 16, kv_cache_dtype='mxfp4')
+    one = torch.zeros(1, dtype=torch.int64)
+    with pytest.raises(ValueError, match='block tables'):
+        model.layers[0].attn(torch.zeros(1, 128), one, (model.k_cache[0], model.v_cache[0]), one, [1], [False])

@@ -581,7 +581,7 @@ class AttnPlan:
     # paged_context[r] = its position + 1 cached rows): RoPE, cache write and attention of a layer
     # can then be ONE launch (ops.paged_decode_append with rope tables)
     pure_decode: bool = False
-    # cos / sin rows of the step's positions (RotaryPositions), made by the first layer that asks and shared by the rest
+    # cos / sin rows of the positions of the model call that is running (RotaryPositions), shared by its layers; None between calls
     angles: Optional[tuple] = None
 
 
@@ -877,14 +877,14 @@ class SelfAttention(nn.Module):
     def forward(self, x, positions, kv_cache, slot_mapping, seq_lens, is_prefill, plan: Optional[AttnPlan] = None):
         T, H, D = x.shape[0], self.num_heads, self.head_dim
         if plan is None:   # called the reference's way: no block tables -> reference semantics
+            if kv_cache[0].dtype == torch.uint8:
+                raise ValueError("a 4-bit cache is read through block tables: pass a plan built with from_cache=True")
             plan = build_attn_plan(positions.tolist(), seq_lens, is_prefill, None, _compute_device(kv_cache[0]))
         qkv = self.qkv(x)
         q, k, v = (t.view(T, H, D) for t in qkv.chunk(3, dim=-1))
         k_cache, v_cache = kv_cache
         if self.rotary is not None:
-            if plan.angles is None:
-                plan.angles = self.rotary.angles(positions)
-            cos, sin = plan.angles
+            cos, sin = self.rotary.angles(positions) if plan.angles is None else plan.angles
             if k_cache.dtype == torch.uint8:
                 q = ops.rope_kv4_write(q, k, v, cos, sin, slot_mapping, k_cache, v_cache, self.rotary.interleaved)
                 attn = kv4_attention_step(q, k_cache, v_cache, plan, self.scale)
@@ -999,10 +999,10 @@ class MiniTransformer(nn.Module):
         head_dim = hidden_size // num_heads
         self.head_dim = head_dim
         self.kv4 = kv_cache_dtype == 'mxfp4'
-        positions = RotaryPositions(head_dim, **(rotary or {})) if self.kv4 or rotary is not None else None
+        self.rotary = RotaryPositions(head_dim, **(rotary or {})) if self.kv4 or rotary is not None else None
         self.embedding = nn.Embedding(vocab_size, hidden_size)
         self.layers = nn.ModuleList(
-            TransformerLayer(hidden_size, num_heads, intermediate_size, positions) for _ in range(num_layers))
+            TransformerLayer(hidden_size, num_heads, intermediate_size, self.rotary) for _ in range(num_layers))
         self.norm = RMSNorm(hidden_size)
         self.lm_head = nn.Linear(hidden_size, vocab_size, bias=False)
         cache_shape, cache_dtype = (num_layers, num_kv_blocks, block_size, num_heads, head_dim), None
@@ -1052,9 +1052,14 @@ class MiniTransformer(nn.Module):
         """The layer stack for an already planned step; `last` = flattened index of each
         request's final token (None: every token is one, as in a pure decode step)."""
         x, delta = self.embedding(token_ids), None
-        for i, layer in enumerate(self.layers):
-            x, delta = layer.forward_carry(x, delta, positions, (self.k_cache[i], self.v_cache[i]), slot_mapping,
-                                           seq_lens, is_prefill, plan)
+        # (a plan may serve several calls, with other positions or another model: nothing of a call stays in it)
+        plan.angles = None if self.rotary is None else self.rotary.angles(positions)
+        try:
+            for i, layer in enumerate(self.layers):
+                x, delta = layer.forward_carry(x, delta, positions, (self.k_cache[i], self.v_cache[i]), slot_mapping,
+                                               seq_lens, is_prefill, plan)
+        finally:
+            plan.angles = None
         if isinstance(last, torch.Tensor):           # device-side row selection (captured steps)
             x = x.index_select(0, last)
             delta = delta.index_select(0, last) if delta is not None else None
