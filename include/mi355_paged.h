@@ -510,7 +510,7 @@ int mi355_kv4_read_slots(void* k_out, void* v_out, const void* k_cache, const vo
  * context_lens clamped to min(max_context, max_blocks * block_size), 0 gives zeros, ids clamped into
  * the pool) but for the cache's strides.  Scores, softmax and sums are fp32; the cached values and
  * the queries enter the products exactly, the softmax weights with 16 bits for bf16 and fp16 queries
- * and with 24 for fp32 ones.
+ * and with 24 for fp32 ones.  out may be q itself (packed); an out that overlaps q otherwise is refused.
  */
 int mi355_paged_decode_kv4(void* out, const void* q, int64_t q_stride_seq, const void* k_cache,
                            const void* v_cache, const int32_t* block_tables, const int32_t* context_lens,
@@ -528,7 +528,7 @@ size_t mi355_paged_decode_kv4_workspace_bytes(int32_t B, int32_t Hq, int32_t Hkv
  * mi355_paged_prefill over the 4-bit cache: query token j of segment s attends to positions
  * 0 .. seg_pos0[s] + j, whose rows (the segment's own among them) are in the cache.  Rows of out
  * outside every segment are left as they are; a segment may be empty.  A value row that a query must
- * not see never reaches it, NaN or not.  Precision as in mi355_paged_decode_kv4.  total_rows: the tokens
+ * not see never reaches it, NaN or not.  Precision and out as in mi355_paged_decode_kv4.  total_rows: the tokens
  * q and out hold; what a segment has behind them (or behind its first max_q_len) is left out.
  */
 int mi355_paged_prefill_kv4(void* out, const void* q, int64_t q_stride_tok, const void* k_cache,

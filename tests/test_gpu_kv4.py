@@ -897,6 +897,27 @@ def test_chunk_splits_lose_and_double_no_token(ops, device, dtype, seqs, n, Hq, 
     np.testing.assert_array_equal(torch.isnan(out).cpu().numpy(), expect)
 
 
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('seqs,n,Hq,Hkv,D,ctx', [(3, 0, 8, 8, 64, 600), (2, 0, 8, 2, 128, 9000), (40, 0, 40, 2, 64, 300), (2, 37, 8, 2, 64, 500), (1, 9, 8, 2, 128, 6000),
+                                                 (8, 512, 8, 8, 64, 812), (8, 1024, 8, 8, 64, 1024), (4, 512, 32, 8, 128, 600), (9, 250, 8, 8, 256, 600)], ids=str)
+def test_attention_in_place(ops, device, dtype, seqs, n, Hq, Hkv, D, ctx):
+    """out = q: a workgroup has read its query rows before it writes them."""
+    rng = np.random.default_rng(ctx + D)
+    blocks = -(-ctx // 16)
+    kc, vc = (torch.from_numpy(rng.integers(0, 256, ops.kv4_cache_shape(seqs * blocks, Hkv, 16, D), dtype=np.uint8)).cuda() for _ in range(2))
+    kc[..., 8 * D:], vc[..., 8 * D:] = 126, 127
+    tables = torch.arange(seqs * blocks, dtype=torch.int32, device=device).view(seqs, blocks)
+    q = torch.from_numpy(rng.standard_normal((seqs * max(n, 1), Hq, D))).cuda().to(dtype)
+    if n == 0:
+        lens = torch.full((seqs,), ctx, dtype=torch.int32, device=device)
+        call = lambda **kw: ops.paged_decode_kv4(q, kc, vc, tables, lens, ctx, **kw)
+    else:
+        meta = torch.tensor([[i * n for i in range(seqs)], [n] * seqs, [ctx - n] * seqs], dtype=torch.int32, device=device)
+        call = lambda **kw: ops.paged_prefill_kv4(q, kc, vc, tables, meta[0], meta[1], meta[2], n, ctx, **kw)
+    want = call()
+    assert call(out=q) is q and torch.equal(q, want)
+
+
 # ------------------------------------------------------------------ extremes of scores and values
 FORMS = [   # sequences, query rows each (0: decode), Hq, Hkv, D, context: each way rows and contexts are cut up
     (3, 0, 8, 8, 64, 600), (2, 0, 8, 2, 128, 9000), (70, 0, 8, 8, 64, 700), (1, 40, 8, 8, 64, 600), (1, 9, 8, 2, 128, 6000), (8, 512, 8, 8, 64, 812),

@@ -146,6 +146,14 @@ def test_c_entry_points_refuse(name, good, change, want):
     assert name.replace('mi355_', '') in message
 
 
+@pytest.mark.parametrize('name,good', [('mi355_paged_decode_kv4', DECODE), ('mi355_paged_prefill_kv4', CHUNK)])
+@pytest.mark.parametrize('out,qs,dtype', [(P + 1024, 512, 1), (P - 1024, 512, 2), (P, 1536, 1), (P + 512 * 4, 1536, 0), (P + 2048 - 16, 512, 1)])
+def test_outputs_that_overlap_the_queries_are_refused(name, good, out, qs, dtype):
+    rows = dict(B=2) if 'B' in good else dict(rows=2)
+    rc, message = _call(name, good, out=out, qs=qs, dtype=dtype, **rows)
+    assert rc == -1 and 'overlaps' in message
+
+
 @pytest.mark.parametrize('name,good,empty', [
     ('mi355_rope_angles', ANGLES, dict(T=0, cos=None)), ('mi355_rope_rotate', ROTATE, dict(T=0, x=None)),
     ('mi355_rope_kv4_write', WRITE, dict(T=0, q=None, slots=None)), ('mi355_kv4_read_slots', READ, dict(T=0, ko=None)),

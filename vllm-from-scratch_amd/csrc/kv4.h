@@ -56,6 +56,17 @@ static inline Kv4Cache kv4_cache(const void* k, const void* v, int64_t s_blk, in
   return Kv4Cache{static_cast<char*>(const_cast<void*>(k)), static_cast<char*>(const_cast<void*>(v)), s_blk, s_head,
                   num_blocks, tpb, mul, 31 + up};
 }
+// Whether `out` (contiguous) and the span of T rows from x share bytes.
+static inline bool kv4_overlaps(const char* out, int64_t out_bytes, const char* x, int64_t stride, int64_t width, int T) {
+  return out < x + ((int64_t)(T - 1) * stride + width) && x < out + out_bytes;
+}
+// An output of attention may be the query rows themselves (a workgroup reads its own before it writes them), but share no
+// bytes with them otherwise.
+static inline bool kv4_out_ok(const void* out, const void* q, int64_t q_stride, int64_t row, int T, int dtype) {
+  const int64_t eb = dtype == MI355_F32 ? 4 : 2;
+  return (out == q && (q_stride == row || T == 1)) ||
+         !kv4_overlaps(static_cast<const char*>(out), T * row * eb, static_cast<const char*>(q), q_stride * eb, row * eb, T);
+}
 // Checks what every entry point over the cache asks of it; 0 or the recorded error.
 int kv4_check_cache(const char* what, const void* k_cache, const void* v_cache, int Hkv, int D, int block_size,
                     int num_blocks, int64_t s_blk, int64_t s_head);

@@ -375,6 +375,8 @@ extern "C" int mi355_paged_decode_kv4(void* out, const void* q, int64_t q_stride
   const int epl = dtype == MI355_F32 ? 4 : 8;
   if (q_stride_seq % epl || q_stride_seq < (int64_t)Hq * D || (((uintptr_t)q | (uintptr_t)out) & 15))
     return fail(MI355_EINVAL, "paged_decode_kv4: query rows must be 16-byte aligned and a sequence's heads packed");
+  if (!kv4_out_ok(out, q, q_stride_seq, (int64_t)Hq * D, B, dtype))
+    return fail(MI355_EINVAL, "paged_decode_kv4: the output overlaps the query rows without being them");
   if (pl.ws_bytes && (!workspace || workspace_bytes < pl.ws_bytes || ((uintptr_t)workspace & 15)))
     return fail(MI355_EWORKSPACE, "paged_decode_kv4: workspace of %zu bytes needed (16-byte aligned), %zu given", pl.ws_bytes,
                 workspace ? workspace_bytes : (size_t)0);

@@ -384,11 +384,6 @@ int launch_read(ReadParams4& p, int D, hipStream_t s) {
   return two ? launch_read<Tag, 2>(p, D, s) : launch_read<Tag, 1>(p, D, s);
 }
 
-// Whether `out` (contiguous) and the span of rows from x share bytes.
-bool overlaps(const char* out, int64_t out_bytes, const char* x, int64_t stride, int64_t width, int T) {
-  return out < x + ((int64_t)(T - 1) * stride + width) && x < out + out_bytes;
-}
-
 // Query (and, with slots, key / value) rows through kv4_append_kernel.
 int append_impl(const char* what, AppendParams4& p, int T, int D, int rotary_dim, int interleaved, int dtype,
                 hipStream_t s) {
@@ -406,9 +401,9 @@ int append_impl(const char* what, AppendParams4& p, int T, int D, int rotary_dim
                   p.v_stride_tok < (int64_t)p.Hkv * D || (((uintptr_t)p.k | (uintptr_t)p.v) & 15)))
     return fail(MI355_EINVAL, "%s: key / value rows must be 16-byte aligned and a token's heads packed", what);
   const int64_t eb = dtype == MI355_F32 ? 4 : 2, out_bytes = (int64_t)T * p.Hq * D * eb;
-  if (T > 0 && (overlaps(p.q_out, out_bytes, p.q, p.q_stride_tok * eb, p.Hq * D * eb, T) ||
-                (p.slots && (overlaps(p.q_out, out_bytes, p.k, p.k_stride_tok * eb, p.Hkv * D * eb, T) ||
-                             overlaps(p.q_out, out_bytes, p.v, p.v_stride_tok * eb, p.Hkv * D * eb, T)))))
+  if (T > 0 && (kv4_overlaps(p.q_out, out_bytes, p.q, p.q_stride_tok * eb, p.Hq * D * eb, T) ||
+                (p.slots && (kv4_overlaps(p.q_out, out_bytes, p.k, p.k_stride_tok * eb, p.Hkv * D * eb, T) ||
+                             kv4_overlaps(p.q_out, out_bytes, p.v, p.v_stride_tok * eb, p.Hkv * D * eb, T)))))
     return fail(MI355_EINVAL, "%s: the output overlaps the rows it is made from", what);
   if (rotary_dim == 0) p.cos = p.sin = nullptr;
   p.R = rotary_dim;
